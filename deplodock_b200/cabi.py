@@ -73,6 +73,8 @@ _SIGNATURES: dict[str, list] = {
     "emk_set_wait_limit_ms": [c_void_p, c_int],
     "emk_set_launch_overlap": [c_void_p, c_int],
     "emk_rmsnorm": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_int, c_void_p],
+    "emk_rmsnorm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float,
+                         c_int, c_void_p],
     "emk_softmax_lastdim": [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p],
     "emk_linear_bf16": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int,
                         c_void_p],
@@ -107,6 +109,12 @@ _SIGNATURES: dict[str, list] = {
     "emk_sdpa_causal_gqa_bf16_varlen": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                         c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
                                         c_void_p, c_int64, c_void_p],
+    "emk_kv8_append": [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                       c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p],
+    "emk_sdpa_kv8_workspace_bytes": [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64],
+    "emk_sdpa_kv8": [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                     c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64,
+                     c_void_p],
     "emk_pool_norm_l2_varlen": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p],
     "emk_sdpa_simt": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
                       c_int64, c_float, c_int, c_int, c_void_p],
@@ -119,7 +127,8 @@ _SIGNATURES: dict[str, list] = {
 }
 _RESTYPES = {"emk_status_string": c_char_p, "emk_last_error": c_char_p,
              "emk_linear_bf16_w8_workspace_bytes": c_int64, "emk_sdpa_varlen_workspace_bytes": c_int64,
-             "emk_linear_f32_tc_workspace_bytes": c_int64, "emk_gemm_bf16_chain_workspace_bytes": c_int64}
+             "emk_linear_f32_tc_workspace_bytes": c_int64, "emk_gemm_bf16_chain_workspace_bytes": c_int64,
+             "emk_sdpa_kv8_workspace_bytes": c_int64}
 
 #: every symbol ``include/emk.h`` declares; ``tests/test_cabi_symbols.py`` checks the header against this list
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -124,6 +124,8 @@ extern "C" int emk_device_status(emk_handle_t h, emk_stream_t stream) {
       EMK_SET_ERR(h, "out-of-range %s (code %d); the access was clamped or dropped",
                   code == EMK_DEV_BOUNDS_TOKEN_ID ? "token id in the embedding gather"
                   : code == EMK_DEV_BOUNDS_POSITION ? "rotary position"
+                  : code == EMK_DEV_BOUNDS_PAGE ? "page id in a cache's page table"
+                  : code == EMK_DEV_BOUNDS_CACHE_LEN ? "length of a cached sequence"
                   : "sequence in cu_seqlens", code);
       return EMK_ERR_BOUNDS;
     }

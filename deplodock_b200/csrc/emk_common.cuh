@@ -84,7 +84,9 @@ enum {
   // bounds-check build (-DEMK_BOUNDS_CHECK) only: a data-dependent index was outside its range
   EMK_DEV_BOUNDS_TOKEN_ID = 201,   // embedding gather: id outside [0, vocab)
   EMK_DEV_BOUNDS_POSITION = 202,   // rotary position outside the table
-  EMK_DEV_BOUNDS_CU_SEQLENS = 203  // packed attention: a sequence outside the token rows or longer than max_seqlen
+  EMK_DEV_BOUNDS_CU_SEQLENS = 203, // packed attention: a sequence outside the token rows or longer than max_seqlen
+  EMK_DEV_BOUNDS_PAGE = 204,       // 8-bit cache: page id outside the pool
+  EMK_DEV_BOUNDS_CACHE_LEN = 205   // 8-bit cache: a length that the page table's row cannot hold, or a negative one
 };
 
 // The bounds-check build of the library (python -m deplodock_b200.build --bounds-check -> libemk_check.so) stands in

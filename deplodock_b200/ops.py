@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import math
 from ctypes import c_void_p
+from typing import NamedTuple
 
 import torch
 
@@ -62,6 +63,37 @@ def _check_buffer(name: str, t: torch.Tensor | None, numel: int, dtype: torch.dt
         raise ValueError(f"{name} holds {t.numel()} elements, the call needs {numel}")
 
 
+def _cuda_index(*tensors: torch.Tensor | None) -> int:
+    """Index of the one CUDA device that all of ``tensors`` lie on."""
+    idx = -1
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            if not torch.cuda.is_available():
+                raise RuntimeError("deplodock_b200 kernels need a CUDA device (sm_100a); there is no CPU fallback")
+            raise ValueError("expected CUDA tensors")
+        if idx < 0:
+            idx = t.get_device()
+        elif t.get_device() != idx:
+            raise ValueError("expected all tensors on one CUDA device")
+    return idx
+
+
+def _call_on(idx: int, name: str, *args) -> None:
+    """``emk_<name>`` on device ``idx`` (the tensors' own, current or not) and that device's current stream."""
+    h = handle(idx)
+    fn = getattr(h.lib, name)
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if idx == torch.cuda.current_device():
+        rc = fn(h.ptr, *args, stream)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(h.ptr, *args, stream)
+    if rc != cabi.EMK_OK:
+        h.check(rc, name)
+
+
 _DTYPES = {torch.float32: cabi.EMK_F32, torch.bfloat16: cabi.EMK_BF16}
 
 
@@ -89,6 +121,40 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out: torch
     h.check(h.lib.emk_rmsnorm(h.ptr, _ptr(x), _ptr(weight), _ptr(y), rows, cols, float(eps), _dtype_token(x),
                               _stream()), "emk_rmsnorm")
     return y
+
+
+def rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None, *,
+                 out: torch.Tensor | None = None, scale_out: torch.Tensor | None = None,
+                 hidden_out: torch.Tensor | None = None):
+    """RMSNorm over the last axis with an e4m3 output and one fp32 scale per row, ``value = q * scale[row]`` with
+    ``scale = max|y| / 448``: the input of :func:`linear_e4m3`. With ``residual`` (of x's shape and type) the sum
+    ``hidden = x + residual``, rounded to x's type, is normalised and returned too; ``hidden_out`` may be ``x`` or
+    ``residual`` (in place). float32 or bfloat16, any row length. Returns ``(q, scale)`` or ``(q, scale, hidden)``;
+    ``scale`` has the shape of ``x`` without its last axis."""
+    idx = _cuda_index(x, weight, residual, out, scale_out, hidden_out)
+    _check_cuda_contig(x, weight, residual, out, scale_out, hidden_out)
+    dtype = _dtype_token(x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("x needs a last axis of one element at least")
+    cols = x.shape[-1]
+    n = x.numel()
+    if weight.dtype != x.dtype or weight.numel() != cols:
+        raise ValueError("weight must be a vector of the row length with the dtype of x")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+        raise ValueError("residual must have the shape and dtype of x")
+    if hidden_out is not None and residual is None:
+        raise ValueError("hidden_out is the sum of x and residual: give a residual")
+    _check_buffer("out", out, n, torch.float8_e4m3fn)
+    _check_buffer("scale_out", scale_out, n // cols, torch.float32)
+    _check_buffer("hidden_out", hidden_out, n, x.dtype)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn) if out is None else out
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if scale_out is None else scale_out
+    hidden = None if residual is None else torch.empty_like(x) if hidden_out is None else hidden_out
+    if n > 0:
+        _call_on(idx, "emk_rmsnorm_e4m3", x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr(),
+                 q.data_ptr(), scale.data_ptr(), 0 if hidden is None else hidden.data_ptr(), n // cols, cols, float(eps),
+                 dtype)
+    return (q, scale) if hidden is None else (q, scale, hidden)
 
 
 def softmax_lastdim(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -529,6 +595,126 @@ def sdpa_causal_gqa_varlen(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seql
         _ptr(cu_seqlens), B, T, int(max_seqlen), Hq, Hkv, D, ld, ld, ld, Hq * D, float(scale), _ptr(workspace),
         workspace.numel() * workspace.element_size(), _stream()), "emk_sdpa_causal_gqa_bf16_varlen")
     return out
+
+
+class KV8Cache(NamedTuple):
+    """Paged key/value cache in 8 bits: e4m3 codes ``[pages, Hkv, page, D]`` and one fp32 scale per page and KV head
+    ``[pages, Hkv]``; ``value = code * scale``. ``page`` is 16, 32, 64, 128 or 256 tokens, ``D`` 64 or 128. Which pages
+    belong to which sequence is the caller's ``page_table`` (int32 ``[B, max_pages]``)."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv8_cache(num_pages: int, Hkv: int, page: int, D: int = 128, device="cuda") -> KV8Cache:
+    """A zeroed :class:`KV8Cache` of ``num_pages`` pages."""
+    codes = [torch.zeros(num_pages, Hkv, page, D, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in "kv"]
+    scales = [torch.zeros(num_pages, Hkv, dtype=torch.float32, device=device) for _ in "kv"]
+    return KV8Cache(*codes, *scales)
+
+
+def _kv8_sizes(cache: KV8Cache, page_table: torch.Tensor, lens: torch.Tensor) -> tuple[int, int, int, int, int, int]:
+    """Checks a cache, its page table ``[B, max_pages]`` and a length per sequence; (pages, Hkv, page, D, B, max_pages)."""
+    k, v, k_scale, v_scale = cache
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+        raise TypeError("the cache holds float8_e4m3fn codes")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError("the cache's scales are float32")
+    if page_table.dtype != torch.int32 or lens.dtype != torch.int32:
+        raise TypeError("page_table and the sequence lengths must be int32")
+    if k.dim() != 4 or v.shape != k.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+        raise ValueError("cache shapes must be [pages, Hkv, page, D] for the codes and [pages, Hkv] for the scales")
+    if page_table.dim() != 2 or lens.dim() != 1 or lens.shape[0] != page_table.shape[0]:
+        raise ValueError("page_table must be [B, max_pages], the lengths [B]")
+    pages, Hkv, page, D = k.shape
+    return pages, Hkv, page, D, page_table.shape[0], page_table.shape[1]
+
+
+def kv8_append_(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, ctx_lens: torch.Tensor,
+                cu_seqlens: torch.Tensor) -> KV8Cache:
+    """Append keys and values to a paged 8-bit cache, in place (``emk_kv8_append``). ``k``, ``v``: bf16 ``[T, Hkv, D]``,
+    heads contiguous, any row pitch that is a multiple of 8 elements, so views of a fused projection serve; sequence
+    ``b`` holds ``ctx_lens[b]`` tokens and gets the rows ``cu_seqlens[b]:cu_seqlens[b+1]`` (int32 CUDA tensors ``[B]``
+    and ``[B+1]``, left as they are: the caller advances its lengths). No two sequences may write to one page. Scales are
+    powers of two and grow with what a page holds (see ``include/emk.h``)."""
+    idx = _cuda_index(*cache, k, v, page_table, ctx_lens, cu_seqlens)
+    _check_cuda_contig(*cache, page_table, ctx_lens, cu_seqlens)
+    pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, ctx_lens)
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise TypeError("kv8_append_ expects bfloat16 keys and values")
+    if cu_seqlens.dtype != torch.int32:
+        raise TypeError("cu_seqlens must be int32")
+    if k.dim() != 3 or v.shape != k.shape or k.shape[1] != Hkv or k.shape[2] != D:
+        raise ValueError("keys and values must be [T, Hkv, D] with the cache's Hkv and D")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != B + 1:
+        raise ValueError("cu_seqlens must hold B + 1 entries")
+    T = k.shape[0]
+    for t in (k, v):
+        if T > 0 and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D)):
+            raise ValueError("the heads of a token must be contiguous [Hkv, D]")
+    if T > 0 and B > 0:
+        _call_on(idx, "emk_kv8_append", k.data_ptr(), v.data_ptr(), k.stride(0) if T > 1 else Hkv * D,
+                 v.stride(0) if T > 1 else Hkv * D, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                 cache.v_scale.data_ptr(), page_table.data_ptr(), ctx_lens.data_ptr(), cu_seqlens.data_ptr(), B, T,
+                 max_pages, pages, Hkv, page, D)
+    return cache
+
+
+_KV8_WORKSPACE_BYTES: dict[tuple, int] = {}
+
+
+def _sdpa_kv8_workspace_bytes(idx: int, *sizes: int) -> int:
+    n = _KV8_WORKSPACE_BYTES.get((idx, *sizes))
+    if n is None:
+        h = handle(idx)
+        n = _KV8_WORKSPACE_BYTES[(idx, *sizes)] = int(h.lib.emk_sdpa_kv8_workspace_bytes(h.ptr, *sizes))
+    return n
+
+
+def sdpa_kv8_workspace(B: int, Sq: int, Hq: int, cache: KV8Cache, max_pages: int) -> torch.Tensor:
+    """Scratch for :func:`sdpa_kv8` over ``cache`` with a page table of ``max_pages`` columns; it holds nothing between
+    calls. Calls that may run at the same time (two streams, two captured graphs) need one each."""
+    _, Hkv, page, D = cache.k.shape
+    n = _sdpa_kv8_workspace_bytes(cache.k.get_device(), int(B), int(Sq), int(Hq), Hkv, int(max_pages) * page, D)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+
+
+def sdpa_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
+             scale: float | None = None, *, out: torch.Tensor | None = None,
+             workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Grouped-query attention of the last ``Sq`` tokens of every sequence over the paged 8-bit cache
+    (``emk_sdpa_kv8``): the single-token step (``Sq = 1``) and a few draft tokens. ``q``: bf16 ``[B, Sq, Hq, D]``, heads
+    contiguous, any token pitch that is a multiple of 8 elements; ``seq_lens``: int32 CUDA tensor ``[B]``, the cached
+    tokens of each sequence with the ``Sq`` new ones already appended. Query ``i`` sees the tokens up to position
+    ``seq_lens[b] - Sq + i``; one that sees none (an empty or padding sequence) gets zeros. Returns bf16
+    ``[B, Sq, Hq, D]``."""
+    idx = _cuda_index(q, *cache, page_table, seq_lens, out, workspace)
+    _check_cuda_contig(*cache, page_table, seq_lens, out, workspace)
+    pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, seq_lens)
+    if q.dtype != torch.bfloat16:
+        raise TypeError("sdpa_kv8 expects bfloat16 queries")
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] == 0 or Hkv == 0 or q.shape[2] % Hkv != 0:
+        raise ValueError("q must be [B, Sq, Hq, D] with the cache's D and a multiple of its KV heads")
+    if max_pages == 0 or pages == 0:
+        raise ValueError("the page table and the cache must hold a page at least")
+    Sq, Hq = q.shape[1], q.shape[2]
+    _check_buffer("out", out, q.numel(), torch.bfloat16)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    if q.numel() == 0:
+        return o
+    if q.stride(3) != 1 or (Hq > 1 and q.stride(2) != D) or (Sq > 1 and B > 1 and q.stride(0) != Sq * q.stride(1)):
+        raise ValueError("the heads of a query must be contiguous [Hq, D] and its tokens evenly spaced")
+    ld = q.stride(1) if Sq > 1 else q.stride(0) if B > 1 else Hq * D
+    need = _sdpa_kv8_workspace_bytes(idx, B, Sq, Hq, Hkv, max_pages * page, D)
+    if workspace is None:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    _call_on(idx, "emk_sdpa_kv8", q.data_ptr(), ld, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+             cache.v_scale.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), o.data_ptr(), B, Sq, Hq, Hkv, D, page,
+             max_pages, pages, 1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(),
+             workspace.numel() * workspace.element_size())
+    return o
 
 
 def pool_norm_l2_varlen(hidden_states, weight, cu_seqlens: torch.Tensor, eps: float = 1e-6, out=None) -> torch.Tensor:

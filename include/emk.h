@@ -36,8 +36,8 @@ typedef enum {
   EMK_ERR_TIMEOUT = 6,   /* a bounded device-side wait ran out (read back by emk_device_status) */
   EMK_ERR_ARG = 7,       /* null pointer / bad enum                                             */
   EMK_ERR_LIMIT = 8,     /* size beyond a stated fixed maximum of the entry point               */
-  EMK_ERR_BOUNDS = 9     /* bounds-check build only: a token id, rotary position or cu_seqlens entry was out of
-                            range (the access was clamped or dropped); read back by emk_device_status */
+  EMK_ERR_BOUNDS = 9     /* bounds-check build only: a token id, rotary position, cu_seqlens entry, page id or cached
+                            length was out of range (the access was clamped or dropped); read back by emk_device_status */
 } emk_status_t;
 
 /* dtype tokens: same names as the reference's graph dtypes (emmy/compiler/dtype.py:61-69). */
@@ -108,6 +108,16 @@ int emk_rmsnorm(emk_handle_t h, const void* x, const void* w, void* y, int64_t r
  * exactly as torch does. dtype EMK_F32 or EMK_BF16. */
 int emk_softmax_lastdim(emk_handle_t h, const void* x, void* y, int64_t rows, int64_t cols, int dtype,
                         emk_stream_t stream);
+
+/* RMSNorm with the residual's addition and an e4m3 output with one scale per row, for the 8-bit linear layers:
+ *   f = x, or with a residual f = round(x + residual) to `dtype`, stored to hidden (the new residual stream);
+ *   y = f * rsqrt(mean(f^2) + eps) * w in fp32;  scale[row] = max(max |y|, 2^-100) / 448;  q = e4m3(y / scale[row]).
+ * A row with a NaN becomes NaN codes with a NaN scale. x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or
+ * EMK_BF16), residual and hidden both given or both NULL; hidden may be x or residual itself (in place), q may alias
+ * nothing. w: [cols] of `dtype`; q: [rows, cols] e4m3; scale: fp32 [rows]. Any cols; rows of a multiple of 16 bytes at
+ * 16-byte aligned pointers (q 8- or 4-byte) take the vector path. No counterpart in the reference (no 8-bit path). */
+int emk_rmsnorm_e4m3(emk_handle_t h, const void* x, const void* residual, const void* w, void* q, float* scale,
+                     void* hidden, int64_t rows, int64_t cols, float eps, int dtype, emk_stream_t stream);
 
 /* y[M,N] = x[M,K] · W (+ epilogue), bf16 operands, fp32 accumulation in tensor memory, bf16 output.
  * Replaces the emitted k_linear_<hash> kernels (LinearOp/MatmulOp above; TMA ring + mma.sync lowering in
@@ -254,6 +264,38 @@ int emk_sdpa_causal_gqa_bf16_varlen(emk_handle_t h, const void* q, const void* k
                                     int64_t Hq, int64_t Hkv, int64_t D, int64_t ld_q, int64_t ld_k, int64_t ld_v,
                                     int64_t ld_o, float scale, void* workspace, int64_t workspace_bytes,
                                     emk_stream_t stream);
+
+/* Paged key/value cache in 8 bits: codes [num_pages][Hkv][page][D] e4m3 and one fp32 scale per page and KV head
+ * [num_pages][Hkv], for keys and for values, value = code * scale. page_table int32 [B][max_pages] on the device: entry
+ * [b][i] holds the tokens [i * page, (i+1) * page) of sequence b. page: 16, 32, 64, 128 or 256 tokens; D: 64 or 128.
+ * No counterpart in the reference (its serving path keeps no cache).
+ *
+ * emk_kv8_append: sequence b, which holds ctx_lens[b] tokens, gets the rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of k and
+ * v (bf16, T rows of pitch ld_k / ld_v elements, KV head h at column h * D) behind them; ctx_lens int32 [B] and
+ * cu_seqlens int32 [B+1] lie on the device and are left as they are. The scale of a touched page and head becomes the
+ * smallest power of two 2^e, -64 <= e <= 120, with |x| <= 448 * 2^e for every finite appended x, but no smaller than
+ * it was while the page keeps earlier tokens, whose codes are rounded again where it grew. Infinities and NaN become
+ * NaN codes and do not enter the scale. No two sequences may touch the same page in one call. Rows outside every sequence
+ * are not read; tokens that max_pages pages cannot hold, and pages with an id outside [0, num_pages), are dropped.
+ *
+ * emk_sdpa_kv8: o = softmax(scale * q K^T) V over the seq_lens[b] cached tokens of every sequence (int32 [B] on the
+ * device, the Sq queries' own tokens included, already appended); query i sits at position seq_lens[b] - Sq + i and
+ * sees the tokens up to itself; a query that sees none gets zeros. q: bf16, row (b * Sq + i) of pitch ld_q elements,
+ * head h at column h * D; o: bf16 [B * Sq][Hq * D]; Hq a multiple of Hkv. Whatever lies in a page behind a sequence's
+ * last token is not used; scales must not be negative, and a zero value scale makes a page's values zero. Lengths are clamped to what max_pages pages hold, page ids to
+ * the pool. `workspace`: device, 16-byte aligned, emk_sdpa_kv8_workspace_bytes(h, B, Sq, Hq, Hkv, max_pages * page, D)
+ * bytes, not used between calls; calls that may overlap need one each. The first call for a head dimension on a
+ * device sets the kernel's shared-memory attribute: make it before any stream capture. */
+int emk_kv8_append(emk_handle_t h, const void* k, const void* v, int64_t ld_k, int64_t ld_v, void* k_codes,
+                   void* v_codes, float* k_scale, float* v_scale, const int32_t* page_table, const int32_t* ctx_lens,
+                   const int32_t* cu_seqlens, int64_t B, int64_t T, int64_t max_pages, int64_t num_pages, int64_t Hkv,
+                   int64_t page, int64_t D, emk_stream_t stream);
+int64_t emk_sdpa_kv8_workspace_bytes(emk_handle_t h, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv,
+                                     int64_t max_tokens, int64_t D);
+int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const void* k_codes, const void* v_codes,
+                 const float* k_scale, const float* v_scale, const int32_t* page_table, const int32_t* seq_lens, void* o,
+                 int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t page, int64_t max_pages,
+                 int64_t num_pages, float scale, void* workspace, int64_t workspace_bytes, emk_stream_t stream);
 
 /* Pooling for packed sequences: out[b,:] = L2-normalise(RMSNorm(hidden_states[cu_seqlens[b+1]-1, :]; w, eps)), the
  * last token of every sequence (emk_pool_norm_l2 with per-sequence lengths). Empty sequences give zero rows. */
