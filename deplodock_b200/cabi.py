@@ -95,6 +95,7 @@ _SIGNATURES: dict[str, list] = {
     "emk_linear_bf16_w8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
                            c_void_p],
     "emk_linear_bf16_w8_workspace_bytes": [c_int64, c_int64],
+    "emk_linear_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p],
     "emk_elementwise": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p],
     "emk_loop_rope_scores_f32": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                  c_int64, c_float, c_float, c_float, c_void_p],

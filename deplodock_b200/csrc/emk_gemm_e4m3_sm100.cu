@@ -1,0 +1,545 @@
+// e4m3 x e4m3 GEMM on the 5th-generation tensor cores: y[m,n] = bf16(x_scale[m] * w_scale[n] * sum_k x[m,k] * W[n,k]),
+// x [M,K] and W [N,K] e4m3 codes, one fp32 scale per row of each, products exact, sums in fp32 in tensor memory.
+// tcgen05.mma kind::f8f6f4 takes 32 codes (32 bytes) along K per instruction: the shared-memory tiles are the bf16
+// kernels' byte for byte (128-byte rows, 128-byte swizzle), with twice the K in them.
+//
+// Two kernels:
+//   gemm2_e4m3_kernel   many rows: CTA pairs on 256 x 256 tiles, persistent, two accumulators in tensor memory (the
+//                       structure of emk_gemm2_sm100.cu: producer / MMA / eight epilogue warps per CTA). Bound by the
+//                       tensor cores.
+//   gemm_e4m3_rows_kernel   few rows: the operands change places, 128 rows of W are the instruction's M and 16 to 128
+//                       tokens its N, so that no tensor-core row is padding and the grid is cut along W. The K axis is
+//                       split over a cluster's CTAs, whose partial tiles meet in distributed shared memory (a fixed
+//                       order of additions: the same bits on every run, no workspace, no atomics). Bound by reading W.
+#include "emk_gemm_common.cuh"
+
+namespace {
+
+using namespace emk;
+
+constexpr int BKB = 128;  // bytes (= codes) of K per slice: one swizzle row
+
+// Instruction descriptor for kind::f8f6f4, e4m3 operands (format 0), both K-major, fp32 accumulation.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma8_pair_lohi(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(hi), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma8_lohi(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(hi), "r"(accumulate)
+      : "memory");
+}
+
+struct Gemm8Args {
+  __nv_bfloat16* y;
+  const float* x_scale;
+  const float* w_scale;
+  int M, N;
+  int tiles_m, tiles_n, kblocks;  // kblocks: 128-byte slices of K
+  int wide;                       // rows of y are 32-byte aligned
+  int stages;                     // few-rows kernel: ring depth
+  int* status;
+  unsigned long long limit_ns;
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// Many rows: CTA pairs
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int P8_THREADS = 320;  // warps 0-3 and 6-9: epilogue (left / right half of the tile's columns), 4: TMA, 5: MMA
+constexpr int P8_GROUP_M = 8;
+constexpr int P8_BN = 256;
+constexpr int P8_STAGES = 3;
+constexpr int P8_KSUB = 2;
+constexpr int P8_SUB = BM * BKB;                 // one slice of this CTA's 128 rows of x; the W half has as many
+constexpr int P8_OPERAND_STAGE = P8_KSUB * P8_SUB;
+
+struct __align__(8) P8Barriers {
+  uint64_t full[P8_STAGES];
+  uint64_t empty[P8_STAGES];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr int P8_SMEM = P8_STAGES * 2 * P8_OPERAND_STAGE + 1024 + (int)sizeof(P8Barriers);
+
+// 32 accumulator columns [col0, col0 + 32) of output row `row`
+__device__ __forceinline__ void store32_e4m3(const Gemm8Args& g, const uint32_t* r, int row, int col0, float xs) {
+  if (row >= g.M || col0 >= g.N) return;
+  uint32_t o[16];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col0 + q * 4 < g.N) s = __ldg(reinterpret_cast<const float4*>(g.w_scale + col0 + q * 4));  // N is a multiple of 8
+    o[2 * q] = pack_bf16x2(__uint_as_float(r[4 * q]) * xs * s.x, __uint_as_float(r[4 * q + 1]) * xs * s.y);
+    o[2 * q + 1] = pack_bf16x2(__uint_as_float(r[4 * q + 2]) * xs * s.z, __uint_as_float(r[4 * q + 3]) * xs * s.w);
+  }
+  __nv_bfloat16* out = g.y + (int64_t)row * g.N + col0;
+  if (g.wide && col0 + 32 <= g.N) {
+    st_global_v8(out, o);
+    st_global_v8(out + 16, o + 8);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (col0 + q * 8 < g.N)
+        *reinterpret_cast<uint4*>(out + q * 8) = make_uint4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+  }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P8_THREADS, 1)
+gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Gemm8Args g) {
+  constexpr uint32_t STAGE_TX = 2u * (2 * P8_OPERAND_STAGE);  // both CTAs' bytes land on the leader's barrier
+  constexpr uint32_t IDESC = make_idesc_e4m3(2 * BM, P8_BN);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + P8_STAGES * P8_OPERAND_STAGE;
+  P8Barriers* bars = reinterpret_cast<P8Barriers*>(sB + P8_STAGES * P8_OPERAND_STAGE);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1;
+  const int npairs = gridDim.x >> 1;
+  const int ntiles = g.tiles_m * g.tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < P8_STAGES; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->tmem_full[i], 1);
+      mbar_init(&bars->tmem_empty[i], 16);  // 8 epilogue warps of each CTA
+    }
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&tma_a);
+    tma_prefetch_desc(&tma_b);
+  }
+  if (warp == 0) {
+    tmem_alloc_pair(&bars->tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+  const WaitCtx wc{&bars->abort_flag, g.status, g.limit_ns};
+
+  if (warp == 4) {
+    if (lane == 0) {  // TMA producer (both CTAs)
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+        int tm, tn;
+        tile_coords(tile, g.tiles_m, g.tiles_n, P8_GROUP_M, tm, tn);
+        const int m0 = tm * 2 * BM + (int)rank * BM;
+        const int n0 = tn * P8_BN + (int)rank * (P8_BN / 2);
+        for (int kb = 0; kb < g.kblocks; kb += P8_KSUB) {
+          if (!mbar_wait(&bars->empty[stage], phase ^ 1u, wc, EMK_DEV_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full_leader = mapa_u32(smem_u32(&bars->full[stage]), 0);
+          if (leader) mbar_arrive_expect_tx(&bars->full[stage], STAGE_TX);
+#pragma unroll
+          for (int u = 0; u < P8_KSUB; ++u) {  // slices past K are zero-filled by TMA and add nothing
+            const int k0 = (kb + u) * BKB;
+            tma_load_2d_pair(sA + stage * P8_OPERAND_STAGE + u * P8_SUB, &tma_a, full_leader, k0, m0);
+            tma_load_2d_pair(sB + stage * P8_OPERAND_STAGE + u * P8_SUB, &tma_b, full_leader, k0, n0);
+          }
+          if (++stage == P8_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 5) {
+    if (leader && lane == 0) {  // MMA issuer
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      const uint32_t desc_hi = smem_desc_hi(1024);
+      const uint32_t a_lo0 = smem_desc_lo(smem_u32(sA), 0);
+      const uint32_t b_lo0 = smem_desc_lo(smem_u32(sB), 0);
+      for (int tile = pair; tile < ntiles && ok; tile += npairs, ++local) {
+        const int acc = local & 1;
+        const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
+        if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, wc, EMK_DEV_TIMEOUT_MMA)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * P8_BN);
+        for (int kb = 0; kb < g.kblocks; kb += P8_KSUB) {
+          if (!mbar_wait(&bars->full[stage], phase, wc, EMK_DEV_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          const uint32_t a_st = a_lo0 + (uint32_t)(stage * (P8_OPERAND_STAGE >> 4));
+          const uint32_t b_st = b_lo0 + (uint32_t)(stage * (P8_OPERAND_STAGE >> 4));
+#pragma unroll
+          for (int u = 0; u < P8_KSUB; ++u) {
+#pragma unroll
+            for (int k = 0; k < BKB / 32; ++k) {
+              const uint32_t off = (uint32_t)((u * P8_SUB + k * 32) >> 4);
+              umma8_pair_lohi(d_tmem, a_st + off, b_st + off, desc_hi, IDESC, (u | k) != 0 ? 1u : (uint32_t)(kb != 0));
+            }
+          }
+          const uint32_t e_local = smem_u32(&bars->empty[stage]);
+          tc_commit_pair(e_local);
+          tc_commit_pair(mapa_u32(e_local, 1));
+          if (++stage == P8_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) {
+          const uint32_t f_local = smem_u32(&bars->tmem_full[acc]);
+          tc_commit_pair(f_local);
+          tc_commit_pair(mapa_u32(f_local, 1));
+        }
+      }
+    }
+  } else {
+    // epilogue: warps 0..3 the left half of the columns, 6..9 the right half; a warp may only touch the tensor-memory
+    // lanes of its quarter (warp_id % 4)
+    const int quarter = warp & 3;
+    const int half = warp >= 6 ? 1 : 0;
+    int local = 0;
+    for (int tile = pair; tile < ntiles; tile += npairs, ++local) {
+      const int acc = local & 1;
+      const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
+      int tm, tn;
+      tile_coords(tile, g.tiles_m, g.tiles_n, P8_GROUP_M, tm, tn);
+      const int row = tm * 2 * BM + (int)rank * BM + quarter * 32 + lane;
+      const int n0 = tn * P8_BN + half * (P8_BN / 2);
+      const float xs = row < g.M ? __ldg(g.x_scale + row) : 0.f;
+      if (!mbar_wait_warp(&bars->tmem_full[acc], acc_phase, wc, EMK_DEV_TIMEOUT_EPILOGUE)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * P8_BN + half * (P8_BN / 2));
+      uint32_t r[2][32];
+      tmem_ld_x32(taddr, r[0]);
+#pragma unroll
+      for (int c = 0; c < P8_BN / 64; ++c) {
+        tmem_ld_wait_regs(r[c & 1]);
+        if (c + 1 < P8_BN / 64) tmem_ld_x32(taddr + (uint32_t)((c + 1) * 32), r[(c + 1) & 1]);
+        store32_e4m3(g, r[c & 1], row, n0 + c * 32, xs);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&bars->tmem_empty[acc]), 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (bars->abort_flag) abort_drain();
+  cluster_sync_all();  // the peer's shared and tensor memory stay alive until the leader's MMAs are done
+  if (warp == 0) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows: W rows along the instruction's M, tokens along its N, K split over the cluster
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int R8_THREADS = 192;  // warps 0-3: epilogue, 4: TMA, 5: MMA
+constexpr int R8_MAX_STAGES = 12;
+constexpr int R8_MAX_SPLIT = 8;  // portable cluster size
+constexpr int R8_W_STAGE = BM * BKB;
+
+struct __align__(8) R8Barriers {
+  uint64_t full[R8_MAX_STAGES];
+  uint64_t empty[R8_MAX_STAGES];
+  uint64_t tmem_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ uint32_t cluster_size_x() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+template <int NT>  // tokens per tile
+__global__ void __launch_bounds__(R8_THREADS)
+gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x, const Gemm8Args g) {
+  constexpr int X_STAGE = NT * BKB;
+  constexpr int STAGE = R8_W_STAGE + X_STAGE;
+  constexpr uint32_t TMEM_COLS = NT < 32 ? 32 : NT;
+  constexpr uint32_t IDESC = make_idesc_e4m3(BM, NT);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t split = cluster_size_x();
+  const uint32_t rank = cluster_ctarank();
+  // [split][NT / split][128] partial sums of this CTA's share of the tokens, written by all CTAs of the cluster
+  float* red = reinterpret_cast<float*>(ring + g.stages * STAGE);
+  R8Barriers* bars = reinterpret_cast<R8Barriers*>(reinterpret_cast<uint8_t*>(red) + (split > 1 ? NT * BM * 4 : 0));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int tile = blockIdx.x / split;
+  const int tn = tile % g.tiles_n, tm = tile / g.tiles_n;
+  const int kb0 = (int)((int64_t)g.kblocks * rank / split), kb1 = (int)((int64_t)g.kblocks * (rank + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < g.stages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    mbar_init(&bars->tmem_full, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&tma_w);
+    tma_prefetch_desc(&tma_x);
+  }
+  if (warp == 0) {
+    tmem_alloc(&bars->tmem_base, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();  // every CTA of the cluster runs before any writes to its shared memory
+  tc_fence_after();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+  const WaitCtx wc{&bars->abort_flag, g.status, g.limit_ns};
+  bool done = false;  // epilogue warps: the accumulator is complete
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&bars->empty[stage], phase ^ 1u, wc, EMK_DEV_TIMEOUT_PRODUCER)) break;
+        mbar_arrive_expect_tx(&bars->full[stage], STAGE);
+        tma_load_2d(ring + stage * STAGE, &tma_w, &bars->full[stage], kb * BKB, tn * BM);
+        tma_load_2d(ring + stage * STAGE + R8_W_STAGE, &tma_x, &bars->full[stage], kb * BKB, tm * NT);
+        if (++stage == g.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t desc_hi = smem_desc_hi(1024);
+      const uint32_t lo0 = smem_desc_lo(smem_u32(ring), 0);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&bars->full[stage], phase, wc, EMK_DEV_TIMEOUT_MMA)) {
+          ok = false;
+          break;
+        }
+        const uint32_t w_lo = lo0 + (uint32_t)(stage * (STAGE >> 4));
+        const uint32_t x_lo = w_lo + (uint32_t)(R8_W_STAGE >> 4);
+#pragma unroll
+        for (int k = 0; k < BKB / 32; ++k)
+          umma8_lohi(tmem_base, w_lo + (uint32_t)(k * 2), x_lo + (uint32_t)(k * 2), desc_hi, IDESC,
+                     k != 0 ? 1u : (uint32_t)(kb != kb0));
+        tc_commit(&bars->empty[stage]);
+        if (++stage == g.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) tc_commit(&bars->tmem_full);
+    }
+    __syncwarp();
+  } else {
+    done = mbar_wait_warp(&bars->tmem_full, 0, wc, EMK_DEV_TIMEOUT_EPILOGUE);
+    if (done) {
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(warp * 32) << 16);
+      const int n = tn * BM + warp * 32 + lane;
+      const int t0 = tm * NT;
+      const float ws = n < g.N ? __ldg(g.w_scale + n) : 0.f;
+#pragma unroll
+      for (int c = 0; c < NT / 16; ++c) {
+        uint32_t r[16];
+        tmem_ld_x16(taddr + (uint32_t)(c * 16), r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int tok = c * 16 + i;
+          if (t0 + tok < g.M) {  // uniform over the warp
+            const float v = __uint_as_float(r[i]);
+            if (split == 1) {
+              if (n < g.N) g.y[(int64_t)(t0 + tok) * g.N + n] = __float2bfloat16_rn(v * __ldg(g.x_scale + t0 + tok) * ws);
+            } else {
+              // token `tok` belongs to CTA tok / (NT / split), which keeps a plane per source rank
+              const uint32_t per = NT / split;
+              const uint32_t at = smem_u32(red + (rank * per + (uint32_t)tok % per) * BM + warp * 32 + lane);
+              st_cluster_f32(mapa_u32(at, (uint32_t)tok / per), v);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  __syncthreads();
+  if (bars->abort_flag) abort_drain();
+  if (split > 1) {
+    cluster_sync_all();  // reached by every thread of every CTA, whatever happened above
+    if (warp < 4 && done) {
+      const uint32_t per = NT / split;
+      const int n = tn * BM + warp * 32 + lane;
+      const float ws = n < g.N ? __ldg(g.w_scale + n) : 0.f;
+      for (uint32_t i = 0; i < per; ++i) {
+        const int tok = tm * NT + (int)(rank * per + i);
+        if (tok >= g.M) break;
+        float v = 0.f;
+        for (uint32_t s = 0; s < split; ++s) v += red[(s * per + i) * BM + warp * 32 + lane];
+        if (n < g.N) g.y[(int64_t)tok * g.N + n] = __float2bfloat16_rn(v * __ldg(g.x_scale + tok) * ws);
+      }
+    }
+  }
+  if (warp == 0) tmem_dealloc(tmem_base, TMEM_COLS);
+}
+
+constexpr int rows_smem(int nt, int stages, int split) {
+  return stages * (R8_W_STAGE + nt * BKB) + (split > 1 ? nt * BM * 4 : 0) + 1024 + (int)sizeof(R8Barriers);
+}
+
+template <int NT>
+int launch_rows(emk_handle_t h, const CUtensorMap& tw, const CUtensorMap& tx, Gemm8Args g, int split, cudaStream_t s) {
+  constexpr int BUDGET = NT == 128 ? 220 * 1024 : 110 * 1024;  // one CTA per SM at 128 tokens, else two
+  const int room = (BUDGET - rows_smem(NT, 0, split)) / (R8_W_STAGE + NT * BKB);
+  const int want = (g.kblocks + split - 1) / split;
+  g.stages = want < room ? want : room;
+  if (g.stages > R8_MAX_STAGES) g.stages = R8_MAX_STAGES;
+  const int smem = rows_smem(NT, g.stages, split);
+  static emk_device_once once;
+  {
+    std::lock_guard<std::mutex> lk(once.mu);
+    if (!once.done[h->device]) {
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(gemm_e4m3_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, BUDGET));
+      once.done[h->device] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(g.tiles_m * g.tiles_n * split), 1, 1);
+  cfg.blockDim = dim3(R8_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = h->overlap_launch != 0 ? 2 : 1;
+  EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, gemm_e4m3_rows_kernel<NT>, tw, tx, g));
+  EMK_LAUNCH_CHECK(h);
+  return EMK_OK;
+}
+
+int linear_rows(emk_handle_t h, const void* x, const void* w, Gemm8Args g, int64_t K, cudaStream_t s) {
+  const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
+  g.tiles_m = (g.M + nt - 1) / nt;
+  g.tiles_n = (g.N + BM - 1) / BM;
+  // Split K until two CTAs per SM have work, each at least two slices.
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  int split = 1;
+  while (split < R8_MAX_SPLIT && tiles * split * 2 <= 2 * (int64_t)h->sm_count && g.kblocks >= split * 4) split *= 2;
+  CUtensorMap tw, tx;
+  int rc = emk_make_tmap_2d(h, &tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (uint64_t)K, (uint64_t)g.N, (uint64_t)K, BKB, BM,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != EMK_OK) return rc;
+  rc = emk_make_tmap_2d(h, &tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)K, (uint64_t)g.M, (uint64_t)K, BKB,
+                        (uint32_t)nt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != EMK_OK) return rc;
+  switch (nt) {
+    case 16: return launch_rows<16>(h, tw, tx, g, split, s);
+    case 32: return launch_rows<32>(h, tw, tx, g, split, s);
+    case 64: return launch_rows<64>(h, tw, tx, g, split, s);
+    default: return launch_rows<128>(h, tw, tx, g, split, s);
+  }
+}
+
+int linear_pairs(emk_handle_t h, const void* x, const void* w, Gemm8Args g, int64_t K, cudaStream_t s) {
+  g.tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
+  g.tiles_n = (g.N + P8_BN - 1) / P8_BN;
+  CUtensorMap ta, tb;
+  int rc = emk_make_tmap_2d(h, &ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)K, (uint64_t)g.M, (uint64_t)K, BKB, BM,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != EMK_OK) return rc;
+  rc = emk_make_tmap_2d(h, &tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (uint64_t)K, (uint64_t)g.N, (uint64_t)K, BKB, BM,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != EMK_OK) return rc;
+  static emk_device_once once;
+  {
+    std::lock_guard<std::mutex> lk(once.mu);
+    if (!once.done[h->device]) {
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(gemm2_e4m3_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM));
+      once.done[h->device] = true;
+    }
+  }
+  const int ntiles = g.tiles_m * g.tiles_n;
+  const int pairs = ntiles < h->sm_count / 2 ? ntiles : h->sm_count / 2;
+  EMK_CUDA_TRY(h, launch_after_prologue(gemm2_e4m3_kernel, 2u * (unsigned)pairs, P8_THREADS, P8_SMEM, s,
+                                        h->overlap_launch != 0, ta, tb, g));
+  EMK_LAUNCH_CHECK(h);
+  return EMK_OK;
+}
+
+}  // namespace
+
+extern "C" int emk_linear_e4m3(emk_handle_t h, const void* x, const float* x_scale, const void* w, const float* w_scale,
+                               void* y, int64_t M, int64_t N, int64_t K, emk_stream_t stream) {
+  if (!h || !x || !x_scale || !w || !w_scale || !y) return EMK_ERR_ARG;
+  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff) return EMK_ERR_SHAPE;
+  if ((K % 16) != 0 || (N % 8) != 0) {
+    EMK_SET_ERR(h, "emk_linear_e4m3: K must be a multiple of 16 and N of 8; got K=%lld N=%lld", (long long)K, (long long)N);
+    return EMK_ERR_ALIGN;
+  }
+  if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)w_scale) & 15u) != 0 || ((uintptr_t)x_scale & 3u) != 0)
+    return EMK_ERR_ALIGN;
+  if ((M + 15) / 16 * ((N + 127) / 128) > (1 << 28)) {
+    EMK_SET_ERR(h, "emk_linear_e4m3: output of %lld x %lld is too large for one launch", (long long)M, (long long)N);
+    return EMK_ERR_LIMIT;
+  }
+  Gemm8Args g = {};
+  g.y = (__nv_bfloat16*)y;
+  g.x_scale = x_scale;
+  g.w_scale = w_scale;
+  g.M = (int)M;
+  g.N = (int)N;
+  g.kblocks = (int)((K + BKB - 1) / BKB);
+  g.wide = ((N % 16) == 0 && ((uintptr_t)y & 31u) == 0) ? 1 : 0;
+  g.status = h->status_dev;
+  g.limit_ns = h->wait_limit_ns;
+  return M <= 256 ? linear_rows(h, x, w, g, K, (cudaStream_t)stream) : linear_pairs(h, x, w, g, K, (cudaStream_t)stream);
+}

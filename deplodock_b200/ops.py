@@ -522,6 +522,31 @@ def linear_w8(x: torch.Tensor, w_e4m3: torch.Tensor, scale: torch.Tensor, out=No
     return y
 
 
+def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """LinearOp on 8-bit operands: e4m3 activations ``[..., K]`` with one fp32 scale per row (what :func:`rmsnorm_e4m3`
+    returns) times e4m3 weights ``[N, K]`` with one fp32 scale per output channel (those of :func:`linear_w8`), bf16 out.
+    K must be a multiple of 16, N of 8."""
+    idx = _cuda_index(x, x_scale, w, w_scale, out)
+    _check_cuda_contig(x, x_scale, w, w_scale, out)
+    if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
+        raise TypeError("linear_e4m3 expects float8_e4m3fn activations and weights")
+    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise TypeError("linear_e4m3 expects float32 scales")
+    if x.dim() == 0 or w.dim() != 2 or x.shape[-1] != w.shape[1] or x.shape[-1] == 0:
+        raise ValueError("weight [N,K] does not match x")
+    N, K = w.shape
+    M = x.numel() // K
+    if x_scale.numel() != M or w_scale.numel() != N:
+        raise ValueError("x_scale must hold a value per row of x, w_scale one per row of w")
+    _check_buffer("out", out, M * N, torch.bfloat16)
+    y = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device) if out is None else out
+    if M > 0:
+        _call_on(idx, "emk_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), y.data_ptr(), M,
+                 N, K)
+    return y
+
+
 def sdpa_causal_gqa(q, k, v, scale: float | None = None, out=None) -> torch.Tensor:
     """SdpaOp(is_causal=True) with grouped KV heads (``ir/frontend/ir.py:241-275``); q ``[B,Hq,S,128]``, k/v
     ``[B,Hkv,S,128]`` bf16, on the tcgen05 flash kernel."""

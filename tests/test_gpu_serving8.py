@@ -130,6 +130,90 @@ def test_rmsnorm_e4m3_refusals(ops):
 
 
 # ------------------------------------------------------------------------------------------------------------
+# e4m3 linear
+# ------------------------------------------------------------------------------------------------------------
+def _codes(g, rows, cols):
+    return (torch.randn(rows, cols, generator=g) * 60).clamp(-448, 448).to(E4M3)
+
+
+def _linear_check(got, x, xs, w, ws):
+    a, b = x.double() * xs.double()[:, None], w.double() * ws.double()[:, None]
+    want, mass = a @ b.T, a.abs() @ b.abs().T
+    # fp32 sums of exact products: the tensor core adds 32 at a time, each addition truncating
+    tol = want.abs() * 2.0 ** -8 + mass * (x.shape[1] / 32 + 40) * 2.0 ** -23
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol).all(), float((err / tol.clamp_min(1e-300)).max())
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 64, 65, 128, 129, 200, 256, 257, 300, 511, 1000])
+@pytest.mark.parametrize("N,K", [(8, 16), (136, 1040), (1000, 528), (520, 2048)])
+def test_linear_e4m3(ops, M, N, K):
+    g = _gen(M * 1000 + N + K)
+    x, w = _codes(g, M, K), _codes(g, N, K)
+    xs, ws = torch.rand(M, generator=g) * 0.01, torch.rand(N, generator=g) * 0.001
+    got = ops.linear_e4m3(x.cuda(), xs.cuda(), w.cuda(), ws.cuda())
+    ops.device_status()
+    assert got.shape == (M, N) and got.dtype == torch.bfloat16
+    _linear_check(got, x, xs, w, ws)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 6144, 2048), (9, 40000, 256), (40, 256, 16384), (100, 4096, 1024), (513, 2048, 4096)])
+def test_linear_e4m3_larger(ops, M, N, K):
+    g = _gen(M + N + K)
+    x, w = _codes(g, M, K), _codes(g, N, K)
+    xs, ws = torch.rand(M, generator=g) * 0.01, torch.rand(N, generator=g) * 0.001
+    args = [t.cuda() for t in (x, xs, w, ws)]
+    got = ops.linear_e4m3(*args)
+    _linear_check(got, x, xs, w, ws)
+    for _ in range(3):
+        assert torch.equal(ops.linear_e4m3(*args), got)  # the same bits every time
+
+
+@pytest.mark.parametrize("M", [3, 100, 300])
+def test_linear_e4m3_leaves_what_is_not_its_own(ops, M):
+    N, K = 264, 144
+    g = _gen(M)
+    x, w = _codes(g, M, K), _codes(g, N, K)
+    xs, ws = torch.rand(M, generator=g), torch.rand(N, generator=g)
+    buf = torch.full((M * N + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert ops.linear_e4m3(x.cuda(), xs.cuda(), w.cuda(), ws.cuda(), out=buf) is buf
+    assert (buf[M * N:] == 7.0).all()
+    _linear_check(buf[:M * N].view(M, N), x, xs, w, ws)
+
+
+@pytest.mark.parametrize("M", [4, 130, 400])
+def test_linear_e4m3_nan_codes_stay_in_their_row_and_column(ops, M):
+    N, K = 256, 256
+    g = _gen(M + 1)
+    x, w = _codes(g, M, K), _codes(g, N, K)
+    x.view(torch.uint8)[2, 100] = 0x7f
+    w.view(torch.uint8)[9, 30] = 0xff
+    ones = torch.ones(max(M, N)).cuda()
+    nan = torch.isnan(ops.linear_e4m3(x.cuda(), ones[:M], w.cuda(), ones[:N])).cpu()
+    want = torch.zeros(M, N, dtype=torch.bool)
+    want[2], want[:, 9] = True, True
+    assert torch.equal(nan, want)
+
+
+def test_linear_e4m3_refusals_and_empty(ops):
+    g = _gen(1)
+    x, w = _codes(g, 4, 32).cuda(), _codes(g, 16, 32).cuda()
+    xs, ws = torch.ones(4, device="cuda"), torch.ones(16, device="cuda")
+    for f in (lambda: ops.linear_e4m3(x, xs[:3], w, ws), lambda: ops.linear_e4m3(x, xs, w, ws[:8]),
+              lambda: ops.linear_e4m3(x, xs, w[:, :16].contiguous(), ws), lambda: ops.linear_e4m3(x, xs, w[:12], ws[:12]),
+              lambda: ops.linear_e4m3(_codes(g, 4, 24).cuda(), xs, _codes(g, 16, 24).cuda(), ws),
+              lambda: ops.linear_e4m3(x, xs, w, ws, out=torch.empty(4, 15, dtype=torch.bfloat16, device="cuda")),
+              lambda: ops.linear_e4m3(x[:, ::2], xs, w[:, ::2], ws), lambda: ops.linear_e4m3(x.cpu(), xs, w, ws)):
+        with pytest.raises(ValueError):
+            f()
+    for f in (lambda: ops.linear_e4m3(x.float(), xs, w, ws), lambda: ops.linear_e4m3(x, xs.double(), w, ws)):
+        with pytest.raises(TypeError):
+            f()
+    assert ops.linear_e4m3(x[:0], xs[:0], w, ws).shape == (0, 16)
+    assert ops.linear_e4m3(x.view(2, 2, 32), xs.view(2, 2), w, ws).shape == (2, 2, 16)
+
+
+# ------------------------------------------------------------------------------------------------------------
 # the paged 8-bit cache: append
 # ------------------------------------------------------------------------------------------------------------
 def _pow2_scale(amax: float) -> float:

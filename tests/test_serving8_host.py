@@ -93,6 +93,20 @@ def test_rmsnorm_refuses(lib, fake_handle, kw, want):
     assert _norm(lib, None) == cabi.EMK_ERR_ARG
 
 
+@pytest.mark.parametrize("kw,want", [
+    (dict(x=0), "ARG"), (dict(xs=0), "ARG"), (dict(M=0), "SHAPE"), (dict(N=0), "SHAPE"), (dict(K=0), "SHAPE"),
+    (dict(M=1 << 31), "SHAPE"), (dict(K=24), "ALIGN"), (dict(N=12), "ALIGN"), (dict(x=P + 8), "ALIGN"), (dict(ws=P + 4), "ALIGN"),
+    (dict(xs=P + 2), "ALIGN"), (dict(M=1 << 30, N=1 << 30), "LIMIT")])
+def test_linear_refuses(lib, fake_handle, kw, want):
+    from deplodock_b200 import cabi
+
+    a = dict(x=P, xs=P, w=P, ws=P, y=P, M=2, N=16, K=32)
+    a.update(kw)
+    args = (a["x"], a["xs"], a["w"], a["ws"], a["y"], a["M"], a["N"], a["K"], None)
+    assert lib.emk_linear_e4m3(fake_handle, *args) == getattr(cabi, f"EMK_ERR_{want}")
+    assert lib.emk_linear_e4m3(None, *args) == cabi.EMK_ERR_ARG
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the message of a machine without a GPU")
 def test_no_cpu_fallback():
     from deplodock_b200 import ops
