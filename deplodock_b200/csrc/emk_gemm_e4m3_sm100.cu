@@ -279,8 +279,10 @@ __device__ __forceinline__ uint32_t cluster_size_x() {
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 
 template <int NT>  // tokens per tile
@@ -294,9 +296,8 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t split = cluster_size_x();
   const uint32_t rank = cluster_ctarank();
-  // [split][NT / split][128] partial sums of this CTA's share of the tokens, written by all CTAs of the cluster
-  float* red = reinterpret_cast<float*>(ring + g.stages * STAGE);
-  R8Barriers* bars = reinterpret_cast<R8Barriers*>(reinterpret_cast<uint8_t*>(red) + (split > 1 ? NT * BM * 4 : 0));
+  float* part = reinterpret_cast<float*>(ring);  // [NT][128] partial sums, once the ring is done with
+  R8Barriers* bars = reinterpret_cast<R8Barriers*>(ring + max(g.stages * STAGE, NT * BM * 4));
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -323,14 +324,11 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   }
   tc_fence_before();
   __syncthreads();
-  if (split > 1) cluster_sync_all();  // every CTA of the cluster runs before any writes to its shared memory
   tc_fence_after();
   grid_dependency_wait();
   grid_launch_dependents();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
   const WaitCtx wc{&bars->abort_flag, g.status, g.limit_ns};
-  bool done = false;  // epilogue warps: the accumulator is complete
-
   if (warp == 4) {
     if (lane == 0) {
       int stage = 0;
@@ -375,70 +373,69 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
     }
     __syncwarp();
   } else {
-    done = mbar_wait_warp(&bars->tmem_full, 0, wc, EMK_DEV_TIMEOUT_EPILOGUE);
-    if (done) {
+    // the partial tile goes to shared memory, token-major, over the ring: every MMA that read it has finished
+    if (mbar_wait_warp(&bars->tmem_full, 0, wc, EMK_DEV_TIMEOUT_EPILOGUE)) {
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(warp * 32) << 16);
-      const int n = tn * BM + warp * 32 + lane;
-      const int t0 = tm * NT;
-      const float ws = n < g.N ? __ldg(g.w_scale + n) : 0.f;
 #pragma unroll
       for (int c = 0; c < NT / 16; ++c) {
         uint32_t r[16];
         tmem_ld_x16(taddr + (uint32_t)(c * 16), r);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int tok = c * 16 + i;
-          if (t0 + tok < g.M) {  // uniform over the warp
-            const float v = __uint_as_float(r[i]);
-            if (split == 1) {
-              if (n < g.N) g.y[(int64_t)(t0 + tok) * g.N + n] = __float2bfloat16_rn(v * __ldg(g.x_scale + t0 + tok) * ws);
-            } else {
-              // token `tok` belongs to CTA tok / (NT / split), which keeps a plane per source rank
-              const uint32_t per = NT / split;
-              const uint32_t at = smem_u32(red + (rank * per + (uint32_t)tok % per) * BM + warp * 32 + lane);
-              st_cluster_f32(mapa_u32(at, (uint32_t)tok / per), v);
-            }
-          }
-        }
+        for (int i = 0; i < 16; ++i) part[(c * 16 + i) * BM + warp * 32 + lane] = __uint_as_float(r[i]);
       }
       tc_fence_before();
     }
   }
 
   __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem_base, TMEM_COLS);
   if (bars->abort_flag) abort_drain();
-  if (split > 1) {
-    cluster_sync_all();  // reached by every thread of every CTA, whatever happened above
-    if (warp < 4 && done) {
-      const uint32_t per = NT / split;
-      const int n = tn * BM + warp * 32 + lane;
-      const float ws = n < g.N ? __ldg(g.w_scale + n) : 0.f;
-      for (uint32_t i = 0; i < per; ++i) {
-        const int tok = tm * NT + (int)(rank * per + i);
-        if (tok >= g.M) break;
-        float v = 0.f;
-        for (uint32_t s = 0; s < split; ++s) v += red[(s * per + i) * BM + warp * 32 + lane];
-        if (n < g.N) g.y[(int64_t)tok * g.N + n] = __float2bfloat16_rn(v * __ldg(g.x_scale + tok) * ws);
-      }
+  if (split > 1) cluster_sync_all();  // (reached by every thread of every CTA, whatever happened above)
+  // CTA `rank` finishes the tokens rank, rank + split, ...: a warp takes a token's 128 columns, four per lane, and adds
+  // the cluster's partial sums in the order of the ranks
+  const int n = tn * BM + lane * 4;
+  if (n < g.N && bars->abort_flag == 0) {
+    const float4 ws = __ldg(reinterpret_cast<const float4*>(g.w_scale + n));
+    const uint32_t at = smem_u32(part) + (uint32_t)lane * 16u;
+    const int tokens = min(NT, g.M - tm * NT);
+    for (int tok = (int)rank + (int)split * warp; tok < tokens; tok += (int)split * (R8_THREADS / 32)) {
+      const float xs = __ldg(g.x_scale + tm * NT + tok);
+      float4 v[R8_MAX_SPLIT];
+#pragma unroll
+      for (uint32_t s = 0; s < R8_MAX_SPLIT; ++s)
+        if (s < split) v[s] = ld_cluster_f32x4(mapa_u32(at + (uint32_t)tok * (BM * 4), s));
+#pragma unroll
+      for (uint32_t s = 1; s < R8_MAX_SPLIT; ++s)
+        if (s < split) {
+          v[0].x += v[s].x;
+          v[0].y += v[s].y;
+          v[0].z += v[s].z;
+          v[0].w += v[s].w;
+        }
+      *reinterpret_cast<uint2*>(g.y + (int64_t)(tm * NT + tok) * g.N + n) =
+          make_uint2(pack_bf16x2(v[0].x * xs * ws.x, v[0].y * xs * ws.y), pack_bf16x2(v[0].z * xs * ws.z, v[0].w * xs * ws.w));
     }
   }
-  if (warp == 0) tmem_dealloc(tmem_base, TMEM_COLS);
+  __syncwarp();
+  if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-constexpr int rows_smem(int nt, int stages, int split) {
-  return stages * (R8_W_STAGE + nt * BKB) + (split > 1 ? nt * BM * 4 : 0) + 1024 + (int)sizeof(R8Barriers);
+constexpr int rows_smem(int nt, int stages) {
+  const int ring = stages * (R8_W_STAGE + nt * BKB), part = nt * BM * 4;
+  return (ring > part ? ring : part) + 1024 + (int)sizeof(R8Barriers);
 }
 
 template <int NT>
 int launch_rows(emk_handle_t h, const CUtensorMap& tw, const CUtensorMap& tx, Gemm8Args g, int split, cudaStream_t s) {
-  constexpr int BUDGET = NT == 128 ? 220 * 1024 : 110 * 1024;  // one CTA per SM at 128 tokens, else two
-  const int room = (BUDGET - rows_smem(NT, 0, split)) / (R8_W_STAGE + NT * BKB);
+  constexpr int BUDGET = 110 * 1024;  // two CTAs per SM
+  constexpr int ROOM = (BUDGET - 1024 - (int)sizeof(R8Barriers)) / (R8_W_STAGE + NT * BKB);
+  static_assert(ROOM >= 3 && rows_smem(NT, 1) <= BUDGET, "a ring of three stages");
   const int want = (g.kblocks + split - 1) / split;
-  g.stages = want < room ? want : room;
+  g.stages = want < ROOM ? want : ROOM;
   if (g.stages > R8_MAX_STAGES) g.stages = R8_MAX_STAGES;
-  const int smem = rows_smem(NT, g.stages, split);
+  const int smem = rows_smem(NT, g.stages);
   static emk_device_once once;
   {
     std::lock_guard<std::mutex> lk(once.mu);
