@@ -57,13 +57,12 @@ struct Gemm8Args {
 // ---------------------------------------------------------------------------------------------------------------
 // Many rows: CTA pairs
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int P8_THREADS = 320;  // warps 0-3 and 6-9: epilogue (left / right half of the tile's columns), 4: TMA, 5: MMA
+constexpr int P8_THREADS = 576;  // warps 0-15: epilogue (four per quarter of the columns), 16: TMA, 17: MMA
+constexpr int P8_TMA_WARP = 16, P8_MMA_WARP = 17;
 constexpr int P8_GROUP_M = 8;
-constexpr int P8_BN = 256;
 constexpr int P8_STAGES = 3;
 constexpr int P8_KSUB = 2;
-constexpr int P8_SUB = BM * BKB;                 // one slice of this CTA's 128 rows of x; the W half has as many
-constexpr int P8_OPERAND_STAGE = P8_KSUB * P8_SUB;
+constexpr int P8_A_SUB = BM * BKB;  // one slice of this CTA's 128 rows of x
 
 struct __align__(8) P8Barriers {
   uint64_t full[P8_STAGES];
@@ -73,40 +72,47 @@ struct __align__(8) P8Barriers {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int P8_SMEM = P8_STAGES * 2 * P8_OPERAND_STAGE + 1024 + (int)sizeof(P8Barriers);
+constexpr int p8_smem(int bn) { return P8_STAGES * P8_KSUB * (P8_A_SUB + bn / 2 * BKB) + 1024 + (int)sizeof(P8Barriers); }
 
-// 32 accumulator columns [col0, col0 + 32) of output row `row`
-__device__ __forceinline__ void store32_e4m3(const Gemm8Args& g, const uint32_t* r, int row, int col0, float xs) {
+// 16 accumulator columns [col0, col0 + 16) of output row `row`: one 32-byte sector per lane
+__device__ __forceinline__ void store16_e4m3(const Gemm8Args& g, const uint32_t* r, int row, int col0, float xs) {
   if (row >= g.M || col0 >= g.N) return;
-  uint32_t o[16];
+  uint32_t o[8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
+  for (int q = 0; q < 4; ++q) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (col0 + q * 4 < g.N) s = __ldg(reinterpret_cast<const float4*>(g.w_scale + col0 + q * 4));  // N is a multiple of 8
     o[2 * q] = pack_bf16x2(__uint_as_float(r[4 * q]) * xs * s.x, __uint_as_float(r[4 * q + 1]) * xs * s.y);
     o[2 * q + 1] = pack_bf16x2(__uint_as_float(r[4 * q + 2]) * xs * s.z, __uint_as_float(r[4 * q + 3]) * xs * s.w);
   }
   __nv_bfloat16* out = g.y + (int64_t)row * g.N + col0;
-  if (g.wide && col0 + 32 <= g.N) {
+  if (g.wide) {  // rows of whole 32-byte sectors: N is a multiple of 16
     st_global_v8(out, o);
-    st_global_v8(out + 16, o + 8);
   } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (col0 + q * 8 < g.N)
-        *reinterpret_cast<uint4*>(out + q * 8) = make_uint4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+    *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (col0 + 8 < g.N) *reinterpret_cast<uint4*>(out + 8) = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
+// keeps uses of these registers behind the tcgen05.wait::ld before it
+__device__ __forceinline__ void tie_regs16(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+template <int BN>  // columns of a tile; each CTA loads half of them
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P8_THREADS, 1)
 gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Gemm8Args g) {
-  constexpr uint32_t STAGE_TX = 2u * (2 * P8_OPERAND_STAGE);  // both CTAs' bytes land on the leader's barrier
-  constexpr uint32_t IDESC = make_idesc_e4m3(2 * BM, P8_BN);
+  constexpr int B_SUB = BN / 2 * BKB;  // one slice of this CTA's half of the W tile
+  constexpr int A_STAGE = P8_KSUB * P8_A_SUB, B_STAGE = P8_KSUB * B_SUB;
+  constexpr uint32_t STAGE_TX = 2u * (A_STAGE + B_STAGE);  // both CTAs' bytes land on the leader's barrier
+  constexpr int ACC = 256;             // tensor-memory columns from one accumulator to the next
+  constexpr uint32_t IDESC = make_idesc_e4m3(2 * BM, BN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
-  uint8_t* sB = smem + P8_STAGES * P8_OPERAND_STAGE;
-  P8Barriers* bars = reinterpret_cast<P8Barriers*>(sB + P8_STAGES * P8_OPERAND_STAGE);
+  uint8_t* sB = smem + P8_STAGES * A_STAGE;
+  P8Barriers* bars = reinterpret_cast<P8Barriers*>(sB + P8_STAGES * B_STAGE);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -123,12 +129,12 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->tmem_full[i], 1);
-      mbar_init(&bars->tmem_empty[i], 16);  // 8 epilogue warps of each CTA
+      mbar_init(&bars->tmem_empty[i], 32);  // 16 epilogue warps of each CTA
     }
     bars->abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 4 && lane == 0) {
+  if (warp == P8_TMA_WARP && lane == 0) {
     tma_prefetch_desc(&tma_a);
     tma_prefetch_desc(&tma_b);
   }
@@ -145,7 +151,7 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
   const WaitCtx wc{&bars->abort_flag, g.status, g.limit_ns};
 
-  if (warp == 4) {
+  if (warp == P8_TMA_WARP) {
     if (lane == 0) {  // TMA producer (both CTAs)
       int stage = 0;
       uint32_t phase = 0;
@@ -154,7 +160,7 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
         int tm, tn;
         tile_coords(tile, g.tiles_m, g.tiles_n, P8_GROUP_M, tm, tn);
         const int m0 = tm * 2 * BM + (int)rank * BM;
-        const int n0 = tn * P8_BN + (int)rank * (P8_BN / 2);
+        const int n0 = tn * BN + (int)rank * (BN / 2);
         for (int kb = 0; kb < g.kblocks; kb += P8_KSUB) {
           if (!mbar_wait(&bars->empty[stage], phase ^ 1u, wc, EMK_DEV_TIMEOUT_PRODUCER)) {
             ok = false;
@@ -165,8 +171,8 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
 #pragma unroll
           for (int u = 0; u < P8_KSUB; ++u) {  // slices past K are zero-filled by TMA and add nothing
             const int k0 = (kb + u) * BKB;
-            tma_load_2d_pair(sA + stage * P8_OPERAND_STAGE + u * P8_SUB, &tma_a, full_leader, k0, m0);
-            tma_load_2d_pair(sB + stage * P8_OPERAND_STAGE + u * P8_SUB, &tma_b, full_leader, k0, n0);
+            tma_load_2d_pair(sA + stage * A_STAGE + u * P8_A_SUB, &tma_a, full_leader, k0, m0);
+            tma_load_2d_pair(sB + stage * B_STAGE + u * B_SUB, &tma_b, full_leader, k0, n0);
           }
           if (++stage == P8_STAGES) {
             stage = 0;
@@ -175,7 +181,7 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
         }
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == P8_MMA_WARP) {
     if (leader && lane == 0) {  // MMA issuer
       int stage = 0;
       uint32_t phase = 0;
@@ -189,20 +195,19 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
         const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
         if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, wc, EMK_DEV_TIMEOUT_MMA)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * P8_BN);
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * ACC);
         for (int kb = 0; kb < g.kblocks; kb += P8_KSUB) {
           if (!mbar_wait(&bars->full[stage], phase, wc, EMK_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
-          const uint32_t a_st = a_lo0 + (uint32_t)(stage * (P8_OPERAND_STAGE >> 4));
-          const uint32_t b_st = b_lo0 + (uint32_t)(stage * (P8_OPERAND_STAGE >> 4));
+          const uint32_t a_st = a_lo0 + (uint32_t)(stage * (A_STAGE >> 4));
+          const uint32_t b_st = b_lo0 + (uint32_t)(stage * (B_STAGE >> 4));
 #pragma unroll
           for (int u = 0; u < P8_KSUB; ++u) {
 #pragma unroll
             for (int k = 0; k < BKB / 32; ++k) {
-              const uint32_t off = (uint32_t)((u * P8_SUB + k * 32) >> 4);
-              umma8_pair_lohi(d_tmem, a_st + off, b_st + off, desc_hi, IDESC, (u | k) != 0 ? 1u : (uint32_t)(kb != 0));
+              umma8_pair_lohi(d_tmem, a_st + (uint32_t)((u * P8_A_SUB + k * 32) >> 4), b_st + (uint32_t)((u * B_SUB + k * 32) >> 4), desc_hi, IDESC, (u | k) != 0 ? 1u : (uint32_t)(kb != 0));
             }
           }
           const uint32_t e_local = smem_u32(&bars->empty[stage]);
@@ -221,10 +226,10 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
       }
     }
   } else {
-    // epilogue: warps 0..3 the left half of the columns, 6..9 the right half; a warp may only touch the tensor-memory
-    // lanes of its quarter (warp_id % 4)
-    const int quarter = warp & 3;
-    const int half = warp >= 6 ? 1 : 0;
+    // epilogue: a warp may only touch the tensor-memory lanes of its quarter (warp_id % 4); four warps share a quarter's
+    // rows and take a fourth of the columns each. Sixteen warps instead of eight: the drain of a K = 1024 tile lasts
+    // longer than its multiplication, and a warp spends it waiting (tensor-memory loads, scales, stores).
+    const int quarter = warp & 3, part = warp >> 2;
     int local = 0;
     for (int tile = pair; tile < ntiles; tile += npairs, ++local) {
       const int acc = local & 1;
@@ -232,19 +237,19 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
       int tm, tn;
       tile_coords(tile, g.tiles_m, g.tiles_n, P8_GROUP_M, tm, tn);
       const int row = tm * 2 * BM + (int)rank * BM + quarter * 32 + lane;
-      const int n0 = tn * P8_BN + half * (P8_BN / 2);
+      const int n0 = tn * BN + part * (BN / 4);
       const float xs = row < g.M ? __ldg(g.x_scale + row) : 0.f;
       if (!mbar_wait_warp(&bars->tmem_full[acc], acc_phase, wc, EMK_DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * P8_BN + half * (P8_BN / 2));
-      uint32_t r[2][32];
-      tmem_ld_x32(taddr, r[0]);
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * ACC + part * (BN / 4));
+      uint32_t r[BN / 64][16];
 #pragma unroll
-      for (int c = 0; c < P8_BN / 64; ++c) {
-        tmem_ld_wait_regs(r[c & 1]);
-        if (c + 1 < P8_BN / 64) tmem_ld_x32(taddr + (uint32_t)((c + 1) * 32), r[(c + 1) & 1]);
-        store32_e4m3(g, r[c & 1], row, n0 + c * 32, xs);
-      }
+      for (int c = 0; c < BN / 64; ++c) tmem_ld_x16(taddr + (uint32_t)(c * 16), r[c]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) tie_regs16(r[c]);
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) store16_e4m3(g, r[c], row, n0 + c * 16, xs);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&bars->tmem_empty[acc]), 0));
@@ -467,10 +472,18 @@ int linear_rows(emk_handle_t h, const void* x, const void* w, Gemm8Args g, int64
   const int nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   g.tiles_m = (g.M + nt - 1) / nt;
   g.tiles_n = (g.N + BM - 1) / BM;
-  // Split K until two CTAs per SM have work, each at least two slices.
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  // Split K until every SM has a CTA, each with two slices at least. A third more CTAs than SMs still pays while the
+  // partial tiles are small (1 x 6144 x 2048: 192 CTAs 4.7 us, 96 CTAs 5.3; 128 rows: 9.5 and 9.0), two per SM where each
+  // keeps a long K (128 x 8192 x 8192: 19.7 us against 22.0), and eight parts only for small tiles or few of them
+  // (128 x 2048 x 4096: 8.9 us in eight, 7.9 in four; one row 4.4 and 5.2; 1024 x 128 x 4096: 7.0 and 8.0).
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, sms = h->sm_count;
+  const int most = nt <= 32 || tiles <= 8 ? R8_MAX_SPLIT : 4;
   int split = 1;
-  while (split < R8_MAX_SPLIT && tiles * split * 2 <= 2 * (int64_t)h->sm_count && g.kblocks >= split * 4) split *= 2;
+  while (split < most && g.kblocks >= split * 4) {
+    const int64_t cap = g.kblocks >= split * 2 * 16 ? 2 * sms : nt <= 32 ? sms + sms / 3 : sms;
+    if (tiles * split * 2 > cap) break;
+    split *= 2;
+  }
   CUtensorMap tw, tx;
   int rc = emk_make_tmap_2d(h, &tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (uint64_t)K, (uint64_t)g.N, (uint64_t)K, BKB, BM,
                             CU_TENSOR_MAP_SWIZZLE_128B);
@@ -486,30 +499,53 @@ int linear_rows(emk_handle_t h, const void* x, const void* w, Gemm8Args g, int64
   }
 }
 
-int linear_pairs(emk_handle_t h, const void* x, const void* w, Gemm8Args g, int64_t K, cudaStream_t s) {
+template <int BN>
+int launch_pairs(emk_handle_t h, const CUtensorMap& ta, const void* w, Gemm8Args g, int64_t K, cudaStream_t s) {
   g.tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
-  g.tiles_n = (g.N + P8_BN - 1) / P8_BN;
-  CUtensorMap ta, tb;
-  int rc = emk_make_tmap_2d(h, &ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)K, (uint64_t)g.M, (uint64_t)K, BKB, BM,
-                            CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc != EMK_OK) return rc;
-  rc = emk_make_tmap_2d(h, &tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (uint64_t)K, (uint64_t)g.N, (uint64_t)K, BKB, BM,
-                        CU_TENSOR_MAP_SWIZZLE_128B);
+  g.tiles_n = (g.N + BN - 1) / BN;
+  CUtensorMap tb;
+  const int rc = emk_make_tmap_2d(h, &tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (uint64_t)K, (uint64_t)g.N, (uint64_t)K, BKB,
+                                  BN / 2, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != EMK_OK) return rc;
   static emk_device_once once;
   {
     std::lock_guard<std::mutex> lk(once.mu);
     if (!once.done[h->device]) {
-      EMK_CUDA_TRY(h, cudaFuncSetAttribute(gemm2_e4m3_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(gemm2_e4m3_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, p8_smem(BN)));
       once.done[h->device] = true;
     }
   }
   const int ntiles = g.tiles_m * g.tiles_n;
   const int pairs = ntiles < h->sm_count / 2 ? ntiles : h->sm_count / 2;
-  EMK_CUDA_TRY(h, launch_after_prologue(gemm2_e4m3_kernel, 2u * (unsigned)pairs, P8_THREADS, P8_SMEM, s,
+  EMK_CUDA_TRY(h, launch_after_prologue(gemm2_e4m3_kernel<BN>, 2u * (unsigned)pairs, P8_THREADS, p8_smem(BN), s,
                                         h->overlap_launch != 0, ta, tb, g));
   EMK_LAUNCH_CHECK(h);
   return EMK_OK;
+}
+
+int linear_pairs(emk_handle_t h, const void* x, const void* w, const Gemm8Args& g, int64_t K, cudaStream_t s) {
+  CUtensorMap ta;
+  const int rc = emk_make_tmap_2d(h, &ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)K, (uint64_t)g.M, (uint64_t)K, BKB,
+                                  BM, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != EMK_OK) return rc;
+  // Rounds of tiles over the machine's pairs, times what a round costs at the tile's width: at K = 2048 a 256-column
+  // tile takes 6.4 us, a 192-column one 5.7, a 128-column one 4.4 (operand traffic per multiplication grows as the tile
+  // narrows), so narrow tiles pay only where they save rounds. Measured at 1024 x 6144 x 2048: 17.5 / 15.8 / 17.8 us;
+  // 256 x 4096 x 1024: 8.0 / 6.7 / 5.9; 4096 x 6144 x 2048: 42.4 / 43.8 / 52.7.
+  const int64_t pairs = h->sm_count / 2, tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
+  const auto cost = [&](int64_t bn, int64_t weight) { return (tiles_m * ((g.N + bn - 1) / bn) + pairs - 1) / pairs * weight; };
+  const int64_t c256 = cost(256, 100), c192 = cost(192, 88), c128 = cost(128, 69);
+  if (c128 < c192 && c128 < c256) return launch_pairs<128>(h, ta, w, g, K, s);
+  return c192 < c256 ? launch_pairs<192>(h, ta, w, g, K, s) : launch_pairs<256>(h, ta, w, g, K, s);
+}
+
+// Which kernel: up to 64 rows the pairs would multiply padding; beyond that the rows kernel wins where only its split of K
+// fills the machine: few tiles and a K worth splitting (1024 x 128 x 4096: 7.0 us against 11.4; 512 x 512 x 2048: 6.7
+// against 7.7), or a long K under one row of tiles (128 x 8192 x 8192: 19.7 against 22.4). It loses otherwise
+// (128 x 2048 x 512: 6.8 against 4.9; 128 x 4096 x 1024: 6.4 against 5.8; 256 x 4096 x 1024: 11.0 against 5.8).
+bool few_rows(int64_t M, int64_t N, int64_t K) {
+  if (M <= 64) return true;
+  return ((M + BM - 1) / BM * ((N + BM - 1) / BM) <= 16 && K >= 2048) || (M <= BM && K >= 4096);
 }
 
 }  // namespace
@@ -538,5 +574,5 @@ extern "C" int emk_linear_e4m3(emk_handle_t h, const void* x, const float* x_sca
   g.wide = ((N % 16) == 0 && ((uintptr_t)y & 31u) == 0) ? 1 : 0;
   g.status = h->status_dev;
   g.limit_ns = h->wait_limit_ns;
-  return M <= 256 ? linear_rows(h, x, w, g, K, (cudaStream_t)stream) : linear_pairs(h, x, w, g, K, (cudaStream_t)stream);
+  return few_rows(M, N, K) ? linear_rows(h, x, w, g, K, (cudaStream_t)stream) : linear_pairs(h, x, w, g, K, (cudaStream_t)stream);
 }

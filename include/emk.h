@@ -143,8 +143,8 @@ int64_t emk_linear_bf16_w8_workspace_bytes(int64_t N, int64_t K);
 /* Both operands in 8 bits: y[m,n] = bf16( x_scale[m] * w_scale[n] * sum_k x[m,k] * W[n,k] ), x [M,K] and W [N,K] e4m3
  * codes, fp32 scales [M] and [N], exact products, fp32 accumulation in tensor memory. x and x_scale are what
  * emk_rmsnorm_e4m3 writes; W and w_scale are emk_linear_bf16_w8's. K a multiple of 16, N of 8, pointers 16-byte aligned
- * (x_scale 4). No workspace. The first call of a row class (up to 16, 32, 64, 256 rows, more) on a device sets that
- * kernel's shared-memory attribute: make it before any stream capture. No counterpart in the reference. */
+ * (x_scale 4). No workspace. The sizes choose the kernel, whose first call on a device sets its shared-memory
+ * attribute: make a warm-up call of the same sizes before any stream capture. No counterpart in the reference. */
 int emk_linear_e4m3(emk_handle_t h, const void* x, const float* x_scale, const void* w, const float* w_scale, void* y,
                     int64_t M, int64_t N, int64_t K, emk_stream_t stream);
 
