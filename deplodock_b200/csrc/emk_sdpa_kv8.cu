@@ -17,10 +17,11 @@
 // log2(v_scale) and p * v_scale / max is what is rounded to f16 (2^-12 relative: p in [0, 2^15], so 2^-29 of the largest
 // contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
 //
-// Work split: the tiles of 64 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
-// CTA: sequences of any mix of lengths load all SMs alike without the host knowing the lengths. A row whose tiles fall
-// into one range is finished there; the others leave (max, sum, o) per range in the workspace, at most two per CTA, and a
-// second kernel joins them.
+// Work split: the tiles of 16 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
+// warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths, and a warp needs nothing of
+// its neighbours. Beginning a row costs a warp about as much as a tile (the queries, a pipeline to fill, an output), so a
+// row counts ROW_COST tiles more than it has. A row that falls into one range is finished there; the others leave
+// (maximum, sum, o) per range in the workspace, at most two per warp, and a second kernel joins them.
 #include "emk_kv8.cuh"
 
 #include <cuda_fp16.h>
@@ -33,10 +34,11 @@ using namespace emk;
 constexpr int SK_WARPS = 4;
 constexpr int SK_THREADS = SK_WARPS * 32;
 constexpr int SK_STAGES = 4;
-constexpr int SK_TILE = SK_WARPS * 16;  // tokens
+constexpr int SK_TILE = 16;  // tokens
+constexpr int ROW_COST = 1;
 constexpr int SK_ROWS = 16;
 constexpr int SK_CTAS_PER_SM = 3;
-constexpr int SK_JOIN_WARPS = 8;
+constexpr int SK_JOIN_WARPS = 16;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float P_SHIFT = 8.f;  // p is rounded as 2^8 p: with the lazy maximum (below) at most 2^15
 constexpr float LAZY = 7.f;     // the running maximum moves when the new one is more than 2^7 above it
@@ -52,11 +54,11 @@ struct SdpaArgs {
   const int32_t* lens;
   __nv_bfloat16* o;
   int64_t ld_q;
-  int B, Sq, Hq, Hkv, G, row_tiles, page_shift, max_pages, num_pages;
+  int B, Sq, Hq, Hkv, G, row_tiles, row_cap, page_shift, max_pages, num_pages;
   float scale_log2;
-  int2* info;    // [B * Hkv * row_tiles]: first and last CTA of the row
-  float2* ml;    // [CTAs][2][16]: maximum, sum
-  float* part;   // [CTAs][2][16][D]
+  int2* info;    // [B * Hkv * row_tiles]: first and last range of the row
+  float2* ml;    // [ranges][2][row_cap]: maximum, sum
+  float* part;   // [ranges][2][row_cap][D]
   int* status;
 };
 
@@ -66,7 +68,9 @@ __device__ __forceinline__ int seq_len(const SdpaArgs& a, int b) {
   if (n < 0 || n > room) emk_record_bounds(a.status, EMK_DEV_BOUNDS_CACHE_LEN);
   return (int)min((int64_t)max(n, 0), room);
 }
-__device__ __forceinline__ int64_t seq_tiles(int len) { return ((int64_t)len + SK_TILE - 1) / SK_TILE; }
+__device__ __forceinline__ int seq_tiles(int len) { return (int)(((int64_t)len + SK_TILE - 1) / SK_TILE); }
+// what a row of `tiles` tiles counts in the list
+__device__ __forceinline__ int64_t row_units(int tiles) { return tiles > 0 ? (int64_t)tiles + ROW_COST : 0; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -113,9 +117,9 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Where the flat tile `t` of `total` lies among `ctas` equal ranges [c * total / ctas, (c+1) * total / ctas).
-__device__ __forceinline__ int64_t range_start(int64_t c, int64_t total, int64_t ctas) { return c * total / ctas; }
-__device__ __forceinline__ int64_t range_owner(int64_t t, int64_t total, int64_t ctas) { return ((t + 1) * ctas - 1) / total; }
+// Unit `u` of `total` lies in range range_owner(u); range c is [c * total / ranges, (c+1) * total / ranges).
+__device__ __forceinline__ int64_t range_start(int64_t c, int64_t total, int64_t ranges) { return c * total / ranges; }
+__device__ __forceinline__ int64_t range_owner(int64_t u, int64_t total, int64_t ranges) { return ((u + 1) * ranges - 1) / total; }
 
 template <int D>
 struct SkLayout {
@@ -125,9 +129,7 @@ struct SkLayout {
   static constexpr int WARP_RING = SK_STAGES * STAGE;
   static constexpr int RING = SK_WARPS * WARP_RING;
   static constexpr int SCALES = SK_WARPS * SK_STAGES * 8;
-  static constexpr int O_PITCH = D + 8;                  // floats; spreads the merge's rows over the banks
   static constexpr int SMEM = RING + SCALES;
-  static_assert(SK_WARPS * SK_ROWS * O_PITCH * 4 <= RING, "the merge buffer aliases the ring");
 };
 
 template <int D>
@@ -136,56 +138,43 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
   constexpr int STEPS = D / 16;  // k16 steps of q K^T
   constexpr int NT = D / 8;      // n8 tiles of P V
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_sum[SK_WARPS];
-  __shared__ int64_t s_prefix;
-  __shared__ int s_seq;
-  __shared__ float s_m[SK_WARPS][SK_ROWS], s_l[SK_WARPS][SK_ROWS];
-
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int heads = a.Hkv * a.row_tiles;  // rows (of tiles) per sequence
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // ---- this CTA's range of the flat tile list ----
-  int64_t sum = 0;
-  for (int b = threadIdx.x; b < a.B; b += SK_THREADS) sum += seq_tiles(seq_len(a, b));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
+  // ---- this warp's range of the list ----
   int64_t total = 0;
+  for (int i = lane; i < a.B; i += 32) total += row_units(seq_tiles(seq_len(a, i)));
 #pragma unroll
-  for (int i = 0; i < SK_WARPS; ++i) total += s_sum[i];
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= heads;
-  const int64_t ctas = min((int64_t)gridDim.x, total);  // no more ranges than tiles: none is empty
-  if (blockIdx.x >= ctas) return;
-  int64_t pos = range_start(blockIdx.x, total, ctas);
-  const int64_t end = range_start(blockIdx.x + 1, total, ctas);
-  if (warp == 0) {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const int64_t mine = b0 + lane < a.B ? seq_tiles(seq_len(a, b0 + lane)) * heads : 0;
-      int64_t upto = mine;
+  const int64_t ranges = min((int64_t)gridDim.x * SK_WARPS, total);  // no more ranges than units: none is empty
+  const int64_t range = (int64_t)blockIdx.x + (int64_t)warp * gridDim.x;  // neighbours in the list run on different SMs
+  if (range >= ranges) return;
+  int64_t pos = range_start(range, total, ranges);
+  const int64_t end = range_start(range + 1, total, ranges);
+  int b = 0;
+  int64_t prefix = 0;  // index of sequence b's first unit
+  for (int b0 = 0;; b0 += 32) {
+    const int64_t mine = b0 + lane < a.B ? row_units(seq_tiles(seq_len(a, b0 + lane))) * heads : 0;
+    int64_t upto = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += u;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, pos < base + upto);
-      if (past != 0) {
-        if (lane == __ffs(past) - 1) {
-          s_seq = b0 + lane;
-          s_prefix = base + upto - mine;
-        }
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, upto, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
     }
+    const unsigned past = __ballot_sync(0xffffffffu, pos < prefix + upto);
+    if (past != 0) {
+      const int src = __ffs(past) - 1;
+      b = b0 + src;
+      prefix += __shfl_sync(0xffffffffu, upto - mine, src);
+      break;
+    }
+    prefix += __shfl_sync(0xffffffffu, upto, 31);
+    if (b0 + 32 >= a.B) return;  // not reached: pos lies before total
   }
-  __syncthreads();
-  int b = s_seq;
-  int64_t prefix = s_prefix;  // flat index of sequence b's first tile
 
   uint8_t* ring = smem + warp * L::WARP_RING;
   const uint32_t ring_u32 = smem_u32(ring);
@@ -196,29 +185,29 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
   while (pos < end) {
     // ---- the next row and the part of it that is ours ----
     int len = seq_len(a, b);
-    int64_t tiles = seq_tiles(len);
-    while (pos >= prefix + tiles * heads) {
-      prefix += tiles * heads;
+    int tiles = seq_tiles(len);
+    int64_t units = row_units(tiles);
+    while (pos >= prefix + units * heads) {
+      prefix += units * heads;
       ++b;
       len = seq_len(a, b);
       tiles = seq_tiles(len);
+      units = row_units(tiles);
     }
-    const int hr = (int)((pos - prefix) / tiles);
-    const int64_t row_first = prefix + hr * tiles;
-    const int ta = (int)(pos - row_first);
-    const int tb = (int)min(tiles, end - row_first);
-    pos = row_first + tb;
+    const int hr = (int)((pos - prefix) / units);
+    const int64_t tile0 = prefix + hr * units + ROW_COST;  // the unit of the row's first tile
+    const int ta = (int)max(pos - tile0, (int64_t)0);
+    const int tb = (int)min(end - tile0, (int64_t)tiles);
+    pos = min(end, tile0 + tiles);
+    if (tb <= ta) continue;  // only what a row counts beside its tiles
     const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
     const int rows = min(SK_ROWS, a.G * a.Sq - rt * SK_ROWS);
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
+    const int nsub = tb - ta;
 
-    // ---- the 16-token tiles of this warp: warp, warp + 4, ... of the range ----
-    const int sub_end = min(tb * SK_WARPS, (len + 15) >> 4);
-    const int sub0 = ta * SK_WARPS + warp;
-    const int nsub = sub_end > sub0 ? (sub_end - sub0 + SK_WARPS - 1) / SK_WARPS : 0;
     // lane j holds the page of tile i0 + j of this warp's list, for the 32 tiles that are issued now and the next 32
     auto page_of = [&](int i) {
-      const int s = sub0 + i * SK_WARPS;
+      const int s = ta + i;
       return i < nsub ? kv8_page_id(table, ((int64_t)s * 16) >> a.page_shift, a.num_pages, a.status) : 0;
     };
     int pid_now = page_of(lane), pid_next = page_of(32 + lane);
@@ -229,7 +218,7 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
           pid_next = page_of(i + 32 + lane);
         }
         const int pid = __shfl_sync(0xffffffffu, pid_now, i & 31);
-        const int s = sub0 + i * SK_WARPS;
+        const int s = ta + i;
         const int64_t unit = (int64_t)pid * a.Hkv + hkv;
         const int64_t at = ((unit << a.page_shift) + ((s * 16) & ((1 << a.page_shift) - 1))) * D;
         const int left = len - s * 16;  // tokens of this tile that exist: the others are zeros, whatever the page holds
@@ -332,7 +321,7 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
       }
       const float c0 = qs[0] * ks, c1 = qs[1] * ks;
       const float lvs = lg2(vs), inv_vs = 1.0f / vs;
-      const int tok0 = (sub0 + i * SK_WARPS) * 16 + 2 * t;
+      const int tok0 = (ta + i) * 16 + 2 * t;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         s[u][0] = fmaf(s[u][0], c0, lvs);
@@ -414,71 +403,48 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
       }
     }
 
-    // ---- join the four warps ----
+    // ---- this range's part of the row: channels [2 t NT, (2 t + 2) NT) of rows g and g + 8 per lane ----
     cp_async_wait<0>();
+    const bool whole = ta == 0 && tb == tiles;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
-    __syncthreads();  // every warp is done with its ring, whose memory now holds the rows
-    float* merge = reinterpret_cast<float*>(smem) + warp * SK_ROWS * L::O_PITCH;
+      const int row = g + 8 * r;
+      if (row < rows) {
+        if (whole) {
+          const int rr = rt * SK_ROWS + row;
+          const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
+          const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
+          __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + 2 * t * NT;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if (t == 0) {
-        s_m[warp][g + 8 * r] = m[r];
-        s_l[warp][g + 8 * r] = l[r];
-      }
+          for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)  // channel c * NT + j at j * 8 + c: the two of a lane are neighbours
-        *reinterpret_cast<float2*>(merge + (g + 8 * r) * L::O_PITCH + j * 8 + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-    }
-    __syncthreads();
-    const int row = threadIdx.x >> 3, col = threadIdx.x & 7;
-    const bool whole = ta == 0 && tb == tiles;
-    const int slot = ta == 0 ? 1 : 0;
-    if (row < rows) {
-      float top = -INFINITY;
+            for (int j = 0; j < NT; j += 8)
+              *reinterpret_cast<uint4*>(out + c * NT + j) =
+                  make_uint4(pack_bf16x2(o[j][2 * r + c] * inv, o[j + 1][2 * r + c] * inv),
+                             pack_bf16x2(o[j + 2][2 * r + c] * inv, o[j + 3][2 * r + c] * inv),
+                             pack_bf16x2(o[j + 4][2 * r + c] * inv, o[j + 5][2 * r + c] * inv),
+                             pack_bf16x2(o[j + 6][2 * r + c] * inv, o[j + 7][2 * r + c] * inv));
+          }
+        } else {
+          // the first part of a row ends its range (slot 1), any other begins it (slot 0)
+          const int64_t at = (range * 2 + (ta == 0 ? 1 : 0)) * a.row_cap + row;
+          if (t == 0) a.ml[at] = make_float2(m[r], l[r]);
+          float* out = a.part + at * D + 2 * t * NT;
 #pragma unroll
-      for (int w = 0; w < SK_WARPS; ++w) top = fmaxf(top, s_m[w][row]);
-      float f[SK_WARPS], sum_l = 0.f;
+          for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int w = 0; w < SK_WARPS; ++w) {
-        // a warp without a visible token has -inf here, zeros (or, through a NaN, NaN) in its sums
-        f[w] = s_m[w][row] == -INFINITY ? 1.f : ex2(s_m[w][row] - top);
-        sum_l = fmaf(s_l[w][row], f[w], sum_l);
-      }
-      float acc[NT];
-      const float* from = reinterpret_cast<const float*>(smem) + row * L::O_PITCH + col;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        acc[j] = 0.f;
-#pragma unroll
-        for (int w = 0; w < SK_WARPS; ++w) acc[j] = fmaf(from[w * SK_ROWS * L::O_PITCH + j * 8], f[w], acc[j]);
-      }
-      if (whole) {
-        const int rr = rt * SK_ROWS + row;
-        const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
-        const float inv = sum_l == 0.f ? 0.f : 1.0f / sum_l;
-        __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + col * NT;
-#pragma unroll
-        for (int j = 0; j < NT; j += 8)
-          *reinterpret_cast<uint4*>(out + j) =
-              make_uint4(pack_bf16x2(acc[j] * inv, acc[j + 1] * inv), pack_bf16x2(acc[j + 2] * inv, acc[j + 3] * inv),
-                         pack_bf16x2(acc[j + 4] * inv, acc[j + 5] * inv), pack_bf16x2(acc[j + 6] * inv, acc[j + 7] * inv));
-      } else {
-        const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * SK_ROWS + row;
-        if (col == 0) a.ml[at] = make_float2(top, sum_l);
-        float* out = a.part + at * D + col * NT;
-#pragma unroll
-        for (int j = 0; j < NT; j += 4)
-          *reinterpret_cast<float4*>(out + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            for (int j = 0; j < NT; j += 4)
+              *reinterpret_cast<float4*>(out + c * NT + j) =
+                  make_float4(o[j][2 * r + c], o[j + 1][2 * r + c], o[j + 2][2 * r + c], o[j + 3][2 * r + c]);
+          }
+        }
       }
     }
-    if (ta == 0 && threadIdx.x == 0)
-      a.info[(int64_t)b * heads + hr] =
-          make_int2((int)blockIdx.x, (int)range_owner(row_first + tiles - 1, total, ctas));
-    __syncthreads();  // the merge buffer becomes the ring again
+    if (ta == 0 && lane == 0)
+      a.info[(int64_t)b * heads + hr] = make_int2((int)range, (int)range_owner(tile0 + tiles - 1, total, ranges));
+    __syncwarp();
   }
 }
 
@@ -498,19 +464,18 @@ __global__ void __launch_bounds__(SK_JOIN_WARPS * 32) sdpa_kv8_join_kernel(const
   const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D;
-  if (seq_len(a, b) == 0) {  // no tile, so no CTA wrote this row
+  if (seq_len(a, b) == 0) {  // no tile, so no warp wrote this row
     if (threadIdx.x < D / 8) reinterpret_cast<uint4*>(out)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int2 ctas = a.info[blockIdx.x];
-  if (ctas.x == ctas.y) return;
+  const int2 span = a.info[blockIdx.x];
+  if (span.x == span.y) return;
   float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-  for (int c = ctas.x + warp; c <= ctas.y; c += SK_JOIN_WARPS) {
-    // the first range of a row ends its CTA's list (slot 1), the others begin theirs (slot 0)
-    const int64_t at = ((int64_t)c * 2 + (c == ctas.x ? 1 : 0)) * SK_ROWS + blockIdx.y;
+  for (int c = span.x + warp; c <= span.y; c += SK_JOIN_WARPS) {
+    const int64_t at = ((int64_t)c * 2 + (c == span.x ? 1 : 0)) * a.row_cap + blockIdx.y;
     const float2 ml = a.ml[at];
     const float* p = a.part + at * D + lane * E;
     float v[E];
@@ -564,20 +529,22 @@ bool sizes_ok(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv) {
 }
 
 struct SkPlan {
-  int row_tiles;
+  int row_tiles, row_cap;
   int64_t ctas, info_bytes, ml_bytes, part_bytes;
 };
 
-// The grid never has more CTAs than the longest possible tile list has tiles.
+// The grid never has more warps than the longest possible list has units.
 SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t max_tokens, int64_t D) {
   SkPlan p;
   p.row_tiles = (int)((Hq / Hkv * Sq + SK_ROWS - 1) / SK_ROWS);
-  const int64_t tiles = B * Hkv * p.row_tiles * ((max_tokens + SK_TILE - 1) / SK_TILE);
+  p.row_cap = Hq / Hkv * Sq < SK_ROWS ? (int)(Hq / Hkv * Sq) : SK_ROWS;
+  const int64_t units = (max_tokens + SK_TILE - 1) / SK_TILE + ROW_COST;  // below 2^28
+  const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
   p.ctas = (int64_t)sm_count * SK_CTAS_PER_SM;
-  if (tiles < p.ctas) p.ctas = tiles;
-  p.info_bytes = align16(B * Hkv * p.row_tiles * (int64_t)sizeof(int2));
-  p.ml_bytes = p.ctas * 2 * SK_ROWS * (int64_t)sizeof(float2);
-  p.part_bytes = p.ctas * 2 * SK_ROWS * D * (int64_t)sizeof(float);
+  if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
+  p.info_bytes = align16(rows * (int64_t)sizeof(int2));
+  p.ml_bytes = align16(p.ctas * SK_WARPS * 2 * p.row_cap * (int64_t)sizeof(float2));
+  p.part_bytes = p.ctas * SK_WARPS * 2 * p.row_cap * D * (int64_t)sizeof(float);
   return p;
 }
 
@@ -595,7 +562,7 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
                                         h->overlap_launch != 0, a));
   EMK_LAUNCH_CHECK(h);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_tiles), (unsigned)(a.G * a.Sq < SK_ROWS ? a.G * a.Sq : SK_ROWS), 1);
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_tiles), (unsigned)a.row_cap, 1);
   cfg.blockDim = dim3(SK_JOIN_WARPS * 32, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -662,6 +629,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   a.Hkv = (int)Hkv;
   a.G = (int)(Hq / Hkv);
   a.row_tiles = p.row_tiles;
+  a.row_cap = p.row_cap;
   a.page_shift = __builtin_ctzll((unsigned long long)page);
   a.max_pages = (int)max_pages;
   a.num_pages = (int)num_pages;
