@@ -3,13 +3,20 @@
 // query i of Sq sits at position len - Sq + i and sees the tokens up to itself; a row that sees nothing gives zeros.
 //
 // Bound by HBM: every cached byte is read once and meets 4 * (Hq/Hkv) * Sq flops. The rows that share a KV head (Hq/Hkv
-// heads x Sq queries) form tiles of 16 and go through mma.sync m16n8k16 in f16 with fp32 sums: at a few rows per cache
-// byte the tensor-memory path would be fed 1/16 full tiles, and what counts is the flow of bytes. Each lane of a warp copies
-// with cp.async exactly the bytes that its own mma fragments need (four stages of 16 tokens in flight per warp), so the
-// loop has no barrier: the token and channel order inside a fragment is permuted alike for both operands, which a sum does
-// not notice.
-//   K fragment: lane (g, t) holds token g and 8 + g, channels 16t.. and 64 + 16t..   (4 bytes = one k16 step)
-//   V fragment: lane (g, t) holds tokens 2t, 2t+1, 2t+8, 2t+9, channels 16g..         (pairs of tokens interleaved by prmt)
+// heads x Sq queries) form tiles of 8 or 16 and go through mma.sync m16n8k16 in f16 with fp32 sums, the cache as the
+// instruction's 16 rows and the queries as its 8 columns:
+//   S^T [tokens x rows] = K q^T,   o^T [channels x rows] = V^T P^T
+// so that a group of up to eight rows wastes nothing. (At a few rows per cache byte the tensor-memory path would be fed 1/16
+// full tiles; what counts is the flow of bytes and the instructions per byte.) Every warp copies its own tiles with
+// cp.async, a few tiles of 16 tokens ahead, so the loop has no barrier between warps. A copy instruction moves 512
+// contiguous bytes, lane after lane: with lanes that fetch what their own fragments need instead, 16 bytes of four rows side
+// by side, every sector crossed twice and every lane took a shared-memory cycle of its own (2.0x the sectors, 26 cycles an
+// instruction, and that was the bound: 64 sequences of up to 8192 tokens 136 us). 32-byte units are swizzled so that the
+// fragment loads meet no bank twice. The token and channel order inside a fragment is permuted alike for both operands,
+// which a sum does not notice.
+//   K fragment: lane (g, t) holds tokens g and 8 + g, channels 16t.. and 64 + 16t..   (4 bytes = one k16 step)
+//   V fragment: lane (g, t) holds tokens 2t, 2t+1, 2t+8, 2t+9, channels (D/8) g..    (pairs of tokens interleaved by prmt)
+// P^T comes out of S^T by movmatrix.
 //
 // e4m3 -> f16 is exact. q is scaled per row by a power of two into f16's range (exact; elements 2^-38 below the row's
 // largest may lose bits, far below the fp32 sum's own rounding). The scales of keys go into the logits; the scale of
@@ -18,10 +25,10 @@
 // contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
 //
 // Work split: the tiles of 16 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
-// warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths, and a warp needs nothing of
-// its neighbours. Beginning a row costs a warp about as much as a tile (the queries, a pipeline to fill, an output), so a
-// row counts ROW_COST tiles more than it has. A row that falls into one range is finished there; the others leave
-// (maximum, sum, o) per range in the workspace, at most two per warp, and a second kernel joins them.
+// warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths. Beginning a row costs a
+// warp about as much as a tile (the queries, a pipeline to fill, an output), so a row counts ROW_COST tiles more than it
+// has. A row that falls into one range, or into the ranges of one CTA, is finished there; the others leave
+// (maximum, sum, o) per piece in the workspace and a second kernel joins them.
 #include "emk_kv8.cuh"
 
 #include <cuda_fp16.h>
@@ -33,15 +40,12 @@ using namespace emk;
 
 constexpr int SK_WARPS = 4;
 constexpr int SK_THREADS = SK_WARPS * 32;
-constexpr int SK_STAGES = 4;
-constexpr int SK_TILE = 16;  // tokens
+constexpr int SK_TILE = 16;  // tokens: inside one page
 constexpr int ROW_COST = 1;
-constexpr int SK_ROWS = 16;
-constexpr int SK_CTAS_PER_SM = 3;
-constexpr int SK_JOIN_WARPS = 16;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float P_SHIFT = 8.f;  // p is rounded as 2^8 p: with the lazy maximum (below) at most 2^15
-constexpr float LAZY = 7.f;     // the running maximum moves when the new one is more than 2^7 above it
+constexpr float P_SHIFT = 8.f;   // p is rounded as 2^8 p relative to the running maximum ...
+constexpr float P_LIMIT = 15.f;  // ... which moves when a logit is more than 7 above it: the rounded p is at most 2^15
+constexpr float BIG = 65536.f;   // from here on fp32 logits are so coarse that their differences need a clamp
 constexpr float V_SCALE_MIN = 7.888609052210118e-31f;  // 2^-100: a zero scale (a page of zeros) has a logarithm
 
 struct SdpaArgs {
@@ -54,7 +58,7 @@ struct SdpaArgs {
   const int32_t* lens;
   __nv_bfloat16* o;
   int64_t ld_q;
-  int B, Sq, Hq, Hkv, G, row_tiles, row_cap, page_shift, max_pages, num_pages;
+  int B, Sq, Hq, Hkv, G, row_tiles, tile_rows, row_cap, page_shift, max_pages, num_pages;
   float scale_log2;
   int2* info;    // [B * Hkv * row_tiles]: first and last range of the row
   float2* ml;    // [ranges][2][row_cap]: maximum, sum
@@ -72,11 +76,12 @@ __device__ __forceinline__ int seq_tiles(int len) { return (int)(((int64_t)len +
 // what a row of `tiles` tiles counts in the list
 __device__ __forceinline__ int64_t row_units(int tiles) { return tiles > 0 ? (int64_t)tiles + ROW_COST : 0; }
 
+// `bytes` of src, zeros up to 16
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -96,6 +101,11 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -105,39 +115,60 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// two e4m3 codes in the low half of w -> f16 pair
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-  return *reinterpret_cast<const uint32_t*>(&r);
+// four e4m3 codes -> two f16 pairs (exact)
+__device__ __forceinline__ void e4m3x4_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
-__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+// the transpose of an 8 x 8 tile of 16-bit values, a pair of a row per lane
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Unit `u` of `total` lies in range range_owner(u); range c is [c * total / ranges, (c+1) * total / ranges).
 __device__ __forceinline__ int64_t range_start(int64_t c, int64_t total, int64_t ranges) { return c * total / ranges; }
 __device__ __forceinline__ int64_t range_owner(int64_t u, int64_t total, int64_t ranges) { return ((u + 1) * ranges - 1) / total; }
 
-template <int D>
+// RT: tiles of 8 rows per row tile. One: 16 warps per SM with a 12 KB ring each; two (twice the accumulators and query
+// fragments): as many warps as hold them in registers, 8 at D = 128 and 12 at D = 64. (A spill inside the loop costs more
+// than a third of the warps: local memory has to pass an L1 that the rings leave a few KB.)
+template <int D, int RT>
 struct SkLayout {
-  static constexpr int K_CHUNKS = D / 64 * 2;            // 16-byte pieces of K per lane and 16-token tile
+  static constexpr int ROWS = 8 * RT;
+  static constexpr int CTAS_PER_SM = RT == 1 ? 4 : D == 128 ? 2 : 3;
+  static constexpr int K_CHUNKS = D / 64;                // 16-byte pieces of K per lane and 8 tokens
+  static constexpr int COPIES = D / 32;                  // copy instructions for K or V of a tile
   static constexpr int V_BYTES = D / 8;                  // bytes of V per lane and token (16 or 8)
-  static constexpr int STAGE = 16 * D * 2;               // K and V of 16 tokens
-  static constexpr int WARP_RING = SK_STAGES * STAGE;
+  static constexpr int HALF = SK_TILE * D;               // K or V of a tile
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int STAGES = (RT == 1 ? 12 : D == 128 ? 24 : 16) * 1024 / STAGE;
+  static constexpr int WARP_RING = STAGES * STAGE;
   static constexpr int RING = SK_WARPS * WARP_RING;
-  static constexpr int SCALES = SK_WARPS * SK_STAGES * 8;
-  static constexpr int SMEM = RING + SCALES;
+  static constexpr int SMEM = RING + SK_WARPS * STAGES * 8;  // and the scales of K and V of every stage
+  static constexpr int PIECE_PITCH = D + 4;              // floats; spreads the rows over the banks
+  static_assert(ROWS * PIECE_PITCH * 4 <= WARP_RING, "a warp's last piece lies over its ring");
 };
 
-template <int D>
-__global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(const SdpaArgs a) {
-  using L = SkLayout<D>;
-  constexpr int STEPS = D / 16;  // k16 steps of q K^T
-  constexpr int NT = D / 8;      // n8 tiles of P V
+template <int D, int RT>
+__global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa_kv8_kernel(const SdpaArgs a) {
+  using L = SkLayout<D, RT>;
+  constexpr int STEPS = D / 16;  // k16 steps of K q^T, and m16 tiles of V^T P^T
+  constexpr int CH = D / 8;      // channels of o per lane and row
+  constexpr int ROWS = L::ROWS;
   extern __shared__ __align__(16) uint8_t smem[];
+  // the last piece of a warp's range, where it is not a whole row: its row (or -1), whether it begins / ends the row, the
+  // row's last range
+  __shared__ int s_row[SK_WARPS], s_edge[SK_WARPS], s_owner[SK_WARPS];
+  __shared__ float s_m[SK_WARPS][ROWS], s_l[SK_WARPS][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int heads = a.Hkv * a.row_tiles;  // rows (of tiles) per sequence
@@ -151,13 +182,14 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= heads;
   const int64_t ranges = min((int64_t)gridDim.x * SK_WARPS, total);  // no more ranges than units: none is empty
-  const int64_t range = (int64_t)blockIdx.x + (int64_t)warp * gridDim.x;  // neighbours in the list run on different SMs
-  if (range >= ranges) return;
-  int64_t pos = range_start(range, total, ranges);
-  const int64_t end = range_start(range + 1, total, ranges);
+  if ((int64_t)blockIdx.x * SK_WARPS >= ranges) return;
+  const int64_t range = (int64_t)blockIdx.x * SK_WARPS + warp;  // neighbours in the list join in shared memory
+  int64_t pos = range < ranges ? range_start(range, total, ranges) : 0;
+  const int64_t end = range < ranges ? range_start(range + 1, total, ranges) : 0;
+  if (lane == 0) s_row[warp] = -1;
   int b = 0;
   int64_t prefix = 0;  // index of sequence b's first unit
-  for (int b0 = 0;; b0 += 32) {
+  for (int b0 = 0; pos < end && b0 < a.B; b0 += 32) {
     const int64_t mine = b0 + lane < a.B ? row_units(seq_tiles(seq_len(a, b0 + lane))) * heads : 0;
     int64_t upto = mine;
 #pragma unroll
@@ -173,14 +205,25 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
       break;
     }
     prefix += __shfl_sync(0xffffffffu, upto, 31);
-    if (b0 + 32 >= a.B) return;  // not reached: pos lies before total
   }
 
   uint8_t* ring = smem + warp * L::WARP_RING;
   const uint32_t ring_u32 = smem_u32(ring);
-  float* scale_ring = reinterpret_cast<float*>(smem + L::RING) + warp * SK_STAGES * 2;
+  float* scale_ring = reinterpret_cast<float*>(smem + L::RING) + warp * L::STAGES * 2;
   const uint32_t scale_u32 = smem_u32(scale_ring);
   const uint8_t* const no_bytes = a.k;  // a readable address for zero-filled pieces
+  const int page_mask = (1 << a.page_shift) - 1, page_bytes = D << a.page_shift;
+  // What this lane copies: 16 bytes at 16 * lane of every 512. Where they go: K with its 32-byte units swizzled by the
+  // token's parity (D = 128; at 64 two tokens share a 128-byte line and need none), V by the token's pair.
+  const uint8_t* const k_lane = a.k + lane * 16;
+  const uint8_t* const v_lane = a.v + lane * 16;
+  const uint32_t k_to = D == 128 ? (lane * 16) ^ (((lane >> 3) & 1) << 6) : lane * 16;
+  const uint32_t v_to = D == 128 ? (lane * 16) ^ ((lane >> 4) << 5) : (lane * 16) ^ (((lane >> 3) & 3) << 5);
+  const int copy_row = D == 128 ? lane >> 3 : lane >> 2;  // token within a copy instruction
+  // Where this lane's fragments are: K chunk c at ^ 64 c, V's odd tokens at + 128 (D = 128) or ^ 64 (D = 64)
+  const int k_from = D == 128 ? g * 128 + (((t >> 1) ^ ((g & 1) << 1)) << 5) + (t & 1) * 16 : g * 64 + t * 16;
+  const int v_from = D == 128 ? t * 256 + (((g >> 1) ^ t) << 5) + (g & 1) * 16 : t * 128 + (((g >> 2) ^ t) << 5) + (g & 3) * 8;
+  const float* const scale_lane = lane == 0 ? a.ks : a.vs;
 
   while (pos < end) {
     // ---- the next row and the part of it that is ours ----
@@ -201,62 +244,60 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
     pos = min(end, tile0 + tiles);
     if (tb <= ta) continue;  // only what a row counts beside its tiles
     const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
-    const int rows = min(SK_ROWS, a.G * a.Sq - rt * SK_ROWS);
+    const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int nsub = tb - ta;
 
-    // lane j holds the page of tile i0 + j of this warp's list, for the 32 tiles that are issued now and the next 32
-    auto page_of = [&](int i) {
-      const int s = ta + i;
-      return i < nsub ? kv8_page_id(table, ((int64_t)s * 16) >> a.page_shift, a.num_pages, a.status) : 0;
+    // lane j holds the (page, head) of tile i0 + j of this part, for the 32 tiles that are issued now and the next 32
+    auto unit_of = [&](int i) {
+      return i < nsub ? kv8_page_id(table, ((int64_t)(ta + i) * SK_TILE) >> a.page_shift, a.num_pages, a.status) * a.Hkv + hkv : 0;
     };
-    int pid_now = page_of(lane), pid_next = page_of(32 + lane);
+    int unit_now = unit_of(lane), unit_next = unit_of(32 + lane);
+    int slot = 0;  // ring slot that is filled next
     auto issue = [&](int i) {
       if (i < nsub) {
         if ((i & 31) == 0 && i > 0) {
-          pid_now = pid_next;
-          pid_next = page_of(i + 32 + lane);
+          unit_now = unit_next;
+          unit_next = unit_of(i + 32 + lane);
         }
-        const int pid = __shfl_sync(0xffffffffu, pid_now, i & 31);
-        const int s = ta + i;
-        const int64_t unit = (int64_t)pid * a.Hkv + hkv;
-        const int64_t at = ((unit << a.page_shift) + ((s * 16) & ((1 << a.page_shift) - 1))) * D;
-        const int left = len - s * 16;  // tokens of this tile that exist: the others are zeros, whatever the page holds
-        const uint32_t st = ring_u32 + (i % SK_STAGES) * L::STAGE;
-        const uint8_t* kp = a.k + at;
-        const uint8_t* vp = a.v + at;
+        const int unit = __shfl_sync(0xffffffffu, unit_now, i & 31);
+        const int first = (ta + i) * SK_TILE;
+        const int64_t at = (int64_t)unit * page_bytes + (first & page_mask) * D;
+        const uint32_t sk = ring_u32 + slot * L::STAGE + k_to, sv = ring_u32 + slot * L::STAGE + L::HALF;
+        const uint8_t* kp = k_lane + at;
+        const uint8_t* vp = v_lane + at;
+        const int left = len - first;
+        if (left >= SK_TILE) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int tok = u * 8 + g;
+          for (int u = 0; u < L::COPIES; ++u) cp_async16(sk + u * 512, kp + u * 512);
 #pragma unroll
-          for (int c = 0; c < L::K_CHUNKS / 2; ++c)
-            cp_async16(st + (u * (L::K_CHUNKS / 2) + c) * 512 + lane * 16,
-                       tok < left ? kp + tok * D + c * 64 + t * 16 : no_bytes, tok < left ? 16 : 0);
+          for (int u = 0; u < L::COPIES; ++u) cp_async16(sv + u * 512 + (D == 128 ? v_to ^ ((u & 1) << 6) : v_to), vp + u * 512);
+        } else {  // the sequence's last tile: tokens behind its end are zeros, whatever the page holds
+#pragma unroll
+          for (int u = 0; u < L::COPIES; ++u) {
+            const bool in = u * (SK_TILE / L::COPIES) + copy_row < left;
+            cp_async16(sk + u * 512, in ? kp + u * 512 : no_bytes, in ? 16 : 0);
+            cp_async16(sv + u * 512 + (D == 128 ? v_to ^ ((u & 1) << 6) : v_to), in ? vp + u * 512 : no_bytes, in ? 16 : 0);
+          }
         }
-        const uint32_t sv = st + 16 * D;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int tok = 2 * t + (u & 1) + (u >> 1) * 8;
-          if (D == 128)
-            cp_async16(sv + u * 512 + lane * 16, tok < left ? vp + tok * D + g * 16 : no_bytes, tok < left ? 16 : 0);
-          else
-            cp_async8(sv + u * 256 + lane * 8, tok < left ? vp + tok * D + g * 8 : no_bytes, tok < left ? 8 : 0);
-        }
-        if (lane < 2) cp_async4(scale_u32 + ((i % SK_STAGES) * 2 + lane) * 4, (lane == 0 ? a.ks : a.vs) + unit);
+        if (lane < 2) cp_async4(scale_u32 + (slot * 2 + lane) * 4, scale_lane + unit);
+        slot = slot + 1 == L::STAGES ? 0 : slot + 1;
       }
       cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < SK_STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < L::STAGES - 1; ++i) issue(i);
 
-    // ---- q: rows g and g + 8 of the tile, channels as the K fragment has them ----
-    uint32_t qf[STEPS][4];
-    float qs[2];
-    int limit[2];  // tokens that the row sees
+    // ---- q: row g of each 8-row tile, channels as the K fragment has them ----
+    uint32_t qf[RT][STEPS][2];
+    // of the rows whose logits this lane gets, 2 t and 2 t + 1 of each tile: factor of the logits, tokens that the row sees
+    float qs[RT][2];
+    int limit[RT][2];
+    int limit_min = len;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + r * 8;
-      const int rr = rt * SK_ROWS + row;
+    for (int n = 0; n < RT; ++n) {
+      const int row = n * 8 + g;
+      const int rr = rt * ROWS + row;
       const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
       const bool valid = row < rows;
       const __nv_bfloat16* qp = a.q + ((int64_t)b * a.Sq + (valid ? qi : 0)) * a.ld_q + (int64_t)(valid ? head : 0) * D + t * 16;
@@ -280,113 +321,165 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
       // 2^(14 - exponent of the largest), within the normal floats
       const int e = min(max(127 + 14 - ((int)(__float_as_uint(amax) >> 23) - 127), 1), 253);
       const float up = __uint_as_float((uint32_t)e << 23);
-      qs[r] = amax <= 3.402823466e38f ? a.scale_log2 / up : __uint_as_float(0x7fc00000u);  // a row with no finite scores
+      const float factor = amax <= 3.402823466e38f ? a.scale_log2 / up : __uint_as_float(0x7fc00000u);  // a row with no finite scores
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {  // step j: channels 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1}, {2, 3}
         const uint32_t lo = raw[(j >> 2) * 8 + (j & 3) * 2], hi = raw[(j >> 2) * 8 + (j & 3) * 2 + 1];
-        qf[j][r] = pack_f16x2(bf16_lo(lo) * up, bf16_hi(lo) * up);
-        qf[j][2 + r] = pack_f16x2(bf16_lo(hi) * up, bf16_hi(hi) * up);
+        qf[n][j][0] = pack_f16x2(bf16_lo(lo) * up, bf16_hi(lo) * up);
+        qf[n][j][1] = pack_f16x2(bf16_lo(hi) * up, bf16_hi(hi) * up);
       }
-      limit[r] = valid ? max(len - a.Sq + qi + 1, 0) : len;  // rows past the last are computed and dropped
+      const int sees = valid ? max(len - a.Sq + qi + 1, 0) : len;  // rows past the last are computed and dropped
+      limit_min = min(limit_min, __reduce_min_sync(0xffffffffu, sees));
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        qs[n][e2] = __shfl_sync(0xffffffffu, factor, (2 * t + e2) * 4);
+        limit[n][e2] = __shfl_sync(0xffffffffu, sees, (2 * t + e2) * 4);
+      }
     }
-    const int limit_min = __reduce_min_sync(0xffffffffu, min(limit[0], limit[1]));
 
-    float o[NT][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // o[n][j][2 x + e]: row n * 8 + 2 t + e, channel CH * g + 2 j + x
+    float o[RT][STEPS][4];
+    // running maximum of logit + log2 v_scale, what is added to a logit (P_SHIFT - maximum), sum
+    float m[RT][2], shift[RT][2], l[RT][2];
+    bool big = false;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int n = 0; n < RT; ++n) {
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        shift[n][e] = INFINITY;
+        l[n][e] = 0.f;
+      }
+    }
 
+    int use = 0;  // ring slot that is used next
     for (int i = 0; i < nsub; ++i) {
-      __syncwarp();  // all lanes have read the scales of the stage that is overwritten next
-      issue(i + SK_STAGES - 1);
-      cp_async_wait<SK_STAGES - 1>();
+      __syncwarp();  // all lanes have read the slot that is filled next
+      issue(i + L::STAGES - 1);
+      cp_async_wait<L::STAGES - 1>();
       __syncwarp();
-      const uint8_t* st = ring + (i % SK_STAGES) * L::STAGE;
-      const float ks = scale_ring[(i % SK_STAGES) * 2];
-      const float vs_raw = scale_ring[(i % SK_STAGES) * 2 + 1];
-      const float vs = max_nan(vs_raw, V_SCALE_MIN);
+      const uint8_t* st = ring + use * L::STAGE;
+      const uint8_t* sv = st + L::HALF;
+      const float2 scales = *reinterpret_cast<const float2*>(scale_ring + use * 2);
+      use = use + 1 == L::STAGES ? 0 : use + 1;
 
-      // ---- logits: 16 rows x 16 tokens ----
-      float s[2][4];
+      // ---- logits: 16 tokens x 8 RT rows, two partial sums each ----
+      float s[RT][4];
+      {
+        float s2[RT][2][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+        for (int n = 0; n < RT; ++n) {
 #pragma unroll
-        for (int c = 0; c < L::K_CHUNKS / 2; ++c) {
-          const uint4 kv = *reinterpret_cast<const uint4*>(st + (u * (L::K_CHUNKS / 2) + c) * 512 + lane * 16);
-          const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mma_f16(s[u], qf[c * 4 + j], e4m3x2_f16x2(w[j]), e4m3x2_f16x2(w[j] >> 16));
-        }
-      }
-      const float c0 = qs[0] * ks, c1 = qs[1] * ks;
-      const float lvs = lg2(vs), inv_vs = 1.0f / vs;
-      const int tok0 = (ta + i) * 16 + 2 * t;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u][0] = fmaf(s[u][0], c0, lvs);
-        s[u][1] = fmaf(s[u][1], c0, lvs);
-        s[u][2] = fmaf(s[u][2], c1, lvs);
-        s[u][3] = fmaf(s[u][3], c1, lvs);
-      }
-      if (tok0 - 2 * t + 16 > limit_min) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (tok0 + u * 8 + (e & 1) >= limit[e >> 1]) s[u][e] = -INFINITY;
-        }
-      }
-      // ---- running maximum (of logit + log2 v_scale), moved only when it would be passed by more than 2^LAZY ----
-      float mx[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      }
-      if (__any_sync(0xffffffffu, mx[0] - m[0] > LAZY || mx[1] - m[1] > LAZY)) {  // (a difference: m + 7 may round up)
-        float f[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float to = fmaxf(m[r], mx[r]);
-          f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - to);
-          m[r] = to;
-          l[r] *= f[r];
+          for (int x = 0; x < 4; ++x) s2[n][0][x] = s2[n][1][x] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          o[j][0] *= f[0];
-          o[j][1] *= f[0];
-          o[j][2] *= f[1];
-          o[j][3] *= f[1];
+        for (int c = 0; c < L::K_CHUNKS; ++c) {
+          const uint4 ka = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)));            // token g
+          const uint4 kb = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)) + 8 * D);  // token 8 + g
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_f16x4(j == 0 ? ka.x : j == 1 ? ka.y : j == 2 ? ka.z : ka.w, a0, a2);
+            e4m3x4_f16x4(j == 0 ? kb.x : j == 1 ? kb.y : j == 2 ? kb.z : kb.w, a1, a3);
+#pragma unroll
+            for (int n = 0; n < RT; ++n) mma_f16(s2[n][j & 1], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < RT; ++n) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[n][x] = s2[n][0][x] + s2[n][1][x];
         }
       }
-      const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-      float p[2][4];
+      const float ks = scales.x;
+      const float vs = max_nan(scales.y, V_SCALE_MIN);
+      const float lvs = lg2(vs);
+      const int tok = (ta + i) * SK_TILE + g;
+      const bool edge = (ta + i) * SK_TILE + SK_TILE > limit_min;  // some row does not see all of the tile
+      // p[n][2 u + e]: row n * 8 + 2 t + e, token tok + 8 u. A row that has seen nothing yet has an infinite shift: its
+      // first visible logit makes the maximum move.
+      float p[RT][4];
+      auto exponents = [&]() {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int n = 0; n < RT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[u][e] = ex2((s[u][e] - sub[e >> 1]) + P_SHIFT);
+          for (int x = 0; x < 4; ++x) p[n][x] = fmaf(s[n][x], qs[n][x & 1] * ks, lvs + shift[n][x & 1]);
+          if (edge) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (tok + (x >> 1) * 8 >= limit[n][x & 1]) p[n][x] = -INFINITY;
+          }
+        }
+      };
+      exponents();
+      float most = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < RT; ++n) most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])));
+      if (__any_sync(0xffffffffu, most > P_LIMIT)) {  // rare after a row's first tiles: no shuffles otherwise
+        big = false;
+#pragma unroll
+        for (int n = 0; n < RT; ++n) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              if (!edge || tok + u * 8 < limit[n][e]) mx = fmaxf(mx, fmaf(s[n][2 * u + e], qs[n][e] * ks, lvs));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float to = fmaxf(m[n][e], mx);
+            f[e] = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - to);
+            m[n][e] = to;
+            shift[n][e] = P_SHIFT - to;
+            l[n][e] *= f[e];
+            big = big || (to != -INFINITY && fabsf(to) > BIG);
+          }
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j) {
+            o[n][j][0] *= f[0];
+            o[n][j][1] *= f[1];
+            o[n][j][2] *= f[0];
+            o[n][j][3] *= f[1];
+          }
+        }
+        big = __any_sync(0xffffffffu, big);
+        exponents();
       }
+      if (big) {  // logits that differ by a rounding may differ by more than fp16 holds
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-        l[r] = fmaf((p[0][2 * r] + p[0][2 * r + 1]) + (p[1][2 * r] + p[1][2 * r + 1]), inv_vs, l[r]);
-      const uint32_t pa[4] = {pack_f16x2(p[0][0], p[0][1]), pack_f16x2(p[0][2], p[0][3]), pack_f16x2(p[1][0], p[1][1]),
-                              pack_f16x2(p[1][2], p[1][3])};
-      if (vs_raw == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
-      // ---- o += P V: n8 tile j has the channels j, NT + j, 2 NT + j, ... ----
+        for (int n = 0; n < RT; ++n) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) p[n][x] = p[n][x] > P_LIMIT ? P_LIMIT : p[n][x];
+        }
+      }
+      const float inv_vs = rcp(vs);
+      uint32_t pb[RT][2];  // P^T: row g, tokens 2 t, 2 t + 1 (+ 8)
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p[n][x] = ex2(p[n][x]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[n][e] = fmaf(p[n][e] + p[n][2 + e], inv_vs, l[n][e]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) pb[n][u] = transpose8x8(pack_f16x2(p[n][2 * u], p[n][2 * u + 1]));
+      }
+      if (scales.y == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
+      // ---- o^T += V^T P^T ----
       uint32_t w[4][L::V_BYTES / 4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if constexpr (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4*>(st + 16 * D + u * 512 + lane * 16);
+          const uint4 v = *reinterpret_cast<const uint4*>(sv + v_from + (u & 1) * 128 + (u >> 1) * 1024);
           w[u][0] = v.x;
           w[u][1] = v.y;
           w[u][2] = v.z;
           w[u][3] = v.w;
         } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(st + 16 * D + u * 256 + lane * 8);
+          const uint2 v = *reinterpret_cast<const uint2*>(sv + (v_from ^ ((u & 1) * 64)) + (u >> 1) * 512);
           w[u][0] = v.x;
           w[u][1] = v.y;
         }
@@ -394,123 +487,222 @@ __global__ void __launch_bounds__(SK_THREADS, SK_CTAS_PER_SM) sdpa_kv8_kernel(co
 #pragma unroll
       for (int j = 0; j < L::V_BYTES / 4; ++j) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t a01 = __byte_perm(w[0][j], w[1][j], half == 0 ? 0x5140 : 0x7362);
-          const uint32_t a89 = __byte_perm(w[2][j], w[3][j], half == 0 ? 0x5140 : 0x7362);
-          mma_f16(o[j * 4 + half * 2], pa, e4m3x2_f16x2(a01), e4m3x2_f16x2(a89));
-          mma_f16(o[j * 4 + half * 2 + 1], pa, e4m3x2_f16x2(a01 >> 16), e4m3x2_f16x2(a89 >> 16));
+        for (int half = 0; half < 2; ++half) {  // channels 4 j + 2 half (rows g of the tile) and the next (rows 8 + g)
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_f16x4(__byte_perm(w[0][j], w[1][j], half == 0 ? 0x5140 : 0x7362), a0, a1);
+          e4m3x4_f16x4(__byte_perm(w[2][j], w[3][j], half == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+          for (int n = 0; n < RT; ++n) mma_f16(o[n][j * 2 + half], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
       }
     }
 
-    // ---- this range's part of the row: channels [2 t NT, (2 t + 2) NT) of rows g and g + 8 per lane ----
+    // ---- this range's part of the row: channels [CH g, CH (g + 1)) of rows 2 t and 2 t + 1 of each tile per lane ----
     cp_async_wait<0>();
     const bool whole = ta == 0 && tb == tiles;
+    const bool last = !whole && pos >= end;  // may go on in the next warp's range: left in shared memory
+    if (last) __syncwarp();                   // every lane is done with the ring
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      const int row = g + 8 * r;
-      if (row < rows) {
+    for (int n = 0; n < RT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[n][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int row = n * 8 + 2 * t + e;
+        if (row >= rows) continue;
         if (whole) {
-          const int rr = rt * SK_ROWS + row;
+          const int rr = rt * ROWS + row;
           const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
-          const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
-          __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + 2 * t * NT;
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + g * CH;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int j = 0; j < NT; j += 8)
-              *reinterpret_cast<uint4*>(out + c * NT + j) =
-                  make_uint4(pack_bf16x2(o[j][2 * r + c] * inv, o[j + 1][2 * r + c] * inv),
-                             pack_bf16x2(o[j + 2][2 * r + c] * inv, o[j + 3][2 * r + c] * inv),
-                             pack_bf16x2(o[j + 4][2 * r + c] * inv, o[j + 5][2 * r + c] * inv),
-                             pack_bf16x2(o[j + 6][2 * r + c] * inv, o[j + 7][2 * r + c] * inv));
-          }
+          for (int j = 0; j < STEPS; j += 4)
+            *reinterpret_cast<uint4*>(out + 2 * j) =
+                make_uint4(pack_bf16x2(o[n][j][e] * inv, o[n][j][2 + e] * inv), pack_bf16x2(o[n][j + 1][e] * inv, o[n][j + 1][2 + e] * inv),
+                           pack_bf16x2(o[n][j + 2][e] * inv, o[n][j + 2][2 + e] * inv),
+                           pack_bf16x2(o[n][j + 3][e] * inv, o[n][j + 3][2 + e] * inv));
         } else {
-          // the first part of a row ends its range (slot 1), any other begins it (slot 0)
-          const int64_t at = (range * 2 + (ta == 0 ? 1 : 0)) * a.row_cap + row;
-          if (t == 0) a.ml[at] = make_float2(m[r], l[r]);
-          float* out = a.part + at * D + 2 * t * NT;
+          // (the first part of a row ends its range and takes slot 1, any other begins it and takes slot 0)
+          const int64_t at = range * 2 * a.row_cap + row;
+          if (g == 0) (last ? s_m[warp][row] : a.ml[at].x) = m[n][e];
+          if (g == 0) (last ? s_l[warp][row] : a.ml[at].y) = sum;
+          float* out = (last ? reinterpret_cast<float*>(ring) + row * L::PIECE_PITCH : a.part + at * D) + g * CH;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int j = 0; j < NT; j += 4)
-              *reinterpret_cast<float4*>(out + c * NT + j) =
-                  make_float4(o[j][2 * r + c], o[j + 1][2 * r + c], o[j + 2][2 * r + c], o[j + 3][2 * r + c]);
-          }
+          for (int j = 0; j < STEPS; j += 2)
+            *reinterpret_cast<float4*>(out + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
         }
       }
     }
-    if (ta == 0 && lane == 0)
-      a.info[(int64_t)b * heads + hr] = make_int2((int)range, (int)range_owner(tile0 + tiles - 1, total, ranges));
+    if (lane == 0) {
+      const int row = b * heads + hr;
+      if (whole) a.info[row] = make_int2((int)range, (int)range);
+      if (last) {
+        s_row[warp] = row;
+        s_edge[warp] = (ta == 0 ? 1 : 0) | (tb == tiles ? 2 : 0);
+        s_owner[warp] = (int)range_owner(tile0 + tiles - 1, total, ranges);
+      }
+    }
     __syncwarp();
+  }
+
+  // ---- the last pieces of the CTA's warps: neighbours that belong to one row become one piece ----
+  __syncthreads();
+  for (int w0 = 0; w0 < SK_WARPS; ++w0) {
+    const int row_id = s_row[w0];
+    if (row_id < 0 || (w0 > 0 && s_row[w0 - 1] == row_id)) continue;
+    int w1 = w0 + 1;
+    while (w1 < SK_WARPS && s_row[w1] == row_id) ++w1;
+    const int seq = row_id / heads, hr = row_id - seq * heads;
+    const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
+    const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
+    const bool begins = (s_edge[w0] & 1) != 0, whole = begins && (s_edge[w1 - 1] & 2) != 0;
+    const int64_t first = (int64_t)blockIdx.x * SK_WARPS + w0;  // range of the run's first piece
+    constexpr int TPR = SK_THREADS / ROWS, N = D / TPR;         // threads per row, channels per thread
+    const int row = threadIdx.x / TPR, col = (threadIdx.x % TPR) * N;
+    if (row < rows) {
+      float top = -INFINITY;
+      for (int w = w0; w < w1; ++w) top = fmaxf(top, s_m[w][row]);
+      float sum = 0.f, acc[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = 0.f;
+      for (int w = w0; w < w1; ++w) {
+        // a piece without a visible token has -inf here, zeros (or, through a NaN, NaN) in its sums
+        const float f = s_m[w][row] == -INFINITY ? 1.f : ex2(s_m[w][row] - top);
+        sum = fmaf(s_l[w][row], f, sum);
+        const float* from = reinterpret_cast<const float*>(smem + w * L::WARP_RING) + row * L::PIECE_PITCH + col;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(from + j);
+          acc[j] = fmaf(v.x, f, acc[j]);
+          acc[j + 1] = fmaf(v.y, f, acc[j + 1]);
+          acc[j + 2] = fmaf(v.z, f, acc[j + 2]);
+          acc[j + 3] = fmaf(v.w, f, acc[j + 3]);
+        }
+      }
+      if (whole) {
+        const int rr = rt * ROWS + row;
+        const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        __nv_bfloat16* out = a.o + (((int64_t)seq * a.Sq + qi) * a.Hq + head) * D + col;
+#pragma unroll
+        for (int j = 0; j < N; j += 4)
+          *reinterpret_cast<uint2*>(out + j) =
+              make_uint2(pack_bf16x2(acc[j] * inv, acc[j + 1] * inv), pack_bf16x2(acc[j + 2] * inv, acc[j + 3] * inv));
+      } else {
+        const int64_t at = (first * 2 + (begins ? 1 : 0)) * a.row_cap + row;
+        if (col == 0) {
+          a.ml[at] = make_float2(top, sum);
+          // the others' places in the row's list stay empty
+          for (int w = w0 + 1; w < w1; ++w) a.ml[(first + w - w0) * 2 * a.row_cap + row] = make_float2(-INFINITY, 0.f);
+        }
+        float* out = a.part + at * D + col;
+#pragma unroll
+        for (int j = 0; j < N; j += 4)
+          *reinterpret_cast<float4*>(out + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      }
+    }
+    if (begins && threadIdx.x == 0) a.info[row_id] = make_int2((int)first, whole ? (int)first : s_owner[w0]);
   }
 }
 
-// Joins the ranges of every row that was cut: block (row of tiles, row of the tile), the partial results dealt to warps.
-template <int D>
-__global__ void __launch_bounds__(SK_JOIN_WARPS * 32) sdpa_kv8_join_kernel(const SdpaArgs a) {
+// Joins the pieces of every row that was cut: block (row of tiles, row of the tile). The places of a row's pieces are
+// consecutive ranges; those that were joined within a CTA are empty (maximum -inf, sum 0) but for the first.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) sdpa_kv8_join_kernel(const SdpaArgs a) {
   constexpr int E = D / 32;  // channels per lane
-  __shared__ float s_m[SK_JOIN_WARPS], s_l[SK_JOIN_WARPS];
-  __shared__ float s_o[SK_JOIN_WARPS][D];
+  __shared__ int s_at[WARPS * 32];    // places that hold something, and their factors
+  __shared__ float s_f[WARPS * 32];
+  __shared__ int s_n[WARPS];
+  __shared__ float s_m[WARPS], s_l[WARPS];
+  __shared__ float s_o[WARPS][D];
   grid_dependency_wait();
   grid_launch_dependents();
   const int heads = a.Hkv * a.row_tiles;
   const int b = blockIdx.x / heads, hr = blockIdx.x - b * heads;
   const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
-  const int rr = rt * SK_ROWS + blockIdx.y;
+  const int rr = rt * a.tile_rows + blockIdx.y;
+  const int2 span = a.info[blockIdx.x];  // (of an empty sequence: not written, not used)
+  const int len = seq_len(a, b);
   if (rr >= a.G * a.Sq) return;
   const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D;
-  if (seq_len(a, b) == 0) {  // no tile, so no warp wrote this row
+  if (len == 0) {  // no tile, so no warp wrote this row
     if (threadIdx.x < D / 8) reinterpret_cast<uint4*>(out)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int2 span = a.info[blockIdx.x];
   if (span.x == span.y) return;
-  float m = -INFINITY, l = 0.f, o[E];
+  float m = -INFINITY, l = 0.f, o[E];  // m is the same in all threads, l and o are this warp's part
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int c = span.x + warp; c <= span.y; c += SK_JOIN_WARPS) {
-    const int64_t at = ((int64_t)c * 2 + (c == span.x ? 1 : 0)) * a.row_cap + blockIdx.y;
-    const float2 ml = a.ml[at];
-    const float* p = a.part + at * D + lane * E;
-    float v[E];
-    if constexpr (E == 4) {
-      const float4 u = *reinterpret_cast<const float4*>(p);
-      v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-    } else {
-      const float2 u = *reinterpret_cast<const float2*>(p);
-      v[0] = u.x; v[1] = u.y;
+  for (int c0 = span.x; c0 <= span.y; c0 += WARPS * 32) {
+    // ---- a place per thread: the block's maximum, and a list of those that hold something ----
+    const int c = c0 + (int)threadIdx.x;
+    int at = 0;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (c <= span.y) {
+      at = c * 2 + (c == span.x ? 1 : 0);
+      ml = a.ml[(int64_t)at * a.row_cap + blockIdx.y];
     }
-    const float top = fmaxf(m, ml.x);
-    const float f0 = m == -INFINITY ? 1.f : ex2(m - top), f1 = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);
-    m = top;
-    l = fmaf(l, f0, ml.y * f1);
+    const bool holds = ml.x != -INFINITY || ml.y != 0.f;  // (a NaN sum counts)
+    const unsigned mask = __ballot_sync(0xffffffffu, holds);
+    const float wm = warp_max(ml.x);
+    if (lane == 0) {
+      s_n[warp] = __popc(mask);
+      s_m[warp] = wm;
+    }
+    __syncthreads();
+    float top = m;
+    int before = 0, n = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], f0, v[e] * f1);
+    for (int w = 0; w < WARPS; ++w) {
+      top = fmaxf(top, s_m[w]);
+      before += w < warp ? s_n[w] : 0;
+      n += s_n[w];
+    }
+    if (holds) {
+      const int i = before + __popc(mask & ((1u << lane) - 1));
+      s_at[i] = at;
+      s_f[i] = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);
+    }
+    const float keep = m == -INFINITY ? 1.f : ex2(m - top);
+    m = top;
+    // each thread adds its own place's sum; the warps share the outputs out
+    l = fmaf(l, keep, holds ? ml.y * (ml.x == -INFINITY ? 1.f : ex2(ml.x - top)) : 0.f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= keep;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = warp; i < n; i += WARPS) {
+      const float f = s_f[i];
+      const float* p = a.part + ((int64_t)s_at[i] * a.row_cap + blockIdx.y) * D + lane * E;
+      float v[E];
+      if constexpr (E == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(p);
+        v[0] = u.x; v[1] = u.y;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], f, o[e]);
+    }
+    __syncthreads();
   }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
+  l = warp_sum(l);
+  if (lane == 0) s_l[warp] = l;
 #pragma unroll
   for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
   __syncthreads();
   if (threadIdx.x < D / 2) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < SK_JOIN_WARPS; ++w) top = fmaxf(top, s_m[w]);
     float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < SK_JOIN_WARPS; ++w) {
-      const float f = s_m[w] == -INFINITY ? 1.f : ex2(s_m[w] - top);
-      sum = fmaf(s_l[w], f, sum);
-      x = fmaf(s_o[w][threadIdx.x * 2], f, x);
-      y = fmaf(s_o[w][threadIdx.x * 2 + 1], f, y);
+    for (int w = 0; w < WARPS; ++w) {
+      sum += s_l[w];
+      x += s_o[w][threadIdx.x * 2];
+      y += s_o[w][threadIdx.x * 2 + 1];
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     reinterpret_cast<uint32_t*>(out)[threadIdx.x] = pack_bf16x2(x * inv, y * inv);
@@ -519,28 +711,32 @@ __global__ void __launch_bounds__(SK_JOIN_WARPS * 32) sdpa_kv8_join_kernel(const
 
 int64_t align16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
+// Up to eight rows that share a KV head go as one tile of 8; more as tiles of 16, each reading the cache once.
+int tile_rows_of(int64_t rows) { return rows <= 8 ? 8 : 16; }
+
 // Every product of the sizes that the kernels form in 32 bits fits.
 bool sizes_ok(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv) {
   const int64_t limit = 0x7fffffff;
   if (B <= 0 || Sq <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return false;
   if (B > limit || Sq > limit || Hq > limit || Sq > limit / (Hq / Hkv)) return false;
-  const int64_t row_tiles = (Hq / Hkv * Sq + SK_ROWS - 1) / SK_ROWS;
+  const int64_t rows = Hq / Hkv * Sq, row_tiles = (rows + tile_rows_of(rows) - 1) / tile_rows_of(rows);
   return Hkv <= limit / row_tiles && B <= limit / (Hkv * row_tiles);
 }
 
 struct SkPlan {
-  int row_tiles, row_cap;
+  int row_tiles, tile_rows, row_cap;
   int64_t ctas, info_bytes, ml_bytes, part_bytes;
 };
 
 // The grid never has more warps than the longest possible list has units.
 SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t max_tokens, int64_t D) {
   SkPlan p;
-  p.row_tiles = (int)((Hq / Hkv * Sq + SK_ROWS - 1) / SK_ROWS);
-  p.row_cap = Hq / Hkv * Sq < SK_ROWS ? (int)(Hq / Hkv * Sq) : SK_ROWS;
+  p.tile_rows = tile_rows_of(Hq / Hkv * Sq);
+  p.row_tiles = (int)((Hq / Hkv * Sq + p.tile_rows - 1) / p.tile_rows);
+  p.row_cap = Hq / Hkv * Sq < p.tile_rows ? (int)(Hq / Hkv * Sq) : p.tile_rows;
   const int64_t units = (max_tokens + SK_TILE - 1) / SK_TILE + ROW_COST;  // below 2^28
   const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
-  p.ctas = (int64_t)sm_count * SK_CTAS_PER_SM;
+  p.ctas = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
   if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
   p.info_bytes = align16(rows * (int64_t)sizeof(int2));
   p.ml_bytes = align16(p.ctas * SK_WARPS * 2 * p.row_cap * (int64_t)sizeof(float2));
@@ -548,29 +744,36 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   return p;
 }
 
-template <int D>
+template <int D, int RT>
 int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t s) {
   static emk_device_once once;
   {
     std::lock_guard<std::mutex> lk(once.mu);
     if (!once.done[h->device]) {
-      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
       once.done[h->device] = true;
     }
   }
-  EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_kernel<D>, (unsigned)p.ctas, SK_THREADS, SkLayout<D>::SMEM, s,
+  EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_kernel<D, RT>, (unsigned)p.ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
                                         h->overlap_launch != 0, a));
   EMK_LAUNCH_CHECK(h);
+  // Few rows: a row may be cut into hundreds of pieces, and sixteen warps share them; many rows: a few pieces each.
+  const int64_t blocks = (int64_t)a.B * a.Hkv * a.row_tiles * a.row_cap;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_tiles), (unsigned)a.row_cap, 1);
-  cfg.blockDim = dim3(SK_JOIN_WARPS * 32, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = h->overlap_launch != 0 ? 1 : 0;
-  EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, sdpa_kv8_join_kernel<D>, a));
+  if (blocks <= (int64_t)h->sm_count * 4) {
+    cfg.blockDim = dim3(16 * 32, 1, 1);
+    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, sdpa_kv8_join_kernel<D, 16>, a));
+  } else {
+    cfg.blockDim = dim3(4 * 32, 1, 1);
+    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, sdpa_kv8_join_kernel<D, 4>, a));
+  }
   EMK_LAUNCH_CHECK(h);
   return EMK_OK;
 }
@@ -599,8 +802,8 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   if (B <= 0 || Sq <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_pages <= 0 || num_pages <= 0 ||
       num_pages > 0x7fffffff || max_pages > 0x7fffffff / page || ld_q / D < Hq)
     return EMK_ERR_SHAPE;
-  if (!sizes_ok(B, Sq, Hq, Hkv)) {
-    EMK_SET_ERR(h, "emk_sdpa_kv8: more than 2^31 - 1 tiles of 16 query rows");
+  if (num_pages > 0x7fffffff / Hkv || !sizes_ok(B, Sq, Hq, Hkv)) {
+    EMK_SET_ERR(h, "emk_sdpa_kv8: more than 2^31 - 1 (page, head) pairs or tiles of query rows");
     return EMK_ERR_LIMIT;
   }
   if (((uintptr_t)q & 15u) != 0 || (ld_q & 7) != 0 || (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)o) & 15u) != 0 ||
@@ -629,6 +832,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   a.Hkv = (int)Hkv;
   a.G = (int)(Hq / Hkv);
   a.row_tiles = p.row_tiles;
+  a.tile_rows = p.tile_rows;
   a.row_cap = p.row_cap;
   a.page_shift = __builtin_ctzll((unsigned long long)page);
   a.max_pages = (int)max_pages;
@@ -639,5 +843,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   a.ml = (float2*)(ws + p.info_bytes);
   a.part = (float*)(ws + p.info_bytes + p.ml_bytes);
   a.status = h->status_dev;
-  return D == 128 ? launch_sdpa<128>(h, a, p, (cudaStream_t)stream) : launch_sdpa<64>(h, a, p, (cudaStream_t)stream);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (D == 128) return p.tile_rows == 8 ? launch_sdpa<128, 1>(h, a, p, s) : launch_sdpa<128, 2>(h, a, p, s);
+  return p.tile_rows == 8 ? launch_sdpa<64, 1>(h, a, p, s) : launch_sdpa<64, 2>(h, a, p, s);
 }
