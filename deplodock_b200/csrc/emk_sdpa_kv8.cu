@@ -7,15 +7,15 @@
 // instruction's 16 rows and the queries as its 8 columns:
 //   S^T [tokens x rows] = K q^T,   o^T [channels x rows] = V^T P^T
 // so that a group of up to eight rows wastes nothing. (At a few rows per cache byte the tensor-memory path would be fed 1/16
-// full tiles; what counts is the flow of bytes and the instructions per byte.) Every warp copies its own tiles with
-// cp.async, a few tiles of 16 tokens ahead, so the loop has no barrier between warps. A copy instruction moves 512
-// contiguous bytes, lane after lane: with lanes that fetch what their own fragments need instead, 16 bytes of four rows side
-// by side, every sector crossed twice and every lane took a shared-memory cycle of its own (2.0x the sectors, 26 cycles an
-// instruction, and that was the bound: 64 sequences of up to 8192 tokens 136 us). 32-byte units are swizzled so that the
-// fragment loads meet no bank twice. The token and channel order inside a fragment is permuted alike for both operands,
-// which a sum does not notice.
-//   K fragment: lane (g, t) holds tokens g and 8 + g, channels 16t.. and 64 + 16t..   (4 bytes = one k16 step)
-//   V fragment: lane (g, t) holds tokens 2t, 2t+1, 2t+8, 2t+9, channels (D/8) g..    (pairs of tokens interleaved by prmt)
+// full tiles; what counts is the flow of bytes and the instructions per byte.) A TMA load brings a tile of 16
+// tokens, 16 rows of one page, into the warp's own ring, a few tiles ahead; nothing in the loop waits for another warp. (With
+// cp.async in the order of the fragments, 16 bytes of four rows side by side, every sector crossed twice and every lane took
+// a shared-memory cycle of its own: 26 cycles an instruction, and that was the bound; in address order the copies still took
+// the cycles that the fragment loads need.) The token and channel order inside a fragment is permuted alike for both
+// operands, which a sum does not notice; the permutation of the tokens is the one that TMA's swizzle makes free of bank
+// conflicts.
+//   K fragment: lane (g, t) holds tokens p(g) and 8 + p(g), channels 16t.. and 64 + 16t..   (4 bytes = one k16 step)
+//   V fragment: lane (g, t) holds tokens p(2t), p(2t+1), 8 + both, channels (D/8) g..       (pairs interleaved by prmt)
 // P^T comes out of S^T by movmatrix.
 //
 // e4m3 -> f16 is exact. q is scaled per row by a power of two into f16's range (exact; elements 2^-38 below the row's
@@ -63,7 +63,9 @@ struct SdpaArgs {
   int2* info;    // [B * Hkv * row_tiles]: first and last range of the row
   float2* ml;    // [ranges][2][row_cap]: maximum, sum
   float* part;   // [ranges][2][row_cap][D]
+  int max_ranges;
   int* status;
+  unsigned long long limit_ns;
 };
 
 __device__ __forceinline__ int seq_len(const SdpaArgs& a, int b) {
@@ -74,23 +76,8 @@ __device__ __forceinline__ int seq_len(const SdpaArgs& a, int b) {
 }
 __device__ __forceinline__ int seq_tiles(int len) { return (int)(((int64_t)len + SK_TILE - 1) / SK_TILE); }
 // what a row of `tiles` tiles counts in the list
-__device__ __forceinline__ int64_t row_units(int tiles) { return tiles > 0 ? (int64_t)tiles + ROW_COST : 0; }
+__device__ __forceinline__ int row_units(int tiles) { return tiles > 0 ? tiles + ROW_COST : 0; }
 
-// `bytes` of src, zeros up to 16
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -138,6 +125,17 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
 __device__ __forceinline__ int64_t range_start(int64_t c, int64_t total, int64_t ranges) { return c * total / ranges; }
 __device__ __forceinline__ int64_t range_owner(int64_t u, int64_t total, int64_t ranges) { return ((u + 1) * ranges - 1) / total; }
 
+// Token of row r of an 8-row fragment half. K is read two rows (r even, r odd) to a quarter warp, V one half of every
+// pair: with TMA's 128-byte swizzle (16-byte unit ^ row % 8) the tokens of a pair have to differ in bit 2 and the even rows'
+// tokens in bits 1 and 2; with the 64-byte swizzle of D = 64 (unit ^ row / 2 % 4, two rows a line) the tokens of a pair in
+// bit 0, and four even rows' tokens have to cover both halves of two lines.
+template <int D>
+__device__ __forceinline__ constexpr int token_of(int r) {
+  if (D == 128) return r ^ ((r & 1) << 2);
+  const int e = ((r >> 1) & 1) | (((r >> 1) & 2) << 1);
+  return (r & 1) ? e ^ 3 : e;
+}
+
 // RT: tiles of 8 rows per row tile. One: 16 warps per SM with a 12 KB ring each; two (twice the accumulators and query
 // fragments): as many warps as hold them in registers, 8 at D = 128 and 12 at D = 64. (A spill inside the loop costs more
 // than a third of the warps: local memory has to pass an L1 that the rings leave a few KB.)
@@ -145,26 +143,30 @@ template <int D, int RT>
 struct SkLayout {
   static constexpr int ROWS = 8 * RT;
   static constexpr int CTAS_PER_SM = RT == 1 ? 4 : D == 128 ? 2 : 3;
-  static constexpr int K_CHUNKS = D / 64;                // 16-byte pieces of K per lane and 8 tokens
-  static constexpr int COPIES = D / 32;                  // copy instructions for K or V of a tile
+  static constexpr int K_CHUNKS = D / 64;                // 16-byte pieces of K per lane and token
   static constexpr int V_BYTES = D / 8;                  // bytes of V per lane and token (16 or 8)
   static constexpr int HALF = SK_TILE * D;               // K or V of a tile
   static constexpr int STAGE = 2 * HALF;
   static constexpr int STAGES = (RT == 1 ? 12 : D == 128 ? 24 : 16) * 1024 / STAGE;
   static constexpr int WARP_RING = STAGES * STAGE;
   static constexpr int RING = SK_WARPS * WARP_RING;
-  static constexpr int SMEM = RING + SK_WARPS * STAGES * 8;  // and the scales of K and V of every stage
+  static constexpr int SMEM = RING + 1024;                // the swizzle wants 1024-byte aligned slots
   static constexpr int PIECE_PITCH = D + 4;              // floats; spreads the rows over the banks
   static_assert(ROWS * PIECE_PITCH * 4 <= WARP_RING, "a warp's last piece lies over its ring");
 };
 
 template <int D, int RT>
-__global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa_kv8_kernel(const SdpaArgs a) {
+__global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa_kv8_kernel(const __grid_constant__ CUtensorMap tma_k,
+                                                                                          const __grid_constant__ CUtensorMap tma_v,
+                                                                                          const SdpaArgs a) {
   using L = SkLayout<D, RT>;
   constexpr int STEPS = D / 16;  // k16 steps of K q^T, and m16 tiles of V^T P^T
   constexpr int CH = D / 8;      // channels of o per lane and row
   constexpr int ROWS = L::ROWS;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t s_full[SK_WARPS][L::STAGES];
+  __shared__ int s_abort;
   // the last piece of a warp's range, where it is not a whole row: its row (or -1), whether it begins / ends the row, the
   // row's last range
   __shared__ int s_row[SK_WARPS], s_edge[SK_WARPS], s_owner[SK_WARPS];
@@ -172,8 +174,17 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int heads = a.Hkv * a.row_tiles;  // rows (of tiles) per sequence
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SK_WARPS * L::STAGES; ++i) mbar_init(&s_full[0][0] + i, 1);
+    s_abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tma_k);
+    tma_prefetch_desc(&tma_v);
+  }
+  __syncthreads();
   grid_dependency_wait();
   grid_launch_dependents();
+  const WaitCtx wc{&s_abort, a.status, a.limit_ns};
 
   // ---- this warp's range of the list ----
   int64_t total = 0;
@@ -184,64 +195,59 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
   const int64_t ranges = min((int64_t)gridDim.x * SK_WARPS, total);  // no more ranges than units: none is empty
   if ((int64_t)blockIdx.x * SK_WARPS >= ranges) return;
   const int64_t range = (int64_t)blockIdx.x * SK_WARPS + warp;  // neighbours in the list join in shared memory
-  int64_t pos = range < ranges ? range_start(range, total, ranges) : 0;
-  const int64_t end = range < ranges ? range_start(range + 1, total, ranges) : 0;
   if (lane == 0) s_row[warp] = -1;
-  int b = 0;
-  int64_t prefix = 0;  // index of sequence b's first unit
-  for (int b0 = 0; pos < end && b0 < a.B; b0 += 32) {
-    const int64_t mine = b0 + lane < a.B ? row_units(seq_tiles(seq_len(a, b0 + lane))) * heads : 0;
-    int64_t upto = mine;
+  // the position in the list: unit `off` of sequence b, `left` units to go (the host admits sizes for which these fit)
+  int b = 0, off = 0, left = 0;
+  if (range < ranges) {
+    int64_t pos = range_start(range, total, ranges);
+    left = (int)(range_start(range + 1, total, ranges) - pos);
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int64_t mine = b0 + lane < a.B ? (int64_t)row_units(seq_tiles(seq_len(a, b0 + lane))) * heads : 0;
+      int64_t upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += u;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, pos < upto);
+      if (past != 0) {
+        const int src = __ffs(past) - 1;
+        b = b0 + src;
+        off = (int)(pos - __shfl_sync(0xffffffffu, upto - mine, src));
+        break;
+      }
+      pos -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    const unsigned past = __ballot_sync(0xffffffffu, pos < prefix + upto);
-    if (past != 0) {
-      const int src = __ffs(past) - 1;
-      b = b0 + src;
-      prefix += __shfl_sync(0xffffffffu, upto - mine, src);
-      break;
-    }
-    prefix += __shfl_sync(0xffffffffu, upto, 31);
   }
 
   uint8_t* ring = smem + warp * L::WARP_RING;
-  const uint32_t ring_u32 = smem_u32(ring);
-  float* scale_ring = reinterpret_cast<float*>(smem + L::RING) + warp * L::STAGES * 2;
-  const uint32_t scale_u32 = smem_u32(scale_ring);
-  const uint8_t* const no_bytes = a.k;  // a readable address for zero-filled pieces
-  const int page_mask = (1 << a.page_shift) - 1, page_bytes = D << a.page_shift;
-  // What this lane copies: 16 bytes at 16 * lane of every 512. Where they go: K with its 32-byte units swizzled by the
-  // token's parity (D = 128; at 64 two tokens share a 128-byte line and need none), V by the token's pair.
-  const uint8_t* const k_lane = a.k + lane * 16;
-  const uint8_t* const v_lane = a.v + lane * 16;
-  const uint32_t k_to = D == 128 ? (lane * 16) ^ (((lane >> 3) & 1) << 6) : lane * 16;
-  const uint32_t v_to = D == 128 ? (lane * 16) ^ ((lane >> 4) << 5) : (lane * 16) ^ (((lane >> 3) & 3) << 5);
-  const int copy_row = D == 128 ? lane >> 3 : lane >> 2;  // token within a copy instruction
-  // Where this lane's fragments are: K chunk c at ^ 64 c, V's odd tokens at + 128 (D = 128) or ^ 64 (D = 64)
-  const int k_from = D == 128 ? g * 128 + (((t >> 1) ^ ((g & 1) << 1)) << 5) + (t & 1) * 16 : g * 64 + t * 16;
-  const int v_from = D == 128 ? t * 256 + (((g >> 1) ^ t) << 5) + (g & 1) * 16 : t * 128 + (((g >> 2) ^ t) << 5) + (g & 3) * 8;
-  const float* const scale_lane = lane == 0 ? a.ks : a.vs;
+  const int page_mask = (1 << a.page_shift) - 1;
+  // Where this lane's fragments are in a tile: K chunk c at ^ 64 c, V's second token of the pair at v_odd; + 8 rows: + 8 D
+  const int tk = token_of<D>(g), tv0 = token_of<D>(2 * t), tv1 = token_of<D>(2 * t + 1);
+  const int k_from = D == 128 ? tk * 128 + ((t ^ tk) << 4) : tk * 64 + ((t ^ ((tk >> 1) & 3)) << 4);
+  const int v_even = D == 128 ? tv0 * 128 + ((g ^ tv0) << 4) : tv0 * 64 + (((g >> 1) ^ ((tv0 >> 1) & 3)) << 4) + (g & 1) * 8;
+  const int v_odd = D == 128 ? tv1 * 128 + ((g ^ tv1) << 4) : tv1 * 64 + (((g >> 1) ^ ((tv1 >> 1) & 3)) << 4) + (g & 1) * 8;
+  int slot = 0, use = 0;    // ring slots that are filled and used next: equal between two rows
+  uint32_t phase = 0;       // of the slot that is used next
+  bool alive = true;        // no wait has run out
 
-  while (pos < end) {
+  while (left > 0 && alive) {
     // ---- the next row and the part of it that is ours ----
     int len = seq_len(a, b);
     int tiles = seq_tiles(len);
-    int64_t units = row_units(tiles);
-    while (pos >= prefix + units * heads) {
-      prefix += units * heads;
+    int units = row_units(tiles);
+    while (off >= units * heads) {
+      off -= units * heads;
       ++b;
       len = seq_len(a, b);
       tiles = seq_tiles(len);
       units = row_units(tiles);
     }
-    const int hr = (int)((pos - prefix) / units);
-    const int64_t tile0 = prefix + hr * units + ROW_COST;  // the unit of the row's first tile
-    const int ta = (int)max(pos - tile0, (int64_t)0);
-    const int tb = (int)min(end - tile0, (int64_t)tiles);
-    pos = min(end, tile0 + tiles);
+    const int hr = off / units, within = off - hr * units;  // the row's tiles begin ROW_COST units into it
+    const int ta = max(within - ROW_COST, 0), tb = min(within + left - ROW_COST, tiles);
+    const int step = min(left, units - within);
+    off += step;
+    left -= step;
     if (tb <= ta) continue;  // only what a row counts beside its tiles
     const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
     const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
@@ -253,37 +259,26 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
       return i < nsub ? kv8_page_id(table, ((int64_t)(ta + i) * SK_TILE) >> a.page_shift, a.num_pages, a.status) * a.Hkv + hkv : 0;
     };
     int unit_now = unit_of(lane), unit_next = unit_of(32 + lane);
-    int slot = 0;  // ring slot that is filled next
+    // and the scales of those 32 tiles, for the tiles that are issued and those that are used
+    float ks_issue = __ldg(a.ks + unit_now), vs_issue = __ldg(a.vs + unit_now), ks_use = 0.f, vs_use = 0.f;
     auto issue = [&](int i) {
       if (i < nsub) {
         if ((i & 31) == 0 && i > 0) {
           unit_now = unit_next;
           unit_next = unit_of(i + 32 + lane);
+          ks_issue = __ldg(a.ks + unit_now);
+          vs_issue = __ldg(a.vs + unit_now);
         }
         const int unit = __shfl_sync(0xffffffffu, unit_now, i & 31);
-        const int first = (ta + i) * SK_TILE;
-        const int64_t at = (int64_t)unit * page_bytes + (first & page_mask) * D;
-        const uint32_t sk = ring_u32 + slot * L::STAGE + k_to, sv = ring_u32 + slot * L::STAGE + L::HALF;
-        const uint8_t* kp = k_lane + at;
-        const uint8_t* vp = v_lane + at;
-        const int left = len - first;
-        if (left >= SK_TILE) {
-#pragma unroll
-          for (int u = 0; u < L::COPIES; ++u) cp_async16(sk + u * 512, kp + u * 512);
-#pragma unroll
-          for (int u = 0; u < L::COPIES; ++u) cp_async16(sv + u * 512 + (D == 128 ? v_to ^ ((u & 1) << 6) : v_to), vp + u * 512);
-        } else {  // the sequence's last tile: tokens behind its end are zeros, whatever the page holds
-#pragma unroll
-          for (int u = 0; u < L::COPIES; ++u) {
-            const bool in = u * (SK_TILE / L::COPIES) + copy_row < left;
-            cp_async16(sk + u * 512, in ? kp + u * 512 : no_bytes, in ? 16 : 0);
-            cp_async16(sv + u * 512 + (D == 128 ? v_to ^ ((u & 1) << 6) : v_to), in ? vp + u * 512 : no_bytes, in ? 16 : 0);
-          }
+        if (lane == 0) {
+          const int row = (unit << a.page_shift) + (((ta + i) * SK_TILE) & page_mask);
+          uint64_t* bar = &s_full[warp][slot];
+          mbar_arrive_expect_tx(bar, L::STAGE);
+          tma_load_2d(ring + slot * L::STAGE, &tma_k, bar, 0, row);
+          tma_load_2d(ring + slot * L::STAGE + L::HALF, &tma_v, bar, 0, row);
         }
-        if (lane < 2) cp_async4(scale_u32 + (slot * 2 + lane) * 4, scale_lane + unit);
         slot = slot + 1 == L::STAGES ? 0 : slot + 1;
       }
-      cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < L::STAGES - 1; ++i) issue(i);
@@ -354,16 +349,22 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
       }
     }
 
-    int use = 0;  // ring slot that is used next
     for (int i = 0; i < nsub; ++i) {
       __syncwarp();  // all lanes have read the slot that is filled next
       issue(i + L::STAGES - 1);
-      cp_async_wait<L::STAGES - 1>();
-      __syncwarp();
+      if ((i & 31) == 0) {  // (fewer stages than 32: the tiles that are issued are of the same 32)
+        ks_use = ks_issue;
+        vs_use = vs_issue;
+      }
+      const float ks = __shfl_sync(0xffffffffu, ks_use, i & 31), vs_raw = __shfl_sync(0xffffffffu, vs_use, i & 31);
+      if (!mbar_wait_warp(&s_full[warp][use], phase, wc, EMK_DEV_TIMEOUT_SOFTMAX)) {
+        alive = false;
+        break;
+      }
       const uint8_t* st = ring + use * L::STAGE;
       const uint8_t* sv = st + L::HALF;
-      const float2 scales = *reinterpret_cast<const float2*>(scale_ring + use * 2);
       use = use + 1 == L::STAGES ? 0 : use + 1;
+      phase ^= use == 0 ? 1u : 0u;
 
       // ---- logits: 16 tokens x 8 RT rows, two partial sums each ----
       float s[RT][4];
@@ -376,8 +377,8 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
         }
 #pragma unroll
         for (int c = 0; c < L::K_CHUNKS; ++c) {
-          const uint4 ka = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)));            // token g
-          const uint4 kb = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)) + 8 * D);  // token 8 + g
+          const uint4 ka = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)));            // token p(g)
+          const uint4 kb = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)) + 8 * D);  // token 8 + p(g)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t a0, a1, a2, a3;
@@ -393,10 +394,9 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
           for (int x = 0; x < 4; ++x) s[n][x] = s2[n][0][x] + s2[n][1][x];
         }
       }
-      const float ks = scales.x;
-      const float vs = max_nan(scales.y, V_SCALE_MIN);
+      const float vs = max_nan(vs_raw, V_SCALE_MIN);
       const float lvs = lg2(vs);
-      const int tok = (ta + i) * SK_TILE + g;
+      const int tok = (ta + i) * SK_TILE + tk;
       const bool edge = (ta + i) * SK_TILE + SK_TILE > limit_min;  // some row does not see all of the tile
       // p[n][2 u + e]: row n * 8 + 2 t + e, token tok + 8 u. A row that has seen nothing yet has an infinite shift: its
       // first visible logit makes the maximum move.
@@ -467,21 +467,30 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
 #pragma unroll
         for (int u = 0; u < 2; ++u) pb[n][u] = transpose8x8(pack_f16x2(p[n][2 * u], p[n][2 * u + 1]));
       }
-      if (scales.y == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
+      if (vs_raw == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
       // ---- o^T += V^T P^T ----
       uint32_t w[4][L::V_BYTES / 4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
+        const uint8_t* from = sv + ((u & 1) == 0 ? v_even : v_odd) + (u >> 1) * 8 * D;
         if constexpr (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4*>(sv + v_from + (u & 1) * 128 + (u >> 1) * 1024);
+          const uint4 v = *reinterpret_cast<const uint4*>(from);
           w[u][0] = v.x;
           w[u][1] = v.y;
           w[u][2] = v.z;
           w[u][3] = v.w;
         } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(sv + (v_from ^ ((u & 1) * 64)) + (u >> 1) * 512);
+          const uint2 v = *reinterpret_cast<const uint2*>(from);
           w[u][0] = v.x;
           w[u][1] = v.y;
+        }
+      }
+      if ((ta + i) * SK_TILE + SK_TILE > len) {  // the sequence's last tile: what lies behind its end counts as zeros
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len;
+#pragma unroll
+          for (int j = 0; j < L::V_BYTES / 4; ++j) w[u][j] = in ? w[u][j] : 0u;
         }
       }
 #pragma unroll
@@ -497,10 +506,10 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
       }
     }
 
+    if (!alive) break;
     // ---- this range's part of the row: channels [CH g, CH (g + 1)) of rows 2 t and 2 t + 1 of each tile per lane ----
-    cp_async_wait<0>();
     const bool whole = ta == 0 && tb == tiles;
-    const bool last = !whole && pos >= end;  // may go on in the next warp's range: left in shared memory
+    const bool last = !whole && left == 0;  // may go on in the next warp's range: left in shared memory
     if (last) __syncwarp();                   // every lane is done with the ring
 #pragma unroll
     for (int n = 0; n < RT; ++n) {
@@ -541,7 +550,8 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
       if (last) {
         s_row[warp] = row;
         s_edge[warp] = (ta == 0 ? 1 : 0) | (tb == tiles ? 2 : 0);
-        s_owner[warp] = (int)range_owner(tile0 + tiles - 1, total, ranges);
+        // (a row that begins here and is not whole goes on behind this range's end: its last tile is tiles - tb further)
+        if (ta == 0) s_owner[warp] = (int)range_owner(range_start(range + 1, total, ranges) - 1 + tiles - tb, total, ranges);
       }
     }
     __syncwarp();
@@ -549,6 +559,10 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
 
   // ---- the last pieces of the CTA's warps: neighbours that belong to one row become one piece ----
   __syncthreads();
+  if (s_abort) {  // a wait ran out (recorded): copies may be in flight, and pieces are missing
+    abort_drain();
+    return;
+  }
   for (int w0 = 0; w0 < SK_WARPS; ++w0) {
     const int row_id = s_row[w0];
     if (row_id < 0 || (w0 > 0 && s_row[w0 - 1] == row_id)) continue;
@@ -633,7 +647,8 @@ __global__ void __launch_bounds__(WARPS * 32) sdpa_kv8_join_kernel(const SdpaArg
     if (threadIdx.x < D / 8) reinterpret_cast<uint4*>(out)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     return;
   }
-  if (span.x == span.y) return;
+  // (the bounds hold unless the first kernel gave up on a wait and left places unwritten)
+  if (span.x == span.y || span.x < 0 || span.y < span.x || span.y >= a.max_ranges) return;
   float m = -INFINITY, l = 0.f, o[E];  // m is the same in all threads, l and o are this warp's part
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
@@ -738,6 +753,7 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
   p.ctas = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
   if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
+  if (p.ctas < 1) p.ctas = 1;
   p.info_bytes = align16(rows * (int64_t)sizeof(int2));
   p.ml_bytes = align16(p.ctas * SK_WARPS * 2 * p.row_cap * (int64_t)sizeof(float2));
   p.part_bytes = p.ctas * SK_WARPS * 2 * p.row_cap * D * (int64_t)sizeof(float);
@@ -746,6 +762,13 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
 
 template <int D, int RT>
 int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t s) {
+  CUtensorMap tk, tv;
+  const uint64_t rows = (uint64_t)a.num_pages * a.Hkv << a.page_shift;
+  constexpr CUtensorMapSwizzle SWIZZLE = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  int rc = emk_make_tmap_2d(h, &tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k, D, rows, D, D, SK_TILE, SWIZZLE);
+  if (rc != EMK_OK) return rc;
+  rc = emk_make_tmap_2d(h, &tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.v, D, rows, D, D, SK_TILE, SWIZZLE);
+  if (rc != EMK_OK) return rc;
   static emk_device_once once;
   {
     std::lock_guard<std::mutex> lk(once.mu);
@@ -755,7 +778,7 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     }
   }
   EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_kernel<D, RT>, (unsigned)p.ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
-                                        h->overlap_launch != 0, a));
+                                        h->overlap_launch != 0, tk, tv, a));
   EMK_LAUNCH_CHECK(h);
   // Few rows: a row may be cut into hundreds of pieces, and sixteen warps share them; many rows: a few pieces each.
   const int64_t blocks = (int64_t)a.B * a.Hkv * a.row_tiles * a.row_cap;
@@ -802,8 +825,8 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   if (B <= 0 || Sq <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_pages <= 0 || num_pages <= 0 ||
       num_pages > 0x7fffffff || max_pages > 0x7fffffff / page || ld_q / D < Hq)
     return EMK_ERR_SHAPE;
-  if (num_pages > 0x7fffffff / Hkv || !sizes_ok(B, Sq, Hq, Hkv)) {
-    EMK_SET_ERR(h, "emk_sdpa_kv8: more than 2^31 - 1 (page, head) pairs or tiles of query rows");
+  if (num_pages > 0x7fffffff / page / Hkv || !sizes_ok(B, Sq, Hq, Hkv)) {
+    EMK_SET_ERR(h, "emk_sdpa_kv8: more than 2^31 - 1 rows in the cache or tiles of query rows");
     return EMK_ERR_LIMIT;
   }
   if (((uintptr_t)q & 15u) != 0 || (ld_q & 7) != 0 || (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)o) & 15u) != 0 ||
@@ -811,6 +834,12 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
       ((uintptr_t)workspace & 15u) != 0)
     return EMK_ERR_ALIGN;
   const SkPlan p = plan_of(h->sm_count, B, Sq, Hq, Hkv, max_pages * page, D);
+  const int64_t units = max_pages * page / SK_TILE + 1 + ROW_COST;
+  if (Hkv * p.row_tiles > 0x7fffffff / units || B * Hkv * p.row_tiles * units / (p.ctas * SK_WARPS) > 0x7ffffffe) {
+    EMK_SET_ERR(h, "emk_sdpa_kv8: %lld tokens a sequence are too many for the number of sequences and heads",
+                (long long)(max_pages * page));
+    return EMK_ERR_LIMIT;
+  }
   if (workspace_bytes < p.info_bytes + p.ml_bytes + p.part_bytes) {
     EMK_SET_ERR(h, "emk_sdpa_kv8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                 (long long)(p.info_bytes + p.ml_bytes + p.part_bytes));
@@ -842,7 +871,9 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   a.info = (int2*)ws;
   a.ml = (float2*)(ws + p.info_bytes);
   a.part = (float*)(ws + p.info_bytes + p.ml_bytes);
+  a.max_ranges = (int)(p.ctas * SK_WARPS);
   a.status = h->status_dev;
+  a.limit_ns = h->wait_limit_ns;
   cudaStream_t s = (cudaStream_t)stream;
   if (D == 128) return p.tile_rows == 8 ? launch_sdpa<128, 1>(h, a, p, s) : launch_sdpa<128, 2>(h, a, p, s);
   return p.tile_rows == 8 ? launch_sdpa<64, 1>(h, a, p, s) : launch_sdpa<64, 2>(h, a, p, s);

@@ -73,7 +73,7 @@ def test_workspace_of_bad_sizes_is_zero(lib, fake_handle):
     for sizes in ((0, 1, 8, 2, 64, 128), (1, 1, 7, 2, 64, 128), (1, 1, 8, 0, 64, 128), (1, 1, 8, 2, 0, 128), (1, 1, 8, 2, 64, 96),
                   (1 << 62, 1, 8, 2, 64, 128), (1, 1 << 62, 8, 2, 64, 128)):
         assert f(fake_handle, *sizes) == 0
-    assert f(fake_handle, 2, 1, 8, 2, 64, 128) >= 2 * 2 * 8  # no SMs in the fake: the table of rows is left
+    assert f(fake_handle, 2, 1, 8, 2, 64, 128) >= 2 * 2 * 8
 
 
 def _norm(lib, h, **kw):
