@@ -183,7 +183,6 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
   }
   __syncthreads();
   grid_dependency_wait();
-  grid_launch_dependents();
   const WaitCtx wc{&s_abort, a.status, a.limit_ns};
 
   // ---- this warp's range of the list ----
@@ -557,6 +556,9 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
     __syncwarp();
   }
 
+  // Not earlier: blocks of the next kernel that wait beside this one's long-lived warps cost 19 us of 121 (64 sequences of up
+  // to 8192 tokens); and not at all in the join, whose dependents are such a kernel.
+  grid_launch_dependents();
   // ---- the last pieces of the CTA's warps: neighbours that belong to one row become one piece ----
   __syncthreads();
   if (s_abort) {  // a wait ran out (recorded): copies may be in flight, and pieces are missing
@@ -632,7 +634,6 @@ __global__ void __launch_bounds__(WARPS * 32) sdpa_kv8_join_kernel(const SdpaArg
   __shared__ float s_m[WARPS], s_l[WARPS];
   __shared__ float s_o[WARPS][D];
   grid_dependency_wait();
-  grid_launch_dependents();
   const int heads = a.Hkv * a.row_tiles;
   const int b = blockIdx.x / heads, hr = blockIdx.x - b * heads;
   const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
