@@ -24,6 +24,8 @@
 // log2(v_scale) and p * v_scale / max is what is rounded to f16 (2^-12 relative: p in [0, 2^15], so 2^-29 of the largest
 // contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
 //
+// Two kernels share the loop. Where no sequence can be long (split_of), a cluster of CTAs takes a row tile, deals its tiles
+// to its warps and joins their pieces in distributed shared memory: one launch. Otherwise:
 // Work split: the tiles of 16 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
 // warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths. Beginning a row costs a
 // warp about as much as a tile (the queries, a pipeline to fill, an output), so a row counts ROW_COST tiles more than it
@@ -155,12 +157,295 @@ struct SkLayout {
   static_assert(ROWS * PIECE_PITCH * 4 <= WARP_RING, "a warp's last piece lies over its ring");
 };
 
+// Ring position of a warp: slots that are filled and used next (equal between two parts), phase of the latter's barrier.
+struct RingAt {
+  int slot, use;
+  uint32_t phase;
+};
+
+// What a warp has of a row tile: o[n][j][2 x + e] is row n * 8 + 2 t + e, channel D / 8 * g + 2 j + x; m the running maximum of
+// logit + log2 v_scale, l this lane's part of the sum of 2^(logit - m), both of the rows n * 8 + 2 t + e.
+template <int D, int RT>
+struct Part {
+  float o[RT][D / 16][4];
+  float m[RT][2], l[RT][2];
+};
+
+// Tiles [ta, tb) of the row tile rt of KV head hkv of sequence b, by one warp. False: a wait ran out (recorded).
+template <int D, int RT>
+__device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& tma_k, const CUtensorMap& tma_v, uint8_t* ring,
+                                         uint64_t* full, const WaitCtx& wc, RingAt& at, int b, int hkv, int rt, int len, int ta,
+                                         int tb, Part<D, RT>& part) {
+  using L = SkLayout<D, RT>;
+  constexpr int STEPS = D / 16;  // k16 steps of K q^T, and m16 tiles of V^T P^T
+  constexpr int ROWS = L::ROWS;
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int page_mask = (1 << a.page_shift) - 1;
+  // Where this lane's fragments are in a tile: K chunk c at ^ 64 c, V's second token of the pair at v_odd; + 8 rows: + 8 D
+  const int tk = token_of<D>(g), tv0 = token_of<D>(2 * t), tv1 = token_of<D>(2 * t + 1);
+  const int k_from = D == 128 ? tk * 128 + ((t ^ tk) << 4) : tk * 64 + ((t ^ ((tk >> 1) & 3)) << 4);
+  const int v_even = D == 128 ? tv0 * 128 + ((g ^ tv0) << 4) : tv0 * 64 + (((g >> 1) ^ ((tv0 >> 1) & 3)) << 4) + (g & 1) * 8;
+  const int v_odd = D == 128 ? tv1 * 128 + ((g ^ tv1) << 4) : tv1 * 64 + (((g >> 1) ^ ((tv1 >> 1) & 3)) << 4) + (g & 1) * 8;
+  const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
+  const int32_t* table = a.table + (int64_t)b * a.max_pages;
+  const int nsub = tb - ta;
+
+  // lane j holds the (page, head) of tile i0 + j of this part, for the 32 tiles that are issued now and the next 32
+  auto unit_of = [&](int i) {
+    return i < nsub ? kv8_page_id(table, ((int64_t)(ta + i) * SK_TILE) >> a.page_shift, a.num_pages, a.status) * a.Hkv + hkv : 0;
+  };
+  int unit_now = unit_of(lane), unit_next = unit_of(32 + lane);
+  // and the scales of those 32 tiles, for the tiles that are issued and those that are used
+  float ks_issue = __ldg(a.ks + unit_now), vs_issue = __ldg(a.vs + unit_now), ks_use = 0.f, vs_use = 0.f;
+  auto issue = [&](int i) {
+    if (i < nsub) {
+      if ((i & 31) == 0 && i > 0) {
+        unit_now = unit_next;
+        unit_next = unit_of(i + 32 + lane);
+        ks_issue = __ldg(a.ks + unit_now);
+        vs_issue = __ldg(a.vs + unit_now);
+      }
+      const int unit = __shfl_sync(0xffffffffu, unit_now, i & 31);
+      if (lane == 0) {
+        const int row = (unit << a.page_shift) + (((ta + i) * SK_TILE) & page_mask);
+        uint64_t* bar = &full[at.slot];
+        mbar_arrive_expect_tx(bar, L::STAGE);
+        tma_load_2d(ring + at.slot * L::STAGE, &tma_k, bar, 0, row);
+        tma_load_2d(ring + at.slot * L::STAGE + L::HALF, &tma_v, bar, 0, row);
+      }
+      at.slot = at.slot + 1 == L::STAGES ? 0 : at.slot + 1;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < L::STAGES - 1; ++i) issue(i);
+
+  // ---- q: row g of each 8-row tile, channels as the K fragment has them ----
+  uint32_t qf[RT][STEPS][2];
+  // of the rows whose logits this lane gets, 2 t and 2 t + 1 of each tile: factor of the logits, tokens that the row sees
+  float qs[RT][2];
+  int limit[RT][2];
+  int limit_min = len;
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    const int row = n * 8 + g;
+    const int rr = rt * ROWS + row;
+    const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
+    const bool valid = row < rows;
+    const __nv_bfloat16* qp = a.q + ((int64_t)b * a.Sq + (valid ? qi : 0)) * a.ld_q + (int64_t)(valid ? head : 0) * D + t * 16;
+    uint32_t raw[D / 8];
+    float amax = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint4 v = valid ? *reinterpret_cast<const uint4*>(qp + c * 64 + p * 8) : make_uint4(0, 0, 0, 0);
+        raw[c * 8 + p * 4] = v.x;
+        raw[c * 8 + p * 4 + 1] = v.y;
+        raw[c * 8 + p * 4 + 2] = v.z;
+        raw[c * 8 + p * 4 + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) amax = max_nan(amax, max_nan(fabsf(bf16_lo(raw[i])), fabsf(bf16_hi(raw[i]))));
+    amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // 2^(14 - exponent of the largest), within the normal floats
+    const int e = min(max(127 + 14 - ((int)(__float_as_uint(amax) >> 23) - 127), 1), 253);
+    const float up = __uint_as_float((uint32_t)e << 23);
+    const float factor = amax <= 3.402823466e38f ? a.scale_log2 / up : __uint_as_float(0x7fc00000u);  // a row with no finite scores
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {  // step j: channels 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1}, {2, 3}
+      const uint32_t lo = raw[(j >> 2) * 8 + (j & 3) * 2], hi = raw[(j >> 2) * 8 + (j & 3) * 2 + 1];
+      qf[n][j][0] = pack_f16x2(bf16_lo(lo) * up, bf16_hi(lo) * up);
+      qf[n][j][1] = pack_f16x2(bf16_lo(hi) * up, bf16_hi(hi) * up);
+    }
+    const int sees = valid ? max(len - a.Sq + qi + 1, 0) : len;  // rows past the last are computed and dropped
+    limit_min = min(limit_min, __reduce_min_sync(0xffffffffu, sees));
+#pragma unroll
+    for (int e2 = 0; e2 < 2; ++e2) {
+      qs[n][e2] = __shfl_sync(0xffffffffu, factor, (2 * t + e2) * 4);
+      limit[n][e2] = __shfl_sync(0xffffffffu, sees, (2 * t + e2) * 4);
+    }
+  }
+
+  // what is added to a logit: P_SHIFT - the running maximum
+  float shift[RT][2];
+  bool big = false;
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) part.o[n][j][0] = part.o[n][j][1] = part.o[n][j][2] = part.o[n][j][3] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      part.m[n][e] = -INFINITY;
+      shift[n][e] = INFINITY;
+      part.l[n][e] = 0.f;
+    }
+  }
+
+  for (int i = 0; i < nsub; ++i) {
+    __syncwarp();  // all lanes have read the slot that is filled next
+    issue(i + L::STAGES - 1);
+    if ((i & 31) == 0) {  // (fewer stages than 32: the tiles that are issued are of the same 32)
+      ks_use = ks_issue;
+      vs_use = vs_issue;
+    }
+    const float ks = __shfl_sync(0xffffffffu, ks_use, i & 31), vs_raw = __shfl_sync(0xffffffffu, vs_use, i & 31);
+    if (!mbar_wait_warp(&full[at.use], at.phase, wc, EMK_DEV_TIMEOUT_SOFTMAX)) return false;
+    const uint8_t* st = ring + at.use * L::STAGE;
+    const uint8_t* sv = st + L::HALF;
+    at.use = at.use + 1 == L::STAGES ? 0 : at.use + 1;
+    at.phase ^= at.use == 0 ? 1u : 0u;
+
+    // ---- logits: 16 tokens x 8 RT rows, two partial sums each ----
+    float s[RT][4];
+    {
+      float s2[RT][2][4];
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s2[n][0][x] = s2[n][1][x] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < L::K_CHUNKS; ++c) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)));            // token p(g)
+        const uint4 kb = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)) + 8 * D);  // token 8 + p(g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_f16x4(j == 0 ? ka.x : j == 1 ? ka.y : j == 2 ? ka.z : ka.w, a0, a2);
+          e4m3x4_f16x4(j == 0 ? kb.x : j == 1 ? kb.y : j == 2 ? kb.z : kb.w, a1, a3);
+#pragma unroll
+          for (int n = 0; n < RT; ++n) mma_f16(s2[n][j & 1], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[n][x] = s2[n][0][x] + s2[n][1][x];
+      }
+    }
+    const float vs = max_nan(vs_raw, V_SCALE_MIN);
+    const float lvs = lg2(vs);
+    const int tok = (ta + i) * SK_TILE + tk;
+    const bool edge = (ta + i) * SK_TILE + SK_TILE > limit_min;  // some row does not see all of the tile
+    // p[n][2 u + e]: row n * 8 + 2 t + e, token tok + 8 u. A row that has seen nothing yet has an infinite shift: its
+    // first visible logit makes the maximum move.
+    float p[RT][4];
+    auto exponents = [&]() {
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p[n][x] = fmaf(s[n][x], qs[n][x & 1] * ks, lvs + shift[n][x & 1]);
+        if (edge) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (tok + (x >> 1) * 8 >= limit[n][x & 1]) p[n][x] = -INFINITY;
+        }
+      }
+    };
+    exponents();
+    float most = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < RT; ++n) most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])));
+    if (__any_sync(0xffffffffu, most > P_LIMIT)) {  // rare after a row's first tiles: no shuffles otherwise
+      big = false;
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (!edge || tok + u * 8 < limit[n][e]) mx = fmaxf(mx, fmaf(s[n][2 * u + e], qs[n][e] * ks, lvs));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float to = fmaxf(part.m[n][e], mx);
+          f[e] = part.m[n][e] == -INFINITY ? 0.f : ex2(part.m[n][e] - to);
+          part.m[n][e] = to;
+          shift[n][e] = P_SHIFT - to;
+          part.l[n][e] *= f[e];
+          big = big || (to != -INFINITY && fabsf(to) > BIG);
+        }
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+          part.o[n][j][0] *= f[0];
+          part.o[n][j][1] *= f[1];
+          part.o[n][j][2] *= f[0];
+          part.o[n][j][3] *= f[1];
+        }
+      }
+      big = __any_sync(0xffffffffu, big);
+      exponents();
+    }
+    if (big) {  // logits that differ by a rounding may differ by more than fp16 holds
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p[n][x] = p[n][x] > P_LIMIT ? P_LIMIT : p[n][x];
+      }
+    }
+    const float inv_vs = rcp(vs);
+    uint32_t pb[RT][2];  // P^T: row g, tokens 2 t, 2 t + 1 (+ 8)
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) p[n][x] = ex2(p[n][x]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) part.l[n][e] = fmaf(p[n][e] + p[n][2 + e], inv_vs, part.l[n][e]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) pb[n][u] = transpose8x8(pack_f16x2(p[n][2 * u], p[n][2 * u + 1]));
+    }
+    if (vs_raw == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
+    // ---- o^T += V^T P^T ----
+    uint32_t w[4][L::V_BYTES / 4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint8_t* from = sv + ((u & 1) == 0 ? v_even : v_odd) + (u >> 1) * 8 * D;
+      if constexpr (D == 128) {
+        const uint4 v = *reinterpret_cast<const uint4*>(from);
+        w[u][0] = v.x;
+        w[u][1] = v.y;
+        w[u][2] = v.z;
+        w[u][3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(from);
+        w[u][0] = v.x;
+        w[u][1] = v.y;
+      }
+    }
+    if ((ta + i) * SK_TILE + SK_TILE > len) {  // the sequence's last tile: what lies behind its end counts as zeros
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len;
+#pragma unroll
+        for (int j = 0; j < L::V_BYTES / 4; ++j) w[u][j] = in ? w[u][j] : 0u;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < L::V_BYTES / 4; ++j) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // channels 4 j + 2 half (rows g of the tile) and the next (rows 8 + g)
+        uint32_t a0, a1, a2, a3;
+        e4m3x4_f16x4(__byte_perm(w[0][j], w[1][j], half == 0 ? 0x5140 : 0x7362), a0, a1);
+        e4m3x4_f16x4(__byte_perm(w[2][j], w[3][j], half == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+        for (int n = 0; n < RT; ++n) mma_f16(part.o[n][j * 2 + half], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      }
+    }
+  }
+  return true;
+}
+
 template <int D, int RT>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa_kv8_kernel(const __grid_constant__ CUtensorMap tma_k,
                                                                                           const __grid_constant__ CUtensorMap tma_v,
                                                                                           const SdpaArgs a) {
   using L = SkLayout<D, RT>;
-  constexpr int STEPS = D / 16;  // k16 steps of K q^T, and m16 tiles of V^T P^T
+  constexpr int STEPS = D / 16;
   constexpr int CH = D / 8;      // channels of o per lane and row
   constexpr int ROWS = L::ROWS;
   extern __shared__ uint8_t smem_raw[];
@@ -220,14 +505,7 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
   }
 
   uint8_t* ring = smem + warp * L::WARP_RING;
-  const int page_mask = (1 << a.page_shift) - 1;
-  // Where this lane's fragments are in a tile: K chunk c at ^ 64 c, V's second token of the pair at v_odd; + 8 rows: + 8 D
-  const int tk = token_of<D>(g), tv0 = token_of<D>(2 * t), tv1 = token_of<D>(2 * t + 1);
-  const int k_from = D == 128 ? tk * 128 + ((t ^ tk) << 4) : tk * 64 + ((t ^ ((tk >> 1) & 3)) << 4);
-  const int v_even = D == 128 ? tv0 * 128 + ((g ^ tv0) << 4) : tv0 * 64 + (((g >> 1) ^ ((tv0 >> 1) & 3)) << 4) + (g & 1) * 8;
-  const int v_odd = D == 128 ? tv1 * 128 + ((g ^ tv1) << 4) : tv1 * 64 + (((g >> 1) ^ ((tv1 >> 1) & 3)) << 4) + (g & 1) * 8;
-  int slot = 0, use = 0;    // ring slots that are filled and used next: equal between two rows
-  uint32_t phase = 0;       // of the slot that is used next
+  RingAt at{0, 0, 0};
   bool alive = true;        // no wait has run out
 
   while (left > 0 && alive) {
@@ -250,261 +528,8 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
     if (tb <= ta) continue;  // only what a row counts beside its tiles
     const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
     const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
-    const int32_t* table = a.table + (int64_t)b * a.max_pages;
-    const int nsub = tb - ta;
-
-    // lane j holds the (page, head) of tile i0 + j of this part, for the 32 tiles that are issued now and the next 32
-    auto unit_of = [&](int i) {
-      return i < nsub ? kv8_page_id(table, ((int64_t)(ta + i) * SK_TILE) >> a.page_shift, a.num_pages, a.status) * a.Hkv + hkv : 0;
-    };
-    int unit_now = unit_of(lane), unit_next = unit_of(32 + lane);
-    // and the scales of those 32 tiles, for the tiles that are issued and those that are used
-    float ks_issue = __ldg(a.ks + unit_now), vs_issue = __ldg(a.vs + unit_now), ks_use = 0.f, vs_use = 0.f;
-    auto issue = [&](int i) {
-      if (i < nsub) {
-        if ((i & 31) == 0 && i > 0) {
-          unit_now = unit_next;
-          unit_next = unit_of(i + 32 + lane);
-          ks_issue = __ldg(a.ks + unit_now);
-          vs_issue = __ldg(a.vs + unit_now);
-        }
-        const int unit = __shfl_sync(0xffffffffu, unit_now, i & 31);
-        if (lane == 0) {
-          const int row = (unit << a.page_shift) + (((ta + i) * SK_TILE) & page_mask);
-          uint64_t* bar = &s_full[warp][slot];
-          mbar_arrive_expect_tx(bar, L::STAGE);
-          tma_load_2d(ring + slot * L::STAGE, &tma_k, bar, 0, row);
-          tma_load_2d(ring + slot * L::STAGE + L::HALF, &tma_v, bar, 0, row);
-        }
-        slot = slot + 1 == L::STAGES ? 0 : slot + 1;
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < L::STAGES - 1; ++i) issue(i);
-
-    // ---- q: row g of each 8-row tile, channels as the K fragment has them ----
-    uint32_t qf[RT][STEPS][2];
-    // of the rows whose logits this lane gets, 2 t and 2 t + 1 of each tile: factor of the logits, tokens that the row sees
-    float qs[RT][2];
-    int limit[RT][2];
-    int limit_min = len;
-#pragma unroll
-    for (int n = 0; n < RT; ++n) {
-      const int row = n * 8 + g;
-      const int rr = rt * ROWS + row;
-      const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
-      const bool valid = row < rows;
-      const __nv_bfloat16* qp = a.q + ((int64_t)b * a.Sq + (valid ? qi : 0)) * a.ld_q + (int64_t)(valid ? head : 0) * D + t * 16;
-      uint32_t raw[D / 8];
-      float amax = 0.f;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const uint4 v = valid ? *reinterpret_cast<const uint4*>(qp + c * 64 + p * 8) : make_uint4(0, 0, 0, 0);
-          raw[c * 8 + p * 4] = v.x;
-          raw[c * 8 + p * 4 + 1] = v.y;
-          raw[c * 8 + p * 4 + 2] = v.z;
-          raw[c * 8 + p * 4 + 3] = v.w;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) amax = max_nan(amax, max_nan(fabsf(bf16_lo(raw[i])), fabsf(bf16_hi(raw[i]))));
-      amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // 2^(14 - exponent of the largest), within the normal floats
-      const int e = min(max(127 + 14 - ((int)(__float_as_uint(amax) >> 23) - 127), 1), 253);
-      const float up = __uint_as_float((uint32_t)e << 23);
-      const float factor = amax <= 3.402823466e38f ? a.scale_log2 / up : __uint_as_float(0x7fc00000u);  // a row with no finite scores
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) {  // step j: channels 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1}, {2, 3}
-        const uint32_t lo = raw[(j >> 2) * 8 + (j & 3) * 2], hi = raw[(j >> 2) * 8 + (j & 3) * 2 + 1];
-        qf[n][j][0] = pack_f16x2(bf16_lo(lo) * up, bf16_hi(lo) * up);
-        qf[n][j][1] = pack_f16x2(bf16_lo(hi) * up, bf16_hi(hi) * up);
-      }
-      const int sees = valid ? max(len - a.Sq + qi + 1, 0) : len;  // rows past the last are computed and dropped
-      limit_min = min(limit_min, __reduce_min_sync(0xffffffffu, sees));
-#pragma unroll
-      for (int e2 = 0; e2 < 2; ++e2) {
-        qs[n][e2] = __shfl_sync(0xffffffffu, factor, (2 * t + e2) * 4);
-        limit[n][e2] = __shfl_sync(0xffffffffu, sees, (2 * t + e2) * 4);
-      }
-    }
-
-    // o[n][j][2 x + e]: row n * 8 + 2 t + e, channel CH * g + 2 j + x
-    float o[RT][STEPS][4];
-    // running maximum of logit + log2 v_scale, what is added to a logit (P_SHIFT - maximum), sum
-    float m[RT][2], shift[RT][2], l[RT][2];
-    bool big = false;
-#pragma unroll
-    for (int n = 0; n < RT; ++n) {
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
-        shift[n][e] = INFINITY;
-        l[n][e] = 0.f;
-      }
-    }
-
-    for (int i = 0; i < nsub; ++i) {
-      __syncwarp();  // all lanes have read the slot that is filled next
-      issue(i + L::STAGES - 1);
-      if ((i & 31) == 0) {  // (fewer stages than 32: the tiles that are issued are of the same 32)
-        ks_use = ks_issue;
-        vs_use = vs_issue;
-      }
-      const float ks = __shfl_sync(0xffffffffu, ks_use, i & 31), vs_raw = __shfl_sync(0xffffffffu, vs_use, i & 31);
-      if (!mbar_wait_warp(&s_full[warp][use], phase, wc, EMK_DEV_TIMEOUT_SOFTMAX)) {
-        alive = false;
-        break;
-      }
-      const uint8_t* st = ring + use * L::STAGE;
-      const uint8_t* sv = st + L::HALF;
-      use = use + 1 == L::STAGES ? 0 : use + 1;
-      phase ^= use == 0 ? 1u : 0u;
-
-      // ---- logits: 16 tokens x 8 RT rows, two partial sums each ----
-      float s[RT][4];
-      {
-        float s2[RT][2][4];
-#pragma unroll
-        for (int n = 0; n < RT; ++n) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) s2[n][0][x] = s2[n][1][x] = 0.f;
-        }
-#pragma unroll
-        for (int c = 0; c < L::K_CHUNKS; ++c) {
-          const uint4 ka = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)));            // token p(g)
-          const uint4 kb = *reinterpret_cast<const uint4*>(st + (k_from ^ (c * 64)) + 8 * D);  // token 8 + p(g)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_f16x4(j == 0 ? ka.x : j == 1 ? ka.y : j == 2 ? ka.z : ka.w, a0, a2);
-            e4m3x4_f16x4(j == 0 ? kb.x : j == 1 ? kb.y : j == 2 ? kb.z : kb.w, a1, a3);
-#pragma unroll
-            for (int n = 0; n < RT; ++n) mma_f16(s2[n][j & 1], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < RT; ++n) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) s[n][x] = s2[n][0][x] + s2[n][1][x];
-        }
-      }
-      const float vs = max_nan(vs_raw, V_SCALE_MIN);
-      const float lvs = lg2(vs);
-      const int tok = (ta + i) * SK_TILE + tk;
-      const bool edge = (ta + i) * SK_TILE + SK_TILE > limit_min;  // some row does not see all of the tile
-      // p[n][2 u + e]: row n * 8 + 2 t + e, token tok + 8 u. A row that has seen nothing yet has an infinite shift: its
-      // first visible logit makes the maximum move.
-      float p[RT][4];
-      auto exponents = [&]() {
-#pragma unroll
-        for (int n = 0; n < RT; ++n) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) p[n][x] = fmaf(s[n][x], qs[n][x & 1] * ks, lvs + shift[n][x & 1]);
-          if (edge) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (tok + (x >> 1) * 8 >= limit[n][x & 1]) p[n][x] = -INFINITY;
-          }
-        }
-      };
-      exponents();
-      float most = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < RT; ++n) most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])));
-      if (__any_sync(0xffffffffu, most > P_LIMIT)) {  // rare after a row's first tiles: no shuffles otherwise
-        big = false;
-#pragma unroll
-        for (int n = 0; n < RT; ++n) {
-          float f[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (!edge || tok + u * 8 < limit[n][e]) mx = fmaxf(mx, fmaf(s[n][2 * u + e], qs[n][e] * ks, lvs));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float to = fmaxf(m[n][e], mx);
-            f[e] = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - to);
-            m[n][e] = to;
-            shift[n][e] = P_SHIFT - to;
-            l[n][e] *= f[e];
-            big = big || (to != -INFINITY && fabsf(to) > BIG);
-          }
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j) {
-            o[n][j][0] *= f[0];
-            o[n][j][1] *= f[1];
-            o[n][j][2] *= f[0];
-            o[n][j][3] *= f[1];
-          }
-        }
-        big = __any_sync(0xffffffffu, big);
-        exponents();
-      }
-      if (big) {  // logits that differ by a rounding may differ by more than fp16 holds
-#pragma unroll
-        for (int n = 0; n < RT; ++n) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) p[n][x] = p[n][x] > P_LIMIT ? P_LIMIT : p[n][x];
-        }
-      }
-      const float inv_vs = rcp(vs);
-      uint32_t pb[RT][2];  // P^T: row g, tokens 2 t, 2 t + 1 (+ 8)
-#pragma unroll
-      for (int n = 0; n < RT; ++n) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) p[n][x] = ex2(p[n][x]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) l[n][e] = fmaf(p[n][e] + p[n][2 + e], inv_vs, l[n][e]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) pb[n][u] = transpose8x8(pack_f16x2(p[n][2 * u], p[n][2 * u + 1]));
-      }
-      if (vs_raw == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
-      // ---- o^T += V^T P^T ----
-      uint32_t w[4][L::V_BYTES / 4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint8_t* from = sv + ((u & 1) == 0 ? v_even : v_odd) + (u >> 1) * 8 * D;
-        if constexpr (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4*>(from);
-          w[u][0] = v.x;
-          w[u][1] = v.y;
-          w[u][2] = v.z;
-          w[u][3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(from);
-          w[u][0] = v.x;
-          w[u][1] = v.y;
-        }
-      }
-      if ((ta + i) * SK_TILE + SK_TILE > len) {  // the sequence's last tile: what lies behind its end counts as zeros
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len;
-#pragma unroll
-          for (int j = 0; j < L::V_BYTES / 4; ++j) w[u][j] = in ? w[u][j] : 0u;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < L::V_BYTES / 4; ++j) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // channels 4 j + 2 half (rows g of the tile) and the next (rows 8 + g)
-          uint32_t a0, a1, a2, a3;
-          e4m3x4_f16x4(__byte_perm(w[0][j], w[1][j], half == 0 ? 0x5140 : 0x7362), a0, a1);
-          e4m3x4_f16x4(__byte_perm(w[2][j], w[3][j], half == 0 ? 0x5140 : 0x7362), a2, a3);
-#pragma unroll
-          for (int n = 0; n < RT; ++n) mma_f16(o[n][j * 2 + half], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-        }
-      }
-    }
-
+    Part<D, RT> part;
+    alive = row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part);
     if (!alive) break;
     // ---- this range's part of the row: channels [CH g, CH (g + 1)) of rows 2 t and 2 t + 1 of each tile per lane ----
     const bool whole = ta == 0 && tb == tiles;
@@ -514,7 +539,7 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
     for (int n = 0; n < RT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float sum = l[n][e];
+        float sum = part.l[n][e];
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
@@ -528,18 +553,18 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
 #pragma unroll
           for (int j = 0; j < STEPS; j += 4)
             *reinterpret_cast<uint4*>(out + 2 * j) =
-                make_uint4(pack_bf16x2(o[n][j][e] * inv, o[n][j][2 + e] * inv), pack_bf16x2(o[n][j + 1][e] * inv, o[n][j + 1][2 + e] * inv),
-                           pack_bf16x2(o[n][j + 2][e] * inv, o[n][j + 2][2 + e] * inv),
-                           pack_bf16x2(o[n][j + 3][e] * inv, o[n][j + 3][2 + e] * inv));
+                make_uint4(pack_bf16x2(part.o[n][j][e] * inv, part.o[n][j][2 + e] * inv), pack_bf16x2(part.o[n][j + 1][e] * inv, part.o[n][j + 1][2 + e] * inv),
+                           pack_bf16x2(part.o[n][j + 2][e] * inv, part.o[n][j + 2][2 + e] * inv),
+                           pack_bf16x2(part.o[n][j + 3][e] * inv, part.o[n][j + 3][2 + e] * inv));
         } else {
           // (the first part of a row ends its range and takes slot 1, any other begins it and takes slot 0)
-          const int64_t at = range * 2 * a.row_cap + row;
-          if (g == 0) (last ? s_m[warp][row] : a.ml[at].x) = m[n][e];
-          if (g == 0) (last ? s_l[warp][row] : a.ml[at].y) = sum;
-          float* out = (last ? reinterpret_cast<float*>(ring) + row * L::PIECE_PITCH : a.part + at * D) + g * CH;
+          const int64_t place = range * 2 * a.row_cap + row;
+          if (g == 0) (last ? s_m[warp][row] : a.ml[place].x) = part.m[n][e];
+          if (g == 0) (last ? s_l[warp][row] : a.ml[place].y) = sum;
+          float* out = (last ? reinterpret_cast<float*>(ring) + row * L::PIECE_PITCH : a.part + place * D) + g * CH;
 #pragma unroll
           for (int j = 0; j < STEPS; j += 2)
-            *reinterpret_cast<float4*>(out + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
+            *reinterpret_cast<float4*>(out + 2 * j) = make_float4(part.o[n][j][e], part.o[n][j][2 + e], part.o[n][j + 1][e], part.o[n][j + 1][2 + e]);
         }
       }
     }
@@ -621,6 +646,131 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
     }
     if (begins && threadIdx.x == 0) a.info[row_id] = make_int2((int)first, whole ? (int)first : s_owner[w0]);
   }
+}
+
+__device__ __forceinline__ uint32_t cluster_size_x() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+template <int E>
+__device__ __forceinline__ void ld_cluster_vec(uint32_t addr, float* v) {
+  if constexpr (E == 4)
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+}
+
+// Short sequences: a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose pieces meet in distributed
+// shared memory. No list to cut, no workspace, no second kernel: what is left of a call is one launch and one row's latency.
+template <int D, int RT>
+__global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM)
+sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
+  using L = SkLayout<D, RT>;
+  constexpr int ROWS = L::ROWS, E = D / 32;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t s_full[SK_WARPS][L::STAGES];
+  __shared__ int s_abort;
+  __shared__ float s_m[SK_WARPS][ROWS], s_l[SK_WARPS][ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = (int)cluster_size_x(), rank = (int)cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SK_WARPS * L::STAGES; ++i) mbar_init(&s_full[0][0] + i, 1);
+    s_abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tma_k);
+    tma_prefetch_desc(&tma_v);
+  }
+  __syncthreads();
+  const int heads = a.Hkv * a.row_tiles;
+  const int row_id = blockIdx.x / split;
+  const int b = row_id / heads, hr = row_id - b * heads;
+  const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
+  const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
+  const int pieces = split * SK_WARPS, piece = rank * SK_WARPS + warp;
+  grid_dependency_wait();
+  const WaitCtx wc{&s_abort, a.status, a.limit_ns};
+  const int len = seq_len(a, b), tiles = seq_tiles(len);
+  const int ta = (int)((int64_t)tiles * piece / pieces), tb = (int)((int64_t)tiles * (piece + 1) / pieces);
+  if (lane < ROWS) {
+    s_m[warp][lane] = -INFINITY;
+    s_l[warp][lane] = 0.f;
+  }
+  __syncwarp();
+  if (tb > ta) {
+    uint8_t* ring = smem + warp * L::WARP_RING;
+    RingAt at{0, 0, 0};
+    Part<D, RT> part;
+    if (row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part)) {
+      __syncwarp();  // every lane is done with the ring, which now takes the piece
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = part.l[n][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int row = n * 8 + 2 * t + e;
+          if (g == 0) {
+            s_m[warp][row] = part.m[n][e];
+            s_l[warp][row] = sum;
+          }
+          float* out = reinterpret_cast<float*>(ring) + row * L::PIECE_PITCH + g * (D / 8);
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 2)
+            *reinterpret_cast<float4*>(out + 2 * j) =
+                make_float4(part.o[n][j][e], part.o[n][j][2 + e], part.o[n][j + 1][e], part.o[n][j + 1][2 + e]);
+        }
+      }
+    }
+  }
+  grid_launch_dependents();
+  __syncthreads();
+  if (s_abort) abort_drain();
+  if (split > 1) cluster_sync_all();  // (reached by every thread of every CTA, whatever happened above)
+  // a warp joins a row: lane i looks after piece i, then the lanes share the channels
+  for (int row = piece; row < rows; row += pieces) {
+    float m = -INFINITY, l = 0.f;
+    if (lane < pieces) {
+      m = ld_cluster(mapa_u32(smem_u32(&s_m[lane & (SK_WARPS - 1)][row]), (uint32_t)(lane / SK_WARPS)));
+      l = ld_cluster(mapa_u32(smem_u32(&s_l[lane & (SK_WARPS - 1)][row]), (uint32_t)(lane / SK_WARPS)));
+    }
+    const unsigned holds = __ballot_sync(0xffffffffu, m != -INFINITY || l != 0.f);  // (a NaN sum counts)
+    const float top = warp_max(m);
+    const float f = m == -INFINITY ? 1.f : ex2(m - top);
+    const float sum = warp_sum(l * f);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < pieces; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if ((holds >> i) & 1u) {
+        const uint32_t from = smem_u32(smem) + (uint32_t)((i & (SK_WARPS - 1)) * L::WARP_RING + (row * L::PIECE_PITCH + lane * E) * 4);
+        float v[E];
+        ld_cluster_vec<E>(mapa_u32(from, (uint32_t)(i / SK_WARPS)), v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], fi, acc[e]);
+      }
+    }
+    const int rr = rt * ROWS + row;
+    const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // nothing visible: zeros
+    __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + lane * E;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  }
+  if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
 // Joins the pieces of every row that was cut: block (row of tiles, row of the tile). The places of a row's pieces are
@@ -741,8 +891,30 @@ bool sizes_ok(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv) {
 
 struct SkPlan {
   int row_tiles, tile_rows, row_cap;
+  int split;  // CTAs per row tile of the rows kernel; 0: the list kernel and its join
   int64_t ctas, info_bytes, ml_bytes, part_bytes;
 };
+
+// CTAs per row tile for the rows kernel, or 0 where the list kernel is to run. The host knows the longest a sequence can be
+// (max_tokens), not the lengths. The rows kernel has no list to cut and nothing to join, and wins wherever its CTAs finish
+// about together (8 heads, one sequence of 1500 tokens: 7.3 us against 9.8; 64 sequences of 128: 6.9 / 12.9; of 1024: 26.2 /
+// 35.3; of 4096: 87.2 / 98.5); a sequence much longer than the others it drags through a few warps. So: as many CTAs per row as
+// fill the machine, or twice that, such that the longest possible sequence takes a row's warps (about 1 us a tile and warp)
+// 32 us at most, or 0.4 of the time in which the machine reads half of all that the tables could hold, 64 us at most
+// (64 sequences of 0..8192 tokens: 109.9 us in pairs, 115.2 alone, 102.9 as a list; 128 of 0..4096: 100.1 / 108.7 / 108.6).
+int split_of(int64_t rows, int64_t max_tokens, int64_t D, int64_t slots) {
+  int fill = 1;
+  while (fill < 8 && rows * fill * 2 <= slots) fill *= 2;
+  const double all = (double)rows * (double)max_tokens * (double)D / 6.2e6;  // us: half of 2 D bytes a token and row
+  const double limit = all * 0.4 > 64. ? 64. : all * 0.4 > 32. ? all * 0.4 : 32.;
+  const int64_t tiles = (max_tokens + SK_TILE - 1) / SK_TILE;
+  for (int split = fill; split <= 8 && split <= 2 * fill; split *= 2) {
+    if ((double)tiles / (split * SK_WARPS) > limit) continue;
+    while (split > 1 && tiles < split * 8) split /= 2;  // no CTA with less than two tiles a warp
+    return rows * split <= 0x7fffffff ? split : 0;
+  }
+  return 0;
+}
 
 // The grid never has more warps than the longest possible list has units.
 SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t max_tokens, int64_t D) {
@@ -752,12 +924,15 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   p.row_cap = Hq / Hkv * Sq < p.tile_rows ? (int)(Hq / Hkv * Sq) : p.tile_rows;
   const int64_t units = (max_tokens + SK_TILE - 1) / SK_TILE + ROW_COST;  // below 2^28
   const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
-  p.ctas = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
+  const int64_t slots = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
+  p.split = split_of(rows, max_tokens, D, slots);
+  p.ctas = slots;
   if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
   if (p.ctas < 1) p.ctas = 1;
   p.info_bytes = align16(rows * (int64_t)sizeof(int2));
   p.ml_bytes = align16(p.ctas * SK_WARPS * 2 * p.row_cap * (int64_t)sizeof(float2));
   p.part_bytes = p.ctas * SK_WARPS * 2 * p.row_cap * D * (int64_t)sizeof(float);
+  if (p.split > 0) p.info_bytes = p.ml_bytes = p.part_bytes = 0;  // no workspace
   return p;
 }
 
@@ -775,8 +950,28 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     std::lock_guard<std::mutex> lk(once.mu);
     if (!once.done[h->device]) {
       EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_rows_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
       once.done[h->device] = true;
     }
+  }
+  if (p.split > 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_tiles * p.split), 1, 1);
+    cfg.blockDim = dim3(SK_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = SkLayout<D, RT>::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = h->overlap_launch != 0 ? 2 : 1;
+    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, sdpa_kv8_rows_kernel<D, RT>, tk, tv, a));
+    EMK_LAUNCH_CHECK(h);
+    return EMK_OK;
   }
   EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_kernel<D, RT>, (unsigned)p.ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
                                         h->overlap_launch != 0, tk, tv, a));
@@ -816,8 +1011,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
                             void* o, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
                             int64_t max_pages, int64_t num_pages, float scale, void* workspace, int64_t workspace_bytes,
                             emk_stream_t stream) {
-  if (!h || !q || !k_codes || !v_codes || !k_scale || !v_scale || !page_table || !seq_lens || !o || !workspace)
-    return EMK_ERR_ARG;
+  if (!h || !q || !k_codes || !v_codes || !k_scale || !v_scale || !page_table || !seq_lens || !o) return EMK_ERR_ARG;
   if ((D != 64 && D != 128) || !kv8_page_ok(page)) {
     EMK_SET_ERR(h, "emk_sdpa_kv8: head dimension 64 or 128 and a page of 16, 32, 64, 128 or 256 tokens; got D=%lld page=%lld",
                 (long long)D, (long long)page);
@@ -841,6 +1035,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
                 (long long)(max_pages * page));
     return EMK_ERR_LIMIT;
   }
+  if (workspace == nullptr && p.split == 0) return EMK_ERR_ARG;
   if (workspace_bytes < p.info_bytes + p.ml_bytes + p.part_bytes) {
     EMK_SET_ERR(h, "emk_sdpa_kv8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                 (long long)(p.info_bytes + p.ml_bytes + p.part_bytes));

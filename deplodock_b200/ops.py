@@ -733,12 +733,13 @@ def sdpa_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, seq_len
         raise ValueError("the heads of a query must be contiguous [Hq, D] and its tokens evenly spaced")
     ld = q.stride(1) if Sq > 1 else q.stride(0) if B > 1 else Hq * D
     need = _sdpa_kv8_workspace_bytes(idx, B, Sq, Hq, Hkv, max_pages * page, D)
-    if workspace is None:
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    if workspace is None and need > 0:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     _call_on(idx, "emk_sdpa_kv8", q.data_ptr(), ld, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
              cache.v_scale.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), o.data_ptr(), B, Sq, Hq, Hkv, D, page,
-             max_pages, pages, 1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(),
-             workspace.numel() * workspace.element_size())
+             max_pages, pages, 1.0 / math.sqrt(D) if scale is None else float(scale),
+             0 if workspace is None else workspace.data_ptr(),
+             0 if workspace is None else workspace.numel() * workspace.element_size())
     return o
 
 

@@ -372,12 +372,19 @@ def _attend_check(ops, got, q, cache, table, lens, scale):
                 assert not bad.any(), (b, h, i, m, float(((o - want).abs() / tol).max()))
 
 
-def _attend_case(ops, Sq, Hq, Hkv, D, page, lens, seed=0, q_scale=1.0, sigma_exp=(-2, 3), fused=False, check=True):
+#: tokens a page table has room for: as many as the longest sequence (a kernel of one launch where that is short), or so
+#: many that the sequences' lengths may lie far apart (the list of tiles and its join). The rest of the table is never read.
+ROOM = ["tight", 1 << 20]
+
+
+def _attend_case(ops, Sq, Hq, Hkv, D, page, lens, seed=0, q_scale=1.0, sigma_exp=(-2, 3), fused=False, check=True, room="tight"):
     g = _gen(seed + 31)
     B = len(lens)
     max_pages = max(1, -(-max(lens) // page))
     pages = B * max_pages + 2
     table = torch.randperm(pages, generator=g)[:B * max_pages].view(B, max_pages).int()
+    if room != "tight":
+        table = torch.cat([table, torch.full((B, room // page - max_pages), -1, dtype=torch.int32)], 1)
     cache = _random_cache(ops, pages, Hkv, page, D, seed, sigma_exp)
     # whatever is behind a sequence's last token must not matter: NaN codes there, NaN scales on pages nobody uses
     used = torch.zeros(pages, page, dtype=torch.bool)
@@ -407,47 +414,55 @@ def _attend_case(ops, Sq, Hq, Hkv, D, page, lens, seed=0, q_scale=1.0, sigma_exp
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("page", [16, 64, 256])
 @pytest.mark.parametrize("Hq,Hkv", [(1, 1), (4, 2), (16, 1), (10, 2)])
-def test_sdpa_kv8_single_token(ops, D, page, Hq, Hkv):
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_single_token(ops, D, page, Hq, Hkv, room):
     lens = [1, 0, 2, 15, 16, 17, 63, 64, 65, page, page + 1, 127, 129, 0, 1000, 3]
-    _attend_case(ops, 1, Hq, Hkv, D, page, lens, seed=D + page + Hq)
+    _attend_case(ops, 1, Hq, Hkv, D, page, lens, seed=D + page + Hq, room=room)
 
 
 @pytest.mark.parametrize("Sq", [2, 3, 4, 9])
 @pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (3, 1, 64), (32, 1, 64)])
-def test_sdpa_kv8_several_tokens(ops, Sq, Hq, Hkv, D):
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_several_tokens(ops, Sq, Hq, Hkv, D, room):
     lens = [0, 1, Sq - 1, Sq, Sq + 1, 16, 70, 333]  # the first queries of a sequence shorter than Sq see nothing
-    _attend_case(ops, Sq, Hq, Hkv, D, 32, lens, seed=Sq + Hq, fused=True)
+    _attend_case(ops, Sq, Hq, Hkv, D, 32, lens, seed=Sq + Hq, fused=True, room=room)
 
 
-def test_sdpa_kv8_long_and_ragged(ops):
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_long_and_ragged(ops, room):
     # few sequences: every row is cut over many CTAs; the longest next to the shortest
-    _attend_case(ops, 1, 4, 1, 128, 128, [40000], seed=1)
-    _attend_case(ops, 1, 4, 2, 128, 64, [1, 20000, 0, 300, 64], seed=2)
-    _attend_case(ops, 2, 8, 4, 64, 16, [5, 9000, 1], seed=3, fused=True)
+    _attend_case(ops, 1, 4, 1, 128, 128, [40000], seed=1, room=room)
+    _attend_case(ops, 1, 4, 2, 128, 64, [1, 20000, 0, 300, 64], seed=2, room=room)
+    _attend_case(ops, 2, 8, 4, 64, 16, [5, 9000, 1], seed=3, fused=True, room=room)
 
 
-def test_sdpa_kv8_many_sequences(ops):
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_many_sequences(ops, room):
     lens = [(b * 7919) % 130 for b in range(300)]
-    _attend_case(ops, 1, 2, 1, 64, 16, lens, seed=4)
+    _attend_case(ops, 1, 2, 1, 64, 16, lens, seed=4, room=room)
+    _attend_case(ops, 1, 9, 1, 128, 16, [17] * 700, seed=5, room=room)
 
 
 @pytest.mark.parametrize("q_scale,sigma_exp", [(30.0, (-2, 3)), (1.0, (-58, -40)), (1e-25, (60, 110)), (1.0, (-20, 4)), (0.0, (-2, 3))])
-def test_sdpa_kv8_extreme_scales(ops, q_scale, sigma_exp):
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_extreme_scales(ops, q_scale, sigma_exp, room):
     # peaked rows; pages whose scales lie far apart (a small-scale page may carry all the probability); zero queries
-    _attend_case(ops, 1, 4, 2, 128, 16, [200, 33, 1], seed=5, q_scale=q_scale, sigma_exp=sigma_exp)
+    _attend_case(ops, 1, 4, 2, 128, 16, [200, 33, 1], seed=5, q_scale=q_scale, sigma_exp=sigma_exp, room=room)
 
 
-def test_sdpa_kv8_zero_scale_pages(ops):
-    got, q, cache, table, lens = _attend_case(ops, 1, 4, 2, 128, 16, [100, 40], seed=6, check=False)
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_zero_scale_pages(ops, room):
+    got, q, cache, table, lens = _attend_case(ops, 1, 4, 2, 128, 16, [100, 40], seed=6, check=False, room=room)
     cache.v_scale[table[0, 2]] = 0.0
     cache.k_scale[table[0, 3]] = 0.0
-    cache.v_scale[table[1]] = 0.0
+    cache.v_scale[table[1, :3]] = 0.0
     out = ops.sdpa_kv8(q, cache, table, lens)
     _attend_check(ops, out, q.cpu(), _to(cache, "cpu"), table.cpu(), lens.tolist(), 1 / math.sqrt(128))
 
 
-def test_sdpa_kv8_non_finite_inputs_reach_their_rows_only(ops):
-    got, q, cache, table, lens = _attend_case(ops, 1, 4, 2, 128, 16, [100, 40, 70], seed=7, check=False)
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_non_finite_inputs_reach_their_rows_only(ops, room):
+    got, q, cache, table, lens = _attend_case(ops, 1, 4, 2, 128, 16, [100, 40, 70], seed=7, check=False, room=room)
     q = q.clone()
     q[1, 0, 0, 5] = float("inf")
     cache.v.view(torch.uint8)[table[2, 1], 1, 3, 9] = 0x7f  # one value of sequence 2, KV head 1, channel 9
@@ -460,8 +475,9 @@ def test_sdpa_kv8_non_finite_inputs_reach_their_rows_only(ops):
     assert nan[0, 0, :2].all() and not nan[0, 0, 2:].any()
 
 
-def test_sdpa_kv8_same_bits_every_time_and_given_buffers(ops):
-    got, q, cache, table, lens = _attend_case(ops, 1, 8, 2, 128, 64, [5000, 0, 77], seed=8, check=False)
+@pytest.mark.parametrize("room", ROOM)
+def test_sdpa_kv8_same_bits_every_time_and_given_buffers(ops, room):
+    got, q, cache, table, lens = _attend_case(ops, 1, 8, 2, 128, 64, [5000, 0, 77], seed=8, check=False, room=room)
     ws = ops.sdpa_kv8_workspace(3, 1, 8, cache, table.shape[1])
     ws.fill_(255)  # holds nothing between calls
     out = torch.full_like(got, float("nan"))
@@ -493,12 +509,14 @@ def test_sdpa_kv8_offsets_past_32_bits(ops):
     _attend_check(ops, out, q, small, torch.tensor([[0, 1, 2]]), [600], 1 / math.sqrt(D))
 
 
-def test_kv8_captured_step_replays_with_new_lengths(ops):
+@pytest.mark.parametrize("max_pages", [4, 1 << 16])
+def test_kv8_captured_step_replays_with_new_lengths(ops, max_pages):
     """Append and attention in one captured graph; tokens, lengths and page table are device data."""
-    B, Hq, Hkv, D, page, max_pages = 3, 8, 2, 128, 16, 4
+    B, Hq, Hkv, D, page, used = 3, 8, 2, 128, 16, 4
     g = _gen(10)
-    cache = ops.kv8_cache(B * max_pages, Hkv, page, D)
-    table = torch.randperm(B * max_pages, generator=g).view(B, max_pages).int().cuda()
+    cache = ops.kv8_cache(B * used, Hkv, page, D)
+    table = torch.full((B, max_pages), -1, dtype=torch.int32, device="cuda")
+    table[:, :used] = torch.randperm(B * used, generator=g).view(B, used).int().cuda()
     cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
     ctx = torch.zeros(B, dtype=torch.int32, device="cuda")
     qkv = torch.empty(B, Hq + 2 * Hkv, D, dtype=torch.bfloat16, device="cuda")
@@ -524,7 +542,7 @@ def test_kv8_captured_step_replays_with_new_lengths(ops):
     ops.device_status()
     assert ctx.tolist() == [40] * B
     _attend_check(ops, out, keys[-1][:, :Hq].unsqueeze(1), _to(cache, "cpu"), table.cpu(), [40] * B, 1 / math.sqrt(D))
-    want = ops.kv8_cache(B * max_pages, Hkv, page, D, device="cpu")
+    want = ops.kv8_cache(B * used, Hkv, page, D, device="cpu")
     for i, x in enumerate(keys):
         _append_ref(want.k, want.k_scale, x[:, Hq:Hq + Hkv], table.cpu(), [i] * B, list(range(B + 1)))
         _append_ref(want.v, want.v_scale, x[:, Hq + Hkv:], table.cpu(), [i] * B, list(range(B + 1)))
@@ -551,7 +569,7 @@ def test_kv8_refusals(ops):
         lambda: ops.sdpa_kv8(q[:, :, :3].contiguous(), cache, table, lens),
         lambda: ops.sdpa_kv8(q[:1], cache, table, lens),
         lambda: ops.sdpa_kv8(q, cache, table[:, :0].contiguous(), lens),
-        lambda: ops.sdpa_kv8(q, cache, table, lens, workspace=torch.empty(16, dtype=torch.uint8, device="cuda")),
+        lambda: ops.sdpa_kv8(q, cache, table.repeat(1, 1 << 16), lens, workspace=torch.empty(16, dtype=torch.uint8, device="cuda")),
         lambda: ops.sdpa_kv8(q, cache, table, lens, out=torch.empty(2, 1, 4, 32, dtype=torch.bfloat16, device="cuda")),
         lambda: ops.sdpa_kv8(torch.randn(2, 1, 4, 96, device="cuda").bfloat16(), ops.kv8_cache(4, 2, 16, 96), table, lens),
         lambda: ops.sdpa_kv8(torch.randn(2, 1, 4, 68, device="cuda").bfloat16()[..., 4:], cache, table, lens),

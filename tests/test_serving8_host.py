@@ -55,11 +55,12 @@ def _attend(lib, h, **kw):
 
 
 @pytest.mark.parametrize("kw,want", [
-    (dict(q=0), "ARG"), (dict(ws=0), "ARG"), (dict(B=0), "SHAPE"), (dict(Sq=0), "SHAPE"), (dict(Hq=7), "SHAPE"),
+    (dict(q=0), "ARG"), (dict(ws=0, max_pages=1 << 20), "ARG"), (dict(B=0), "SHAPE"), (dict(Sq=0), "SHAPE"), (dict(Hq=7), "SHAPE"),
     (dict(Hkv=0), "SHAPE"), (dict(page=0), "SHAPE"), (dict(page=48), "SHAPE"), (dict(D=256), "SHAPE"), (dict(D=0), "SHAPE"),
     (dict(max_pages=0), "SHAPE"), (dict(max_pages=1 << 28), "SHAPE"), (dict(ld_q=1016), "SHAPE"), (dict(ld_q=1028), "ALIGN"),
     (dict(q=P + 4), "ALIGN"), (dict(o=P + 8), "ALIGN"), (dict(ws=P + 8), "ALIGN"), (dict(lens=P + 2), "ALIGN"),
-    (dict(B=1 << 40), "LIMIT"), (dict(Sq=1 << 31), "LIMIT"), (dict(B=1 << 30, Hkv=8), "LIMIT"), (dict(), "WORKSPACE")])
+    (dict(B=1 << 40), "LIMIT"), (dict(Sq=1 << 31), "LIMIT"), (dict(B=1 << 30, Hkv=8), "LIMIT"), (dict(num_pages=1 << 28), "LIMIT"),
+    (dict(max_pages=1 << 26, Hq=256, Hkv=256, ld_q=1 << 15), "LIMIT"), (dict(max_pages=1 << 20), "WORKSPACE")])
 def test_attention_refuses(lib, fake_handle, kw, want):
     from deplodock_b200 import cabi
 
@@ -73,7 +74,8 @@ def test_workspace_of_bad_sizes_is_zero(lib, fake_handle):
     for sizes in ((0, 1, 8, 2, 64, 128), (1, 1, 7, 2, 64, 128), (1, 1, 8, 0, 64, 128), (1, 1, 8, 2, 0, 128), (1, 1, 8, 2, 64, 96),
                   (1 << 62, 1, 8, 2, 64, 128), (1, 1 << 62, 8, 2, 64, 128)):
         assert f(fake_handle, *sizes) == 0
-    assert f(fake_handle, 2, 1, 8, 2, 64, 128) >= 2 * 2 * 8
+    assert f(fake_handle, 2, 1, 8, 2, 64, 128) == 0  # short sequences need none
+    assert f(fake_handle, 2, 1, 8, 2, 1 << 20, 128) >= 2 * 2 * 8
 
 
 def _norm(lib, h, **kw):
