@@ -5,9 +5,14 @@
 // No rounding between the sum's and the output's: y stays in fp32 until it is divided by the scale (the bf16 kernel of
 // emk_rmsnorm.cu rounds the normalised value as the eager module does; here the only consumer is the 8-bit rounding).
 //
-// Bound by HBM: x, residual in, h, q out, one pass, the row in registers across both reductions (sum of squares, then
-// the maximum of |y|, which needs the first). A warp holds a row where there are many rows and they fit one warp's
-// registers, eight warps hold it otherwise; rows longer than 8 vectors a thread are re-read (L2) instead.
+// Bound by HBM: x, residual in, h, q out, one pass, the row in registers. r = rsqrt(...) is a positive factor of the whole
+// row, so max |y| = r * max |f * w| and one reduction carries both the sum of squares and the maximum: the row's serial
+// chain (load, reduce, store) is what a warp waits on. All loads of a row are issued before the first store of its sum
+// (they may alias), 8 to 256 threads share a row so that none holds more than four 16-byte packs, and rows of any length at
+// any offset go through the same packs, taken at the aligned places of the whole array with the row's ends masked.
+// Measured at 32768 x 1024 bf16 with a residual (235 MB): two reductions and loads behind stores 55.8 us, loads first 45.1,
+// this form 39.9 (0.90 of the copy bandwidth); 32768 x 1001 (their weights still go element by element): 83.7 us element by
+// element, 49.0 in packs.
 #include "emk_common.cuh"
 
 #include <cuda_fp8.h>
@@ -51,15 +56,14 @@ struct alignas(sizeof(T) * V) Pack {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_pack(const T* p, float* f) {
+__device__ __forceinline__ Pack<T, V> load_raw(const T* p) {
   Pack<T, V> a;
   if constexpr (sizeof(a) == 16) {
     *reinterpret_cast<uint4*>(&a) = __ldcs(reinterpret_cast<const uint4*>(p));
   } else {
     a = *reinterpret_cast<const Pack<T, V>*>(p);
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = to_f<T>(a.e[i]);
+  return a;
 }
 // the weight row: read by every row, so with the default caching
 template <typename T, int V>
@@ -68,112 +72,203 @@ __device__ __forceinline__ void load_weight(const T* p, float* f) {
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = to_f<T>(a.e[i]);
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_pack(T* p, const float* f) {
-  Pack<T, V> a;
-#pragma unroll
-  for (int i = 0; i < V; ++i) a.e[i] = from_f<T>(f[i]);
-  *reinterpret_cast<Pack<T, V>*>(p) = a;
-}
+// V codes of y * k
 template <int V>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float* y, float inv) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* y, float k) {
   if constexpr (V == 1) {
-    *p = __nv_cvt_float_to_fp8(y[0] * inv, __NV_SATFINITE, __NV_E4M3);
+    *p = __nv_cvt_float_to_fp8(y[0] * k, __NV_SATFINITE, __NV_E4M3);
   } else {
     Pack<uint16_t, V / 2> o;
 #pragma unroll
     for (int i = 0; i < V / 2; ++i)
-      o.e[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * inv, y[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      o.e[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * k, y[2 * i + 1] * k), __NV_SATFINITE, __NV_E4M3);
     *reinterpret_cast<Pack<uint16_t, V / 2>*>(p) = o;
-  }
-}
-
-// One element pack of the normalised input: the residual is added in fp32 and rounded once to T, and that rounded sum
-// is both what is stored and what is normalised.
-template <typename T, int V>
-__device__ __forceinline__ void load_sum(const T* x, const T* residual, T* hidden, int64_t at, float* f) {
-  load_pack<T, V>(x + at, f);
-  if (residual != nullptr) {
-    float r[V];
-    load_pack<T, V>(residual + at, r);
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = to_f<T>(from_f<T>(f[i] + r[i]));
-    store_pack<T, V>(hidden + at, f);
   }
 }
 
 __device__ __forceinline__ float row_scale(float amax) { return max_nan(amax, AMAX_FLOOR) / E4M3_MAX; }
 
-// WPR warps hold a row (1 or 8), NV packs of V elements a thread.
-template <typename T, int V, int NV, int WPR>
-__global__ void __launch_bounds__(256) rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w,
-                                                           uint8_t* __restrict__ q, float* __restrict__ scale, T* hidden,
-                                                           int64_t rows, int cols, float eps) {
-  constexpr int TPR = WPR * 32;
-  __shared__ float red_sum[8], red_max[8];
+// 16 bytes of a row, kept as they are loaded (a bf16 pack that the compiler takes apart costs a register an element).
+template <typename T>
+struct Raw;
+template <>
+struct Raw<float> {
+  static constexpr int V = 4;
+  static __device__ __forceinline__ void unpack(uint4 u, float* f) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Raw<__nv_bfloat16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ void unpack(uint4 u, float* f) {
+    f[0] = bf16_lo(u.x); f[1] = bf16_hi(u.x); f[2] = bf16_lo(u.y); f[3] = bf16_hi(u.y);
+    f[4] = bf16_lo(u.z); f[5] = bf16_hi(u.z); f[6] = bf16_lo(u.w); f[7] = bf16_hi(u.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+};
+
+// TPR threads hold a row (8, 32, 64, 128 or 256), NV packs of V elements each. RAGGED: the rows' length is no multiple of V;
+// packs lie at the multiples of V of the whole array, and the elements of a row before its first and behind its last full
+// pack (fewer than V each) go to one thread each. RES: with a residual (a kernel of its own: without one a row needs half
+// the registers, and twice the rows fit an SM).
+template <typename T, int NV, int TPR, bool RAGGED, bool RES>
+__global__ void __launch_bounds__(256, RAGGED ? (NV == 4 && !RES ? 3 : 2) : NV == 8 ? (RES ? 2 : 3) : NV == 4 ? (RES ? 3 : 4) : 5)
+rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint8_t* __restrict__ q, float* __restrict__ scale,
+                    T* hidden, int64_t rows, int cols, float eps) {
+  constexpr int V = Raw<T>::V;
+  constexpr int RPC = 256 / TPR;                       // rows per CTA
+  constexpr int LANES = TPR < 32 ? TPR : 32;           // lanes of a warp that share a row
+  constexpr int WPR = TPR < 32 ? 1 : TPR / 32;         // warps that share a row
+  static_assert(!RAGGED || TPR >= V, "a thread per odd element");
+  __shared__ float red[2][2][8];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int tid = WPR == 1 ? lane : (int)threadIdx.x;
-  const int64_t first = WPR == 1 ? (int64_t)blockIdx.x * 8 + wid : blockIdx.x;
-  const int64_t step = WPR == 1 ? (int64_t)gridDim.x * 8 : gridDim.x;
-  const int nvec = cols / V;
-  for (int64_t row = first; row < rows; row += step) {
+  const int tid = threadIdx.x % TPR;
+  const float inv_cols = 1.0f / (float)cols;
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * RPC; first < rows; first += (int64_t)gridDim.x * RPC) {
+    const int64_t row = first + threadIdx.x / TPR;
     const int64_t base = row * cols;
-    float f[NV][V];
-    float ss = 0.f;
+    // elements before the first full pack, full packs, elements behind them
+    const int head = RAGGED ? min((int)((-base) & (V - 1)), cols) : 0;
+    const int npack = row < rows ? (cols - head) / V : 0;
+    const int tail = RAGGED ? cols - head - (cols - head) / V * V : 0;
+    const int64_t at = base + head;
+    // all loads of the row first: the stores of the sum may alias them, and would hold back every load behind them
+    uint4 xr[NV], rr[RES ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int vi = i * TPR + tid;
-      if (vi < nvec) {
-        load_sum<T, V>(x, residual, hidden, base + (int64_t)vi * V, f[i]);
+      xr[i] = make_uint4(0, 0, 0, 0);
+      if (vi < npack) xr[i] = __ldcs(reinterpret_cast<const uint4*>(x + at + (int64_t)vi * V));
+    }
+    if (RES) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) ss = fmaf(f[i][e], f[i][e], ss);
+      for (int i = 0; i < NV; ++i) {
+        const int vi = i * TPR + tid;
+        rr[i] = make_uint4(0, 0, 0, 0);
+        if (vi < npack) rr[i] = __ldcs(reinterpret_cast<const uint4*>(residual + at + (int64_t)vi * V));
       }
     }
-    ss = warp_sum(ss);
-    if (WPR > 1) {
-      if (lane == 0) red_sum[wid] = ss;
-      __syncthreads();
-      ss = 0.f;
+    // this thread's odd elements: column tid of the head, column tid of the tail
+    float odd[2] = {0.f, 0.f};
+    int odd_col[2] = {-1, -1};
+    if (RAGGED && row < rows) {
+      if (tid < head) odd_col[0] = tid;
+      if (tid < tail) odd_col[1] = cols - tail + tid;
 #pragma unroll
-      for (int i = 0; i < WPR; ++i) ss += red_sum[i];
+      for (int j = 0; j < 2; ++j) {
+        if (odd_col[j] >= 0) {
+          odd[j] = to_f<T>(x[base + odd_col[j]]);
+          if (RES) odd[j] = to_f<T>(from_f<T>(odd[j] + to_f<T>(residual[base + odd_col[j]])));
+        }
+      }
     }
-    const float r = 1.0f / sqrtf(ss / (float)cols + eps);
-    float amax = 0.f;
+    float f[NV][V];  // f * w
+    float ss = 0.f, amax = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int vi = i * TPR + tid;
-      if (vi < nvec) {
+      if (vi < npack) {
+        float v[V];
+        Raw<T>::unpack(xr[i], v);
+        if (RES) {  // the sum is rounded to T once: what is stored is what is normalised
+          float r[V];
+          Raw<T>::unpack(rr[i], r);
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] += r[e];
+          const uint4 h = Raw<T>::pack(v);
+          Raw<T>::unpack(h, v);
+          *reinterpret_cast<uint4*>(hidden + at + (int64_t)vi * V) = h;
+        }
         float wv[V];
-        load_weight<T, V>(w + (int64_t)vi * V, wv);
+        if constexpr (RAGGED) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) wv[e] = to_f<T>(__ldg(w + head + vi * V + e));
+        } else {
+          Raw<T>::unpack(__ldg(reinterpret_cast<const uint4*>(w + (int64_t)vi * V)), wv);
+        }
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          f[i][e] = (f[i][e] * r) * wv[e];
+          ss = fmaf(v[e], v[e], ss);
+          f[i][e] = v[e] * wv[e];
           amax = max_nan(amax, fabsf(f[i][e]));
         }
       }
     }
-    amax = warp_max_nan(amax);
-    if (WPR > 1) {
-      // the sums of the next row are written after this barrier, when all have read this row's; likewise the maxima
-      if (lane == 0) red_max[wid] = amax;
-      __syncthreads();
-      amax = red_max[0];
+    if (RAGGED) {
 #pragma unroll
-      for (int i = 1; i < WPR; ++i) amax = max_nan(amax, red_max[i]);
+      for (int j = 0; j < 2; ++j) {
+        if (odd_col[j] >= 0) {
+          if (RES) hidden[base + odd_col[j]] = from_f<T>(odd[j]);
+          ss = fmaf(odd[j], odd[j], ss);
+          odd[j] *= to_f<T>(__ldg(w + odd_col[j]));
+          amax = max_nan(amax, fabsf(odd[j]));
+        }
+      }
     }
-    const float s = row_scale(amax);
-    const float inv = 1.0f / s;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
+    if (WPR > 1) {  // (two sets of places in turn: the next row's are written while this row's may still be read)
+      if (lane == 0) {
+        red[turn][0][wid] = ss;
+        red[turn][1][wid] = amax;
+      }
+      __syncthreads();
+      const int w0 = wid / WPR * WPR;
+      ss = red[turn][0][w0];
+      amax = red[turn][1][w0];
+#pragma unroll
+      for (int i = 1; i < WPR; ++i) {
+        ss += red[turn][0][w0 + i];
+        amax = max_nan(amax, red[turn][1][w0 + i]);
+      }
+      turn ^= 1;
+    }
+    const float r = 1.0f / sqrtf(ss * inv_cols + eps);
+    const float s = row_scale(amax * r);
+    const float k = r / s;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int vi = i * TPR + tid;
-      if (vi < nvec) store_codes<V>(q + base + (int64_t)vi * V, f[i], inv);
+      if (vi < npack) store_codes<V>(q + at + (int64_t)vi * V, f[i], k);
     }
-    if (tid == 0) scale[row] = s;
+    if (RAGGED) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (odd_col[j] >= 0) store_codes<1>(q + base + odd_col[j], &odd[j], k);
+    }
+    if (tid == 0 && row < rows) scale[row] = s;
   }
 }
 
-// Rows too long for eight packs a thread: one CTA per row, the row re-read (from L2) for the maximum and the codes. With
-// a residual the later sweeps read the stored sum, each element by the thread that wrote it.
+// One pack of the normalised input: the residual is added in fp32 and rounded once to T, and that rounded sum is both what
+// is stored and what is normalised.
+template <typename T, int V>
+__device__ __forceinline__ void sum_pack(const Pack<T, V>& x, const Pack<T, V>& r, bool add, T* hidden, float* f) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = to_f<T>(x.e[i]);
+  if (add) {
+    Pack<T, V> h;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      h.e[i] = from_f<T>(f[i] + to_f<T>(r.e[i]));
+      f[i] = to_f<T>(h.e[i]);
+    }
+    *reinterpret_cast<Pack<T, V>*>(hidden) = h;
+  }
+}
+
+// Rows too long for the registers of a CTA, and pointers that are not aligned: one CTA per row, the row re-read (from L2)
+// for the codes. With a residual the second sweep reads the stored sum, each element by the thread that wrote it.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) rmsnorm_e4m3_long_kernel(const T* x, const T* residual,
                                                                 const T* __restrict__ w, uint8_t* __restrict__ q,
@@ -185,79 +280,102 @@ __global__ void __launch_bounds__(256) rmsnorm_e4m3_long_kernel(const T* x, cons
     const int64_t base = row * cols;
     const T* src = residual != nullptr ? hidden : x;
     float f[V], wv[V];
-    float ss = 0.f;
+    float ss = 0.f, amax = 0.f;
     for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += 256 * V) {
-      load_sum<T, V>(x, residual, hidden, base + c, f);
+      const Pack<T, V> xr = load_raw<T, V>(x + base + c);
+      Pack<T, V> rr = {};
+      if (residual != nullptr) rr = load_raw<T, V>(residual + base + c);
+      sum_pack<T, V>(xr, rr, residual != nullptr, hidden + base + c, f);
+      load_weight<T, V>(w + c, wv);
 #pragma unroll
-      for (int e = 0; e < V; ++e) ss = fmaf(f[e], f[e], ss);
+      for (int e = 0; e < V; ++e) {
+        ss = fmaf(f[e], f[e], ss);
+        amax = max_nan(amax, fabsf(f[e] * wv[e]));
+      }
     }
     ss = warp_sum(ss);
-    if (lane == 0) red_sum[wid] = ss;
-    __syncthreads();
-    ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += red_sum[i];
-    const float r = 1.0f / sqrtf(ss / (float)cols + eps);
-    float amax = 0.f;
-    for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += 256 * V) {
-      load_weight<T, V>(src + base + c, f);
-      load_weight<T, V>(w + c, wv);
-#pragma unroll
-      for (int e = 0; e < V; ++e) amax = max_nan(amax, fabsf((f[e] * r) * wv[e]));
-    }
     amax = warp_max_nan(amax);
-    if (lane == 0) red_max[wid] = amax;
+    if (lane == 0) {
+      red_sum[wid] = ss;
+      red_max[wid] = amax;
+    }
     __syncthreads();
+    ss = red_sum[0];
     amax = red_max[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) amax = max_nan(amax, red_max[i]);
-    const float s = row_scale(amax);
-    const float inv = 1.0f / s;
+    for (int i = 1; i < 8; ++i) {
+      ss += red_sum[i];
+      amax = max_nan(amax, red_max[i]);
+    }
+    __syncthreads();
+    const float r = 1.0f / sqrtf(ss / (float)cols + eps);
+    const float s = row_scale(amax * r);
+    const float k = r / s;
     for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += 256 * V) {
       load_weight<T, V>(src + base + c, f);
       load_weight<T, V>(w + c, wv);
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = (f[e] * r) * wv[e];
-      store_codes<V>(q + base + c, f, inv);
+      for (int e = 0; e < V; ++e) f[e] *= wv[e];
+      store_codes<V>(q + base + c, f, k);
     }
     if (threadIdx.x == 0) scale[row] = s;
   }
 }
 
-template <typename T, int V>
-int launch_vec(emk_handle_t h, const T* x, const T* residual, const T* w, uint8_t* q, float* scale, T* hidden,
-               int64_t rows, int64_t cols, float eps, cudaStream_t s) {
-  const int64_t nvec = cols / V;
-  const int64_t cap = (int64_t)h->sm_count * 16;
-  // A warp a row needs enough rows to fill the machine; below that the row's latency counts and eight warps share it.
-  if (nvec <= 32 * 8 && rows >= (int64_t)h->sm_count * 8) {
-    const int64_t ctas = (rows + 7) / 8;
-    const unsigned grid = (unsigned)(ctas < cap ? ctas : cap);
-    if (nvec <= 32) rmsnorm_e4m3_kernel<T, V, 1, 1><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else if (nvec <= 64) rmsnorm_e4m3_kernel<T, V, 2, 1><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else if (nvec <= 128) rmsnorm_e4m3_kernel<T, V, 4, 1><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else rmsnorm_e4m3_kernel<T, V, 8, 1><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-  } else {
-    const unsigned grid = (unsigned)(rows < cap ? rows : cap);
-    if (nvec <= 256) rmsnorm_e4m3_kernel<T, V, 1, 8><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else if (nvec <= 512) rmsnorm_e4m3_kernel<T, V, 2, 8><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else if (nvec <= 1024) rmsnorm_e4m3_kernel<T, V, 4, 8><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else if (nvec <= 2048) rmsnorm_e4m3_kernel<T, V, 8, 8><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, (int)cols, eps);
-    else rmsnorm_e4m3_long_kernel<T, V><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, cols, eps);
-  }
+template <typename T, int NV, int TPR, bool RAGGED>
+int launch_rows(emk_handle_t h, const T* x, const T* residual, const T* w, uint8_t* q, float* scale, T* hidden, int64_t rows,
+                int cols, float eps, cudaStream_t s) {
+  const int64_t ctas = (rows + 256 / TPR - 1) / (256 / TPR), cap = (int64_t)h->sm_count * 16;
+  const unsigned grid = (unsigned)(ctas < cap ? ctas : cap);
+  if (residual != nullptr)
+    rmsnorm_e4m3_kernel<T, NV, TPR, RAGGED, true><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, cols, eps);
+  else
+    rmsnorm_e4m3_kernel<T, NV, TPR, RAGGED, false><<<grid, 256, 0, s>>>(x, residual, w, q, scale, hidden, rows, cols, eps);
   EMK_LAUNCH_CHECK(h);
   return EMK_OK;
+}
+
+// Threads per row: as few as hold it in four packs each where there are rows for all SMs (short chains of reductions, many
+// rows in flight), at least half a CTA where there are not (the row's latency counts).
+template <typename T, bool RAGGED>
+int launch_packs(emk_handle_t h, const T* x, const T* residual, const T* w, uint8_t* q, float* scale, T* hidden, int64_t rows,
+                 int cols, float eps, cudaStream_t s) {
+  const int n = cols / Raw<T>::V > 0 ? cols / Raw<T>::V : 1;  // full packs a row has at most
+#define EMK_NORM(NV, TPR) launch_rows<T, NV, TPR, RAGGED>(h, x, residual, w, q, scale, hidden, rows, cols, eps, s)
+  if (rows >= (int64_t)h->sm_count * 8) {
+    if (n <= 8) return EMK_NORM(1, 8);
+    if (n <= 16) return EMK_NORM(2, 8);
+    if (n <= 32) return EMK_NORM(4, 8);
+    if (n <= 64) return EMK_NORM(2, 32);
+    if (n <= 128) return EMK_NORM(4, 32);
+    if (n <= 256) return EMK_NORM(4, 64);
+  }
+  if (n <= 128) return EMK_NORM(1, 128);
+  if (n <= 256) return EMK_NORM(2, 128);
+  if (n <= 512) return EMK_NORM(4, 128);
+  if (n <= 1024) return EMK_NORM(4, 256);
+  return EMK_NORM(8, 256);
+#undef EMK_NORM
 }
 
 template <typename T>
 int launch(emk_handle_t h, const void* x, const void* residual, const void* w, void* q, float* scale, void* hidden,
            int64_t rows, int64_t cols, float eps, cudaStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const uintptr_t at = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)w | (uintptr_t)hidden;
+  constexpr int V = Raw<T>::V;
   const T *xt = (const T*)x, *rt = (const T*)residual, *wt = (const T*)w;
-  if (cols % V == 0 && (at & 15u) == 0 && ((uintptr_t)q & (V - 1)) == 0)
-    return launch_vec<T, V>(h, xt, rt, wt, (uint8_t*)q, scale, (T*)hidden, rows, cols, eps, s);
-  return launch_vec<T, 1>(h, xt, rt, wt, (uint8_t*)q, scale, (T*)hidden, rows, cols, eps, s);
+  const bool packs = (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)hidden) & 15u) == 0 && ((uintptr_t)q & (V - 1)) == 0;
+  if (packs && cols / V <= 2048) {
+    if (cols % V == 0 && ((uintptr_t)w & 15u) == 0)
+      return launch_packs<T, false>(h, xt, rt, wt, (uint8_t*)q, scale, (T*)hidden, rows, (int)cols, eps, s);
+    return launch_packs<T, true>(h, xt, rt, wt, (uint8_t*)q, scale, (T*)hidden, rows, (int)cols, eps, s);
+  }
+  const unsigned grid = (unsigned)(rows < (int64_t)h->sm_count * 16 ? rows : (int64_t)h->sm_count * 16);
+  if (packs && cols % V == 0 && ((uintptr_t)w & 15u) == 0)
+    rmsnorm_e4m3_long_kernel<T, V><<<grid, 256, 0, s>>>(xt, rt, wt, (uint8_t*)q, scale, (T*)hidden, rows, cols, eps);
+  else
+    rmsnorm_e4m3_long_kernel<T, 1><<<grid, 256, 0, s>>>(xt, rt, wt, (uint8_t*)q, scale, (T*)hidden, rows, cols, eps);
+  EMK_LAUNCH_CHECK(h);
+  return EMK_OK;
 }
 
 }  // namespace

@@ -112,10 +112,10 @@ int emk_softmax_lastdim(emk_handle_t h, const void* x, void* y, int64_t rows, in
 /* RMSNorm with the residual's addition and an e4m3 output with one scale per row, for the 8-bit linear layers:
  *   f = x, or with a residual f = round(x + residual) to `dtype`, stored to hidden (the new residual stream);
  *   y = f * rsqrt(mean(f^2) + eps) * w in fp32;  scale[row] = max(max |y|, 2^-100) / 448;  q = e4m3(y / scale[row]).
- * A row with a NaN becomes NaN codes with a NaN scale. x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or
+ * A row with a NaN or an infinity (or a product f * w past fp32's range) becomes NaN codes with a NaN scale. x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or
  * EMK_BF16), residual and hidden both given or both NULL; hidden may be x or residual itself (in place), q may alias
- * nothing. w: [cols] of `dtype`; q: [rows, cols] e4m3; scale: fp32 [rows]. Any cols; rows of a multiple of 16 bytes at
- * 16-byte aligned pointers (q 8- or 4-byte) take the vector path. No counterpart in the reference (no 8-bit path). */
+ * nothing. w: [cols] of `dtype`; q: [rows, cols] e4m3; scale: fp32 [rows]. Any cols; pointers that are 16-byte aligned (q
+ * 8-byte) take the vector path. No counterpart in the reference (no 8-bit path). */
 int emk_rmsnorm_e4m3(emk_handle_t h, const void* x, const void* residual, const void* w, void* q, float* scale,
                      void* hidden, int64_t rows, int64_t cols, float eps, int dtype, emk_stream_t stream);
 
