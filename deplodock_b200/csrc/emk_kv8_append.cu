@@ -9,10 +9,15 @@
 // more each time its page's scale grows. Non-finite values become NaN codes and do not enter the scale: one bad token
 // must not wipe out its page.
 //
-// Bound by HBM for prompts (2 bytes read, 1 written per value), by launch latency for single tokens. One CTA owns one
-// (touched page, KV head, K or V): the page's maximum, its scale and the rewrite of its earlier codes need no other CTA, so
-// there are no atomics and no second pass over the cache. The appended rows are read twice (maximum, then codes); the
-// second read of at most 64 KB comes from L1 / L2.
+// Bound by HBM for prompts (2 bytes read, 1 written per value), by launch latency for single tokens. One group of threads
+// owns one (touched page, KV head, K or V): the page's maximum, its scale and the rewrite of its earlier codes need no one
+// else, so there are no atomics and no second pass; the appended rows stay in registers (at most eight 16-byte pieces a
+// thread) between the maximum and the codes. A CTA finds its page once and walks its heads. Which page that is needs no sum
+// over the sequences: sequence b gets the places cu[b] / page + 2 b up to the next one's, never fewer than the pages it
+// can touch, and a warp finds b among 32 places at a time.
+// Measured, 64 sequences of 512 tokens behind up to 2000, 8 heads of 128 (201 MB): rows read twice, a CTA per head 49.0 us;
+// rows in registers, values taken apart into floats 47.3; on pairs of bf16, which leaves the issue slots to eight CTAs an SM
+// 38.4 (0.80 of the copy bandwidth). Pages of 16 tokens 86.9 and 37.5; 256 single tokens 16.1 and 5.2.
 #include "emk_kv8.cuh"
 
 #include <cuda_fp8.h>
@@ -21,7 +26,7 @@ namespace {
 
 using namespace emk;
 
-constexpr int AP_THREADS = 128;
+constexpr int AP_PIECES = 8;  // 16-byte pieces of a page's new rows that a thread holds
 
 struct AppendArgs {
   const __nv_bfloat16* x[2];  // keys, values: [T] rows of pitch ld, head h at h * D
@@ -33,6 +38,8 @@ struct AppendArgs {
   const int32_t* cu;
   int B, max_pages, num_pages, Hkv, page_shift;
   int64_t T;
+  int64_t items;  // places
+  int groups;     // CTAs per place
   int* status;
 };
 
@@ -44,12 +51,45 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-__device__ __forceinline__ float finite_abs(float v) {
-  const float a = fabsf(v);
-  return a <= 3.402823466e38f ? a : 0.f;  // false for infinities and NaN
+// Pairs of bf16 as they are loaded: taken apart into floats, a value cost eleven instructions and their issue was the bound.
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
-// values past the finite range become NaN before the saturating conversion
-__device__ __forceinline__ float nan_if_infinite(float v) { return fabsf(v) <= 3.402823466e38f ? v : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {  // the other one where one is NaN
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// NaN in the place of infinities: x * 0 + x
+__device__ __forceinline__ uint4 finite_or_nan(uint4 v) {
+  return make_uint4(fma_bf16x2(v.x, 0u, v.x), fma_bf16x2(v.y, 0u, v.y), fma_bf16x2(v.z, 0u, v.z), fma_bf16x2(v.w, 0u, v.w));
+}
+// running maximum of the magnitudes, a pair; v from finite_or_nan, whose NaN it passes over
+__device__ __forceinline__ uint32_t max_abs(uint32_t m, uint4 v) {
+  m = max_bf16x2(m, v.x & 0x7fff7fffu);
+  m = max_bf16x2(m, v.y & 0x7fff7fffu);
+  m = max_bf16x2(m, v.z & 0x7fff7fffu);
+  return max_bf16x2(m, v.w & 0x7fff7fffu);
+}
+__device__ __forceinline__ float pair_max(uint32_t m) { return fmaxf(bf16_lo(m), bf16_hi(m)); }
+// Codes of v / s for inv = 1 / s. The product is exact in bf16: s is a power of two (where it is not, because the caller's
+// scale was none, this rounds once more), and what falls below bf16's range is a zero code anyway.
+__device__ __forceinline__ uint2 piece_codes(uint4 v, float inv) {
+  const uint32_t k = pack_bf16x2(inv, inv);
+  const uint32_t w[4] = {mul_bf16x2(v.x, k), mul_bf16x2(v.y, k), mul_bf16x2(v.z, k), mul_bf16x2(v.w, k)};
+  uint32_t o[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    o[j >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(bf16_lo(w[j]), bf16_hi(w[j])), __NV_SATFINITE, __NV_E4M3) << (16 * (j & 1));
+  return make_uint2(o[0], o[1]);
+}
 
 __device__ __forceinline__ void rescale_codes4(uint32_t& c, float ratio) {
   uint32_t out = 0;
@@ -62,114 +102,197 @@ __device__ __forceinline__ void rescale_codes4(uint32_t& c, float ratio) {
   c = out;
 }
 
-template <int D>
-__global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(const AppendArgs a) {
-  constexpr int LPT = D / 8;  // lanes (16-byte pieces) per token
-  constexpr int TPP = AP_THREADS / LPT;  // tokens per pass of the CTA
-  __shared__ float red[AP_THREADS / 32];
+// First place of sequence b (see the top): between 0 and items, not falling in b for lengths that do not fall.
+__device__ __forceinline__ int64_t first_place(const AppendArgs& a, int b) {
+  const int64_t t = min(max((int64_t)__ldg(a.cu + b), (int64_t)0), a.T);
+  return (t >> a.page_shift) + 2 * (int64_t)b;
+}
+
+// What a place stands for; false where nothing does.
+struct Touched {
+  int at, m;      // tokens that stay in the page, tokens that are appended to it
+  int pid;
+  int64_t row0;   // first appended row
+};
+
+__device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t place, Touched& p) {
   const int lane = threadIdx.x & 31;
-  const int head = blockIdx.y, which = blockIdx.z;
   const int page = 1 << a.page_shift;
-
-  // ---- which sequence and which of its touched pages is item blockIdx.x (every warp finds it for itself) ----
-  int64_t item = blockIdx.x;
-  int seq = -1;
-  int64_t ctx = 0, t0 = 0, n = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane;
-    int64_t c_ctx = 0, c_t0 = 0, c_n = 0, count = 0;
-    if (b < a.B) {
-      const int64_t lo = a.cu[b], hi = a.cu[b + 1], held = a.ctx_lens[b];
-      c_t0 = min(max(lo, (int64_t)0), a.T);
-      c_n = max(min(hi, a.T) - c_t0, (int64_t)0);
-      if (lo < 0 || hi > a.T || hi < lo) emk_record_bounds(a.status, EMK_DEV_BOUNDS_CU_SEQLENS);
-      c_ctx = max(held, (int64_t)0);
-      const int64_t room = ((int64_t)a.max_pages << a.page_shift) - c_ctx;
-      if (held < 0 || c_n > max(room, (int64_t)0)) emk_record_bounds(a.status, EMK_DEV_BOUNDS_CACHE_LEN);
-      c_n = min(c_n, max(room, (int64_t)0));  // tokens that the table's row cannot hold are dropped
-      count = c_n > 0 ? ((c_ctx & (page - 1)) + c_n + page - 1) >> a.page_shift : 0;
-    }
-    int64_t upto = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, item < upto);
-    if (past != 0) {
-      const int src = __ffs(past) - 1;
-      item -= __shfl_sync(0xffffffffu, upto - count, src);
-      seq = b0 + src;
-      ctx = __shfl_sync(0xffffffffu, c_ctx, src);
-      t0 = __shfl_sync(0xffffffffu, c_t0, src);
-      n = __shfl_sync(0xffffffffu, c_n, src);
-      break;
-    }
-    item -= __shfl_sync(0xffffffffu, upto, 31);
+  // the last sequence b with first_place(b) <= place, 32 candidates at a time (every warp finds it for itself)
+  int lo = 0, n_left = a.B;  // b lies in [lo, lo + n_left)
+  while (n_left > 1) {
+    const int step = (n_left + 31) / 32;
+    const bool before = lane * step < n_left && first_place(a, lo + lane * step) <= place;
+    const unsigned m = __ballot_sync(0xffffffffu, before);
+    const int i = m == 0 ? 0 : 31 - __clz(m);
+    lo += i * step;
+    n_left = min(step, n_left - i * step);
   }
-  if (seq < 0) return;  // uniform: the grid is an upper bound of the touched pages
-
-  const int64_t slot = (ctx >> a.page_shift) + item;             // which page of the sequence
-  const int64_t first = max(ctx, slot << a.page_shift);          // first and one past the last new token position in it
+  const int seq = lo;
+  const int64_t t0 = min(max((int64_t)a.cu[seq], (int64_t)0), a.T);
+  const int64_t t1 = a.cu[seq + 1], held = a.ctx_lens[seq];
+  const int64_t ctx = max(held, (int64_t)0);
+  const int64_t room = max(((int64_t)a.max_pages << a.page_shift) - ctx, (int64_t)0);
+  int64_t n = max(min(t1, a.T) - t0, (int64_t)0);
+  if (t1 > a.T || t1 < a.cu[seq] || a.cu[seq] < 0) emk_record_bounds(a.status, EMK_DEV_BOUNDS_CU_SEQLENS);
+  if (held < 0 || n > room) emk_record_bounds(a.status, EMK_DEV_BOUNDS_CACHE_LEN);
+  n = min(n, room);  // tokens that the table's row cannot hold are dropped
+  const int64_t slot = (ctx >> a.page_shift) + place - first_place(a, seq);  // which page of the sequence
+  const int64_t first = max(ctx, slot << a.page_shift);                      // new token positions in it: [first, last)
   const int64_t last = min(ctx + n, (slot + 1) << a.page_shift);
-  const int at = (int)(first & (page - 1));                      // tokens that stay in front of them
-  const int m = (int)(last - first);
-  const int pid = a.table[(int64_t)seq * a.max_pages + slot];
-  if (pid < 0 || pid >= a.num_pages) {  // nothing is written through a bad id
+  if (last <= first) return false;  // a place beyond the sequence's pages
+  p.at = (int)(first & (page - 1));
+  p.m = (int)(last - first);
+  p.row0 = t0 + (first - ctx);
+  p.pid = a.table[(int64_t)seq * a.max_pages + slot];
+  if (p.pid < 0 || p.pid >= a.num_pages) {  // nothing is written through a bad id
     emk_record_bounds(a.status, EMK_DEV_BOUNDS_PAGE);
-    return;
+    return false;
   }
-  const int64_t ld = which == 0 ? a.ld[0] : a.ld[1];
-  const __nv_bfloat16* x = (which == 0 ? a.x[0] : a.x[1]) + (t0 + (first - ctx)) * ld + (int64_t)head * D;
-  uint8_t* codes = (which == 0 ? a.codes[0] : a.codes[1]) + (((int64_t)pid * a.Hkv + head) << a.page_shift) * D;
-  float* scale_at = (which == 0 ? a.scales[0] : a.scales[1]) + (int64_t)pid * a.Hkv + head;
-  const int tok = threadIdx.x / LPT, piece = threadIdx.x % LPT;
+  return true;
+}
 
-  // ---- the appended tokens' maximum ----
-  float amax = 0.f;
-  for (int t = tok; t < m; t += TPP) {
-    const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)t * ld + piece * 8);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(finite_abs(bf16_lo(u[i])), finite_abs(bf16_hi(u[i]))));
-  }
-  amax = warp_max(amax);
-  if (lane == 0) red[threadIdx.x >> 5] = amax;
-  const float old = at > 0 ? *scale_at : 0.f;  // read by all before the barrier, written by one after it
-  __syncthreads();
-  amax = red[0];
-#pragma unroll
-  for (int i = 1; i < AP_THREADS / 32; ++i) amax = fmaxf(amax, red[i]);
-  const float mine = pow2_scale(amax);
-  const float s = at > 0 && !(old < mine) ? old : mine;
+// One (head, K or V) of the page: where its rows come from and go to.
+struct Unit {
+  const __nv_bfloat16* x;
+  int64_t ld;
+  uint8_t* codes;
+  float* scale;
+};
+template <int D>
+__device__ __forceinline__ Unit unit_of(const AppendArgs& a, const Touched& p, int u) {
+  const bool v = u >= a.Hkv;
+  const int head = v ? u - a.Hkv : u;
+  const int64_t slab = (int64_t)p.pid * a.Hkv + head;
+  Unit r;
+  r.ld = v ? a.ld[1] : a.ld[0];
+  r.x = (v ? a.x[1] : a.x[0]) + p.row0 * r.ld + (int64_t)head * D;
+  r.codes = (v ? a.codes[1] : a.codes[0]) + (slab << a.page_shift) * D;
+  r.scale = (v ? a.scales[1] : a.scales[0]) + slab;
+  return r;
+}
 
-  // ---- earlier codes of the page, where its scale grew ----
-  if (at > 0 && s != old) {
-    const float ratio = old / s;
-    for (int i = threadIdx.x; i < at * (D / 16); i += AP_THREADS) {
-      uint4 v = reinterpret_cast<uint4*>(codes)[i];
-      rescale_codes4(v.x, ratio);
-      rescale_codes4(v.y, ratio);
-      rescale_codes4(v.z, ratio);
-      rescale_codes4(v.w, ratio);
-      reinterpret_cast<uint4*>(codes)[i] = v;
-    }
+// codes of the first `at` tokens, whose page's scale grew from old to s
+template <int D>
+__device__ __forceinline__ void rescale_page(uint8_t* codes, int at, float ratio, int tid, int threads) {
+#pragma unroll 4
+  for (int i = tid; i < at * (D / 16); i += threads) {
+    uint4 c = reinterpret_cast<uint4*>(codes)[i];
+    rescale_codes4(c.x, ratio);
+    rescale_codes4(c.y, ratio);
+    rescale_codes4(c.z, ratio);
+    rescale_codes4(c.w, ratio);
+    reinterpret_cast<uint4*>(codes)[i] = c;
   }
-  // ---- the new codes ----
+}
+
+// Few tokens a sequence: a warp per (page, head, K or V), nothing held between the two readings of a row (the second one
+// hits L1), so that all warps of a step are resident at once.
+template <int D>
+__global__ void __launch_bounds__(128) kv8_append_few_kernel(const AppendArgs a) {
+  constexpr int LPT = D / 8, TPP = 32 / LPT;
+  const int lane = threadIdx.x & 31;
+  const int u = (int)(blockIdx.x % a.groups) * 4 + (threadIdx.x >> 5);
+  Touched p;
+  if (u >= 2 * a.Hkv || !find_page(a, blockIdx.x / a.groups, p)) return;  // (a warp at a time)
+  const Unit r = unit_of<D>(a, p, u);
+  const int tok = lane / LPT, piece = lane % LPT;
+  const float old = p.at > 0 ? *r.scale : 0.f;
+  uint32_t top = 0;
+  for (int i = tok; i < p.m; i += TPP) top = max_abs(top, finite_or_nan(*reinterpret_cast<const uint4*>(r.x + (int64_t)i * r.ld + piece * 8)));
+  const float amax = warp_max(pair_max(top));
+  const float fresh = pow2_scale(amax);
+  const float s = p.at > 0 && !(old < fresh) ? old : fresh;
+  if (p.at > 0 && s != old) rescale_page<D>(r.codes, p.at, old / s, lane, 32);
   const float inv = 1.0f / s;  // exact: a power of two within 2^-120 .. 2^64
-  for (int t = tok; t < m; t += TPP) {
-    const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)t * ld + piece * 8);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-    uint32_t o[2] = {0, 0};
+  for (int i = tok; i < p.m; i += TPP)
+    *reinterpret_cast<uint2*>(r.codes + (int64_t)(p.at + i) * D + piece * 8) =
+        piece_codes(finite_or_nan(*reinterpret_cast<const uint4*>(r.x + (int64_t)i * r.ld + piece * 8)), inv);
+  __syncwarp();  // all lanes have read the old scale
+  if (lane == 0 && s != old) *r.scale = s;
+}
+
+// TPU threads (a power of two from 32 to 512) per page and head; THREADS >= 128 per CTA. The heads of a page are neighbours
+// in the grid: a token's keys of all heads lie side by side, and are read at about the same time.
+template <int D, int TPU>
+__global__ void __launch_bounds__(TPU < 128 ? 128 : TPU, TPU <= 128 ? 8 : TPU == 256 ? 4 : 2) kv8_append_kernel(const AppendArgs a) {
+  constexpr int THREADS = TPU < 128 ? 128 : TPU;
+  constexpr int GROUPS = THREADS / TPU, WPU = TPU / 32;
+  constexpr int LPT = D / 8;       // pieces per token
+  constexpr int TPP = TPU / LPT;   // tokens per round of the group
+  __shared__ float red[THREADS / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Touched p;
+  if (!find_page(a, blockIdx.x / a.groups, p)) return;  // uniform
+  const int group = threadIdx.x / TPU, tid = threadIdx.x % TPU;
+  const int tok = tid / LPT, piece = tid % LPT;
+  const int u = (int)(blockIdx.x % a.groups) * GROUPS + group;
+  const bool mine = u < 2 * a.Hkv;
+  const Unit r = unit_of<D>(a, p, mine ? u : 0);
+  // ---- the appended tokens and their maximum ----
+  uint4 v[AP_PIECES];
+  uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(
-                       make_float2(nan_if_infinite(bf16_lo(u[i])) * inv, nan_if_infinite(bf16_hi(u[i])) * inv),
-                       __NV_SATFINITE, __NV_E4M3)
-                   << (16 * (i & 1));
-    *reinterpret_cast<uint2*>(codes + (int64_t)(at + t) * D + piece * 8) = make_uint2(o[0], o[1]);
+  for (int i = 0; i < AP_PIECES; ++i) {
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (mine && i * TPP + tok < p.m) v[i] = __ldcs(reinterpret_cast<const uint4*>(r.x + (int64_t)(i * TPP + tok) * r.ld + piece * 8));
   }
-  if (threadIdx.x == 0 && s != old) *scale_at = s;
+  const float old = mine && p.at > 0 ? *r.scale : 0.f;  // read by all before the barrier, written by one after it
+#pragma unroll
+  for (int i = 0; i < AP_PIECES; ++i) {
+    v[i] = finite_or_nan(v[i]);
+    top = max_abs(top, v[i]);
+  }
+  float amax = warp_max(pair_max(top));
+  if (WPU > 1) {
+    if (lane == 0) red[warp] = amax;
+    __syncthreads();
+    amax = red[warp / WPU * WPU];
+#pragma unroll
+    for (int i = 1; i < WPU; ++i) amax = fmaxf(amax, red[warp / WPU * WPU + i]);
+  } else {
+    __syncwarp();
+  }
+  if (!mine) return;
+  const float fresh = pow2_scale(amax);
+  const float s = p.at > 0 && !(old < fresh) ? old : fresh;
+  if (p.at > 0 && s != old) rescale_page<D>(r.codes, p.at, old / s, tid, TPU);
+  const float inv = 1.0f / s;
+#pragma unroll
+  for (int i = 0; i < AP_PIECES; ++i)
+    if (i * TPP + tok < p.m)
+      *reinterpret_cast<uint2*>(r.codes + (int64_t)(p.at + i * TPP + tok) * D + piece * 8) = piece_codes(v[i], inv);
+  if (tid == 0 && s != old) *r.scale = s;
+}
+
+// A CTA per place and `per` of its heads (K and V apart)
+template <typename K>
+int launch_units(emk_handle_t h, K kernel, AppendArgs a, int per, int threads, cudaStream_t s) {
+  a.groups = (2 * a.Hkv + per - 1) / per;
+  if (a.items > 0x7fffffff / a.groups) {
+    EMK_SET_ERR(h, "emk_kv8_append: more than 2^31 - 1 blocks");
+    return EMK_ERR_LIMIT;
+  }
+  kernel<<<(unsigned)(a.items * a.groups), threads, 0, s>>>(a);
+  EMK_LAUNCH_CHECK(h);
+  return EMK_OK;
+}
+template <int D, int TPU>
+int launch_append(emk_handle_t h, const AppendArgs& a, cudaStream_t s) {
+  constexpr int THREADS = TPU < 128 ? 128 : TPU;
+  return launch_units(h, kv8_append_kernel<D, TPU>, a, THREADS / TPU, THREADS, s);
+}
+
+template <int D>
+int launch_append_page(emk_handle_t h, const AppendArgs& a, cudaStream_t s) {
+  switch (((1 << a.page_shift) * D) / (8 * AP_PIECES)) {  // threads that hold a page's rows
+    case 16:
+    case 32: return launch_append<D, 32>(h, a, s);
+    case 64: return launch_append<D, 64>(h, a, s);
+    case 128: return launch_append<D, 128>(h, a, s);
+    case 256: return launch_append<D, 256>(h, a, s);
+    default: return launch_append<D, 512>(h, a, s);
+  }
 }
 
 }  // namespace
@@ -180,7 +303,7 @@ extern "C" int emk_kv8_append(emk_handle_t h, const void* k, const void* v, int6
                               int64_t num_pages, int64_t Hkv, int64_t page, int64_t D, emk_stream_t stream) {
   if (!h || !k || !v || !k_codes || !v_codes || !k_scale || !v_scale || !page_table || !ctx_lens || !cu_seqlens)
     return EMK_ERR_ARG;
-  if (B <= 0 || T <= 0 || max_pages <= 0 || num_pages <= 0 || Hkv <= 0 || Hkv > 65535 || B > 0x3fffffff ||
+  if (B <= 0 || T <= 0 || max_pages <= 0 || num_pages <= 0 || Hkv <= 0 || Hkv > 0x1fffffff || B > 0x1fffffff ||
       T > 0x7fffffff || max_pages > 0x7fffffff || num_pages > 0x7fffffff)
     return EMK_ERR_SHAPE;
   if ((D != 64 && D != 128) || !kv8_page_ok(page)) {
@@ -211,11 +334,9 @@ extern "C" int emk_kv8_append(emk_handle_t h, const void* k, const void* v, int6
   a.Hkv = (int)Hkv;
   a.page_shift = __builtin_ctzll((unsigned long long)page);
   a.status = h->status_dev;
-  // touched pages: every one holds a new token (<= T), and n tokens touch at most n / page + 2
-  const int64_t items = T < T / page + 2 * B ? T : T / page + 2 * B;
-  const dim3 grid((unsigned)items, (unsigned)Hkv, 2);
-  if (D == 128) kv8_append_kernel<128><<<grid, AP_THREADS, 0, (cudaStream_t)stream>>>(a);
-  else kv8_append_kernel<64><<<grid, AP_THREADS, 0, (cudaStream_t)stream>>>(a);
-  EMK_LAUNCH_CHECK(h);
-  return EMK_OK;
+  a.items = T / page + 2 * B;  // places: first_place(B)
+  cudaStream_t s = (cudaStream_t)stream;
+  if (T <= 4 * B)  // (a single long sequence among empty ones is slower this way, and right)
+    return D == 128 ? launch_units(h, kv8_append_few_kernel<128>, a, 4, 128, s) : launch_units(h, kv8_append_few_kernel<64>, a, 4, 128, s);
+  return D == 128 ? launch_append_page<128>(h, a, s) : launch_append_page<64>(h, a, s);
 }
