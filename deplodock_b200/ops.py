@@ -65,33 +65,42 @@ def _check_buffer(name: str, t: torch.Tensor | None, numel: int, dtype: torch.dt
 
 def _cuda_index(*tensors: torch.Tensor | None) -> int:
     """Index of the one CUDA device that all of ``tensors`` lie on."""
-    idx = -1
+    idx = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()  # -1: not on a CUDA device
+        if d == idx:
+            continue
+        if d < 0:
             if not torch.cuda.is_available():
                 raise RuntimeError("deplodock_b200 kernels need a CUDA device (sm_100a); there is no CPU fallback")
             raise ValueError("expected CUDA tensors")
-        if idx < 0:
-            idx = t.get_device()
-        elif t.get_device() != idx:
+        if idx is not None:
             raise ValueError("expected all tensors on one CUDA device")
+        idx = d
     return idx
 
 
 def _call_on(idx: int, name: str, *args) -> None:
-    """``emk_<name>`` on device ``idx`` (the tensors' own, current or not) and that device's current stream."""
-    h = handle(idx)
+    """``name`` of the library on device ``idx`` (the tensors' own, current or not) and that device's current stream."""
+    h = _handles.get(idx)
+    if h is None:
+        h = handle(idx)
     fn = getattr(h.lib, name)
-    stream = torch._C._cuda_getCurrentRawStream(idx)
-    if idx == torch.cuda.current_device():
-        rc = fn(h.ptr, *args, stream)
+    if idx == torch._C._cuda_getDevice():
+        rc = fn(h.ptr, *args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(h.ptr, *args, stream)
+            rc = fn(h.ptr, *args, torch._C._cuda_getCurrentRawStream(idx))
     if rc != cabi.EMK_OK:
         h.check(rc, name)
+
+
+def _check_contig(*tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            raise ValueError("expected contiguous tensors")
 
 
 _DTYPES = {torch.float32: cabi.EMK_F32, torch.bfloat16: cabi.EMK_BF16}
@@ -132,7 +141,7 @@ def rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     ``residual`` (in place). float32 or bfloat16, any row length. Returns ``(q, scale)`` or ``(q, scale, hidden)``;
     ``scale`` has the shape of ``x`` without its last axis."""
     idx = _cuda_index(x, weight, residual, out, scale_out, hidden_out)
-    _check_cuda_contig(x, weight, residual, out, scale_out, hidden_out)
+    _check_contig(x, weight, residual, out, scale_out, hidden_out)
     dtype = _dtype_token(x)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("x needs a last axis of one element at least")
@@ -528,7 +537,7 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     returns) times e4m3 weights ``[N, K]`` with one fp32 scale per output channel (those of :func:`linear_w8`), bf16 out.
     K must be a multiple of 16, N of 8."""
     idx = _cuda_index(x, x_scale, w, w_scale, out)
-    _check_cuda_contig(x, x_scale, w, w_scale, out)
+    _check_contig(x, x_scale, w, w_scale, out)
     if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
         raise TypeError("linear_e4m3 expects float8_e4m3fn activations and weights")
     if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
@@ -665,7 +674,7 @@ def kv8_append_(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: t
     and ``[B+1]``, left as they are: the caller advances its lengths). No two sequences may write to one page. Scales are
     powers of two and grow with what a page holds (see ``include/emk.h``)."""
     idx = _cuda_index(*cache, k, v, page_table, ctx_lens, cu_seqlens)
-    _check_cuda_contig(*cache, page_table, ctx_lens, cu_seqlens)
+    _check_contig(*cache, page_table, ctx_lens, cu_seqlens)
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, ctx_lens)
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise TypeError("kv8_append_ expects bfloat16 keys and values")
@@ -716,7 +725,7 @@ def sdpa_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, seq_len
     ``seq_lens[b] - Sq + i``; one that sees none (an empty or padding sequence) gets zeros. Returns bf16
     ``[B, Sq, Hq, D]``."""
     idx = _cuda_index(q, *cache, page_table, seq_lens, out, workspace)
-    _check_cuda_contig(*cache, page_table, seq_lens, out, workspace)
+    _check_contig(*cache, page_table, seq_lens, out, workspace)
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, seq_lens)
     if q.dtype != torch.bfloat16:
         raise TypeError("sdpa_kv8 expects bfloat16 queries")

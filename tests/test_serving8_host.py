@@ -126,6 +126,68 @@ def test_no_cpu_fallback():
         ops.kv8_append_(cache, q[0], q[0], table, lens, torch.zeros(2, dtype=torch.int32))
 
 
+class _On:
+    """Stands for a tensor on a device."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+@pytest.mark.parametrize("devices,want", [((0, 0), 0), ((3, None, 3), 3), ((-1, 0), ValueError), ((0, -1), ValueError), ((-1, -1), ValueError),
+                                          ((0, 1), ValueError), ((0, 0, 0, -1), ValueError)])
+def test_all_tensors_lie_on_one_device(monkeypatch, devices, want):
+    from deplodock_b200 import ops
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    tensors = [None if d is None else _On(d) for d in devices]
+    if want is ValueError:
+        with pytest.raises(ValueError):
+            ops._cuda_index(*tensors)
+    else:
+        assert ops._cuda_index(*tensors) == want
+
+
+def test_call_runs_on_the_tensors_device_and_its_stream(monkeypatch):
+    """The tensors' device need not be the current one; the stream is that device's."""
+    import contextlib
+
+    from deplodock_b200 import cabi, ops
+
+    seen, current = [], [0]
+
+    @contextlib.contextmanager
+    def device(idx):
+        before, current[0] = current[0], idx
+        yield
+        current[0] = before
+
+    class Lib:
+        @staticmethod
+        def emk_thing(*args):
+            seen.append((current[0], args))
+            return cabi.EMK_OK if args[1] == 7 else cabi.EMK_ERR_SHAPE
+
+    class Handle:
+        lib, ptr = Lib, "ptr"
+
+        @staticmethod
+        def check(rc, what):
+            raise ValueError(f"{what}: {rc}")
+
+    monkeypatch.setattr(ops, "_handles", {2: Handle, 0: Handle})
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda idx: 100 + idx, raising=False)
+    ops._call_on(2, "emk_thing", 7)
+    ops._call_on(0, "emk_thing", 7)
+    assert seen == [(2, ("ptr", 7, 102)), (0, ("ptr", 7, 100))] and current[0] == 0
+    with pytest.raises(ValueError, match="emk_thing"):
+        ops._call_on(0, "emk_thing", 8)
+
+
 def test_cache_shapes_are_checked():
     from deplodock_b200 import ops
 
