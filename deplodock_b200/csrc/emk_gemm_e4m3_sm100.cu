@@ -5,8 +5,8 @@
 //
 // Two kernels:
 //   gemm2_e4m3_kernel   many rows: CTA pairs on 256 x 256 tiles, persistent, two accumulators in tensor memory (the
-//                       structure of emk_gemm2_sm100.cu: producer / MMA / eight epilogue warps per CTA). Bound by the
-//                       tensor cores.
+//                       structure of emk_gemm2_sm100.cu: producer / MMA / sixteen epilogue warps per CTA). Bound by the
+//                       tensor cores at K = 2048, by them and the output's drain together at K = 1024.
 //   gemm_e4m3_rows_kernel   few rows: the operands change places, 128 rows of W are the instruction's M and 16 to 128
 //                       tokens its N, so that no tensor-core row is padding and the grid is cut along W. The K axis is
 //                       split over a cluster's CTAs, whose partial tiles meet in distributed shared memory (a fixed
@@ -48,7 +48,6 @@ struct Gemm8Args {
   const float* w_scale;
   int M, N;
   int tiles_m, tiles_n, kblocks;  // kblocks: 128-byte slices of K
-  int wide;                       // rows of y are 32-byte aligned
   int stages;                     // few-rows kernel: ring depth
   int* status;
   unsigned long long limit_ns;
@@ -72,25 +71,18 @@ struct __align__(8) P8Barriers {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int p8_smem(int bn) { return P8_STAGES * P8_KSUB * (P8_A_SUB + bn / 2 * BKB) + 1024 + (int)sizeof(P8Barriers); }
+constexpr int P8_OUT = 32 * 64;  // bytes of a warp's staging buffer: 32 rows of 32 columns
+constexpr int p8_smem(int bn) {
+  return P8_STAGES * P8_KSUB * (P8_A_SUB + bn / 2 * BKB) + 16 * P8_OUT + 1024 + (int)sizeof(P8Barriers);
+}
+static_assert(p8_smem(256) <= 227 * 1024, "shared memory of a CTA");
 
-// 16 accumulator columns [col0, col0 + 16) of output row `row`: one 32-byte sector per lane
-__device__ __forceinline__ void store16_e4m3(const Gemm8Args& g, const uint32_t* r, int row, int col0, float xs) {
-  if (row >= g.M || col0 >= g.N) return;
-  uint32_t o[8];
+// 16 accumulator columns of a row -> bf16, scaled; lane first + i of wl holds column i's scale
+__device__ __forceinline__ void scale16_e4m3(float wl, int first, const uint32_t* r, float xs, uint32_t* o) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col0 + q * 4 < g.N) s = __ldg(reinterpret_cast<const float4*>(g.w_scale + col0 + q * 4));  // N is a multiple of 8
-    o[2 * q] = pack_bf16x2(__uint_as_float(r[4 * q]) * xs * s.x, __uint_as_float(r[4 * q + 1]) * xs * s.y);
-    o[2 * q + 1] = pack_bf16x2(__uint_as_float(r[4 * q + 2]) * xs * s.z, __uint_as_float(r[4 * q + 3]) * xs * s.w);
-  }
-  __nv_bfloat16* out = g.y + (int64_t)row * g.N + col0;
-  if (g.wide) {  // rows of whole 32-byte sectors: N is a multiple of 16
-    st_global_v8(out, o);
-  } else {
-    *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
-    if (col0 + 8 < g.N) *reinterpret_cast<uint4*>(out + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+  for (int q = 0; q < 8; ++q) {
+    const float s0 = __shfl_sync(~0u, wl, first + 2 * q), s1 = __shfl_sync(~0u, wl, first + 2 * q + 1);
+    o[q] = pack_bf16x2(__uint_as_float(r[2 * q]) * xs * s0, __uint_as_float(r[2 * q + 1]) * xs * s1);
   }
 }
 
@@ -112,7 +104,8 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
   uint8_t* sB = smem + P8_STAGES * A_STAGE;
-  P8Barriers* bars = reinterpret_cast<P8Barriers*>(sB + P8_STAGES * B_STAGE);
+  uint8_t* sOut = sB + P8_STAGES * B_STAGE;
+  P8Barriers* bars = reinterpret_cast<P8Barriers*>(sOut + 16 * P8_OUT);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -227,8 +220,8 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
     }
   } else {
     // epilogue: a warp may only touch the tensor-memory lanes of its quarter (warp_id % 4); four warps share a quarter's
-    // rows and take a fourth of the columns each. Sixteen warps instead of eight: the drain of a K = 1024 tile lasts
-    // longer than its multiplication, and a warp spends it waiting (tensor-memory loads, scales, stores).
+    // rows and take a fourth of the columns each. The drain of a K = 1024 tile lasts longer than its multiplication, and a
+    // warp spends it waiting (tensor-memory loads, the turn through shared memory, stores).
     const int quarter = warp & 3, part = warp >> 2;
     int local = 0;
     for (int tile = pair; tile < ntiles; tile += npairs, ++local) {
@@ -239,20 +232,53 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
       const int row = tm * 2 * BM + (int)rank * BM + quarter * 32 + lane;
       const int n0 = tn * BN + part * (BN / 4);
       const float xs = row < g.M ? __ldg(g.x_scale + row) : 0.f;
+      float wl[(BN + 127) / 128];  // the columns' scales, one a lane
+#pragma unroll
+      for (int c = 0; c < (BN + 127) / 128; ++c) wl[c] = n0 + c * 32 + lane < g.N ? __ldg(g.w_scale + n0 + c * 32 + lane) : 0.f;
       if (!mbar_wait_warp(&bars->tmem_full[acc], acc_phase, wc, EMK_DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * ACC + part * (BN / 4));
-      uint32_t r[BN / 64][16];
+      // Lanes hold rows; what leaves is turned through shared memory, 32 columns at a time (16 last where a warp has 48), so
+      // that four lanes write 64 bytes of a row side by side. Stored as they are held (a sector per lane and row) and with
+      // each column's scale loaded by every lane, a 32768 x 4096 output of K = 1024 took 124 us instead of 116.
+      uint8_t* const buf = sOut + warp * P8_OUT;
+      constexpr int NC = BN / 64;
 #pragma unroll
-      for (int c = 0; c < BN / 64; ++c) tmem_ld_x16(taddr + (uint32_t)(c * 16), r[c]);
-      tmem_ld_wait();
+      for (int c = 0; c < NC; c += 2) {
+        const int n = c + 1 < NC ? 2 : 1;  // 16-column chunks of this turn
+        uint32_t r[2][16];
+        tmem_ld_x16(taddr + (uint32_t)(c * 16), r[0]);
+        if (n == 2) tmem_ld_x16(taddr + (uint32_t)(c * 16 + 16), r[1]);
+        tmem_ld_wait();
+        tie_regs16(r[0]);
+        if (n == 2) tie_regs16(r[1]);
+        if (c + 2 >= NC) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&bars->tmem_empty[acc]), 0));
+        }
+        __syncwarp();  // the buffer's last contents have been read
 #pragma unroll
-      for (int c = 0; c < BN / 64; ++c) tie_regs16(r[c]);
+        for (int u = 0; u < n; ++u) {
+          uint32_t o[8];
+          scale16_e4m3(wl[c / 2], u * 16, r[u], xs, o);
 #pragma unroll
-      for (int c = 0; c < BN / 64; ++c) store16_e4m3(g, r[c], row, n0 + c * 16, xs);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&bars->tmem_empty[acc]), 0));
+          for (int v = 0; v < 2; ++v)  // 16-byte piece 2 u + v of row `lane`, swizzled by the row pair
+            *reinterpret_cast<uint4*>(buf + lane * 64 + (((2 * u + v) ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        }
+        __syncwarp();
+        const int piece = lane & 3;
+        const int col = n0 + c * 16 + piece * 8;
+        const bool in = piece < 2 * n && col < g.N;  // N is a multiple of 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = i * 8 + (lane >> 2);
+          const int64_t m = (int64_t)row - lane + rr;
+          if (in && m < g.M)
+            *reinterpret_cast<uint4*>(g.y + m * g.N + col) = *reinterpret_cast<const uint4*>(buf + rr * 64 + ((piece ^ ((rr >> 1) & 3)) << 4));
+        }
+      }
     }
   }
 
@@ -528,10 +554,11 @@ int linear_pairs(emk_handle_t h, const void* x, const void* w, const Gemm8Args& 
   const int rc = emk_make_tmap_2d(h, &ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)K, (uint64_t)g.M, (uint64_t)K, BKB,
                                   BM, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != EMK_OK) return rc;
-  // Rounds of tiles over the machine's pairs, times what a round costs at the tile's width: at K = 2048 a 256-column
-  // tile takes 6.4 us, a 192-column one 5.7, a 128-column one 4.4 (operand traffic per multiplication grows as the tile
-  // narrows), so narrow tiles pay only where they save rounds. Measured at 1024 x 6144 x 2048: 17.5 / 15.8 / 17.8 us;
-  // 256 x 4096 x 1024: 8.0 / 6.7 / 5.9; 4096 x 6144 x 2048: 42.4 / 43.8 / 52.7.
+  // Rounds of tiles over the machine's pairs, times what a round costs at the tile's width: with every pair busy a round of
+  // 256-, 192- or 128-column tiles takes 7.3 / 6.0 / 4.8 us at K = 2048 and 3.8 / 3.2 / 2.5 at K = 1024 (operand traffic
+  // per multiplication grows as the tile narrows), so narrow tiles pay only where they save rounds; the weights stand a
+  // little above those ratios because near a tie the wide tile is the faster. Measured at 1024 x 6144 x 2048:
+  // 17.0 / 15.7 / 17.9 us; 256 x 4096 x 1024: 7.7 / 6.5 / 5.7; 4096 x 6144 x 2048: 42.6 / 44.5 / 53.8.
   const int64_t pairs = h->sm_count / 2, tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
   const auto cost = [&](int64_t bn, int64_t weight) { return (tiles_m * ((g.N + bn - 1) / bn) + pairs - 1) / pairs * weight; };
   const int64_t c256 = cost(256, 100), c192 = cost(192, 88), c128 = cost(128, 69);
@@ -571,7 +598,6 @@ extern "C" int emk_linear_e4m3(emk_handle_t h, const void* x, const float* x_sca
   g.M = (int)M;
   g.N = (int)N;
   g.kblocks = (int)((K + BKB - 1) / BKB);
-  g.wide = ((N % 16) == 0 && ((uintptr_t)y & 31u) == 0) ? 1 : 0;
   g.status = h->status_dev;
   g.limit_ns = h->wait_limit_ns;
   return few_rows(M, N, K) ? linear_rows(h, x, w, g, K, (cudaStream_t)stream) : linear_pairs(h, x, w, g, K, (cudaStream_t)stream);
