@@ -25,7 +25,8 @@
 // contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
 //
 // Two kernels share the loop. Where no sequence can be long (split_of), a cluster of CTAs takes a row tile, deals its tiles
-// to its warps and joins their pieces in distributed shared memory: one launch. Otherwise:
+// to its warps and joins their pieces in distributed shared memory: one launch. The CTAs of the longest sequences come first.
+// Otherwise:
 // Work split: the tiles of 16 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
 // warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths. Beginning a row costs a
 // warp about as much as a tile (the queries, a pipeline to fill, an output), so a row counts ROW_COST tiles more than it
@@ -66,6 +67,7 @@ struct SdpaArgs {
   float2* ml;    // [ranges][2][row_cap]: maximum, sum
   float* part;   // [ranges][2][row_cap][D]
   int max_ranges;
+  int ranked;    // rows kernel: the longest sequences first
   int* status;
   unsigned long long limit_ns;
 };
@@ -399,7 +401,6 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
 #pragma unroll
       for (int u = 0; u < 2; ++u) pb[n][u] = transpose8x8(pack_f16x2(p[n][2 * u], p[n][2 * u + 1]));
     }
-    if (vs_raw == 0.f) continue;  // a page of zeros: it counts in the sum and adds nothing (uniform over the warp)
     // ---- o^T += V^T P^T ----
     uint32_t w[4][L::V_BYTES / 4];
 #pragma unroll
@@ -417,10 +418,12 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
         w[u][1] = v.y;
       }
     }
-    if ((ta + i) * SK_TILE + SK_TILE > len) {  // the sequence's last tile: what lies behind its end counts as zeros
+    // What lies behind the sequence's end counts as zeros, and so does a page whose scale is zero: its tokens count in the sum and
+    // add nothing.
+    if ((ta + i) * SK_TILE + SK_TILE > len || vs_raw == 0.f) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len;
+        const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len && vs_raw != 0.f;
 #pragma unroll
         for (int j = 0; j < L::V_BYTES / 4; ++j) w[u][j] = in ? w[u][j] : 0u;
       }
@@ -666,6 +669,64 @@ __device__ __forceinline__ void ld_cluster_vec(uint32_t addr, float* v) {
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
 }
 
+// The sequence that comes at place `rank` when the longest come first: by buckets of a quarter octave of their tiles, those of
+// a bucket in their own order. All threads of the block, B <= RANKED; the length comes back too.
+constexpr int RANKED = 256;
+__device__ __forceinline__ int sequence_of_rank(const SdpaArgs& a, int rank, int& len) {
+  __shared__ int s_count[SK_THREADS], s_warp[SK_WARPS], s_pick[2];
+  __shared__ int s_len[RANKED];
+  __shared__ uint8_t s_bucket[RANKED];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  s_count[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int b = tid; b < RANKED; b += SK_THREADS) {
+    int bucket = 0xff;  // none's
+    if (b < a.B) {
+      const int n = seq_len(a, b);
+      const uint32_t x = (uint32_t)seq_tiles(n) << 2;  // tiles are below 2^28
+      const int e = 31 - __clz(x | 4u);                // their exponent + 2
+      bucket = x == 0 ? SK_THREADS - 1 : SK_THREADS - 2 - (((e - 2) << 2) + (int)((x >> (e - 2)) & 3u));  // 0: the longest
+      s_len[b] = n;
+      atomicAdd(&s_count[bucket], 1);
+    }
+    s_bucket[b] = (uint8_t)bucket;
+  }
+  __syncthreads();
+  const int mine = s_count[tid];
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) s_warp[warp] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < SK_WARPS - 1; ++w) upto += w < warp ? s_warp[w] : 0;
+  if (rank < upto && rank >= upto - mine) {
+    s_pick[0] = tid;
+    s_pick[1] = rank - (upto - mine);
+  }
+  __syncthreads();
+  const int bucket = s_pick[0];
+  int left = s_pick[1];
+#pragma unroll
+  for (int b0 = 0; b0 < RANKED; b0 += 32) {
+    const bool hit = s_bucket[b0 + lane] == bucket;
+    const unsigned in = __ballot_sync(0xffffffffu, hit);
+    const int n = __popc(in);
+    if (left < n) {
+      const unsigned here = __ballot_sync(0xffffffffu, hit && __popc(in & ((1u << lane) - 1)) == left);
+      const int b = b0 + __ffs(here) - 1;
+      len = s_len[b];
+      return b;
+    }
+    left -= n;
+  }
+  return 0;  // not reached: rank < B
+}
+
 // Short sequences: a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose pieces meet in distributed
 // shared memory. No list to cut, no workspace, no second kernel: what is left of a call is one launch and one row's latency.
 template <int D, int RT>
@@ -691,13 +752,19 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
   __syncthreads();
   const int heads = a.Hkv * a.row_tiles;
   const int row_id = blockIdx.x / split;
-  const int b = row_id / heads, hr = row_id - b * heads;
+  int b = row_id / heads;
+  const int hr = row_id - b * heads;
   const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
   const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
   const int pieces = split * SK_WARPS, piece = rank * SK_WARPS + warp;
   grid_dependency_wait();
   const WaitCtx wc{&s_abort, a.status, a.limit_ns};
-  const int len = seq_len(a, b), tiles = seq_tiles(len);
+  int len;
+  if (a.ranked)
+    b = sequence_of_rank(a, b, len);
+  else
+    len = seq_len(a, b);
+  const int tiles = seq_tiles(len);
   const int ta = (int)((int64_t)tiles * piece / pieces), tb = (int)((int64_t)tiles * (piece + 1) / pieces);
   if (lane < ROWS) {
     s_m[warp][lane] = -INFINITY;
@@ -892,28 +959,39 @@ bool sizes_ok(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv) {
 struct SkPlan {
   int row_tiles, tile_rows, row_cap;
   int split;  // CTAs per row tile of the rows kernel; 0: the list kernel and its join
+  int ranked;
   int64_t ctas, info_bytes, ml_bytes, part_bytes;
 };
 
 // CTAs per row tile for the rows kernel, or 0 where the list kernel is to run. The host knows the longest a sequence can be
 // (max_tokens), not the lengths. The rows kernel has no list to cut and nothing to join, and wins wherever its CTAs finish
 // about together (8 heads, one sequence of 1500 tokens: 7.3 us against 9.8; 64 sequences of 128: 6.9 / 12.9; of 1024: 26.2 /
-// 35.3; of 4096: 87.2 / 98.5); a sequence much longer than the others it drags through a few warps. So: as many CTAs per row as
-// fill the machine, or twice that, such that the longest possible sequence takes a row's warps (about 1 us a tile and warp)
-// 32 us at most, or 0.4 of the time in which the machine reads half of all that the tables could hold, 64 us at most
-// (64 sequences of 0..8192 tokens: 109.9 us in pairs, 115.2 alone, 102.9 as a list; 128 of 0..4096: 100.1 / 108.7 / 108.6).
-int split_of(int64_t rows, int64_t max_tokens, int64_t D, int64_t slots) {
+// 35.4; of 4096: 88.2 / 98.3; 64 of 0..8192 tokens: 91.6 / 102.5; 128 of 0..4096: 87.0 / 108.9); a sequence much longer than
+// the others it drags through a few warps, 0.7 us a tile at least. So: as many CTAs per row as fill the machine, or twice
+// that, such that a row's warps take `limit` tiles each at most of the longest possible sequence:
+//   32 (16 rows to a tile, where a tile takes longer: 24 if twice as many CTAs allow it; 17 x 4 tokens of up to 4097: 23.7 us
+//   against 28.8), or as many as the machine reads in 0.75 us of the time that half of all the tables could hold takes, to 64;
+//   10 where even 8 CTAs per row leave half of the machine idle (one sequence of 4096: 10.4 us against about 11, of 8192: 15.1 /
+//   12.8, of 16384: 24.6 / 15.9).
+// More CTAs than that cost their start (about 6 us of a slot each) and are taken where that is small beside the reading (64 of
+// 0..16384: 163 us in fours, 180 as a list).
+int split_of(int64_t rows, int64_t max_tokens, int64_t D, int64_t slots, bool small_tile) {
   int fill = 1;
   while (fill < 8 && rows * fill * 2 <= slots) fill *= 2;
   const double all = (double)rows * (double)max_tokens * (double)D / 6.2e6;  // us: half of 2 D bytes a token and row
-  const double limit = all * 0.4 > 64. ? 64. : all * 0.4 > 32. ? all * 0.4 : 32.;
   const int64_t tiles = (max_tokens + SK_TILE - 1) / SK_TILE;
-  for (int split = fill; split <= 8 && split <= 2 * fill; split *= 2) {
-    if ((double)tiles / (split * SK_WARPS) > limit) continue;
-    while (split > 1 && tiles < split * 8) split /= 2;  // no CTA with less than two tiles a warp
-    return rows * split <= 0x7fffffff ? split : 0;
+  const bool idle = rows * 16 <= slots;
+  const double lo = idle ? 10. : small_tile ? 32. : 24.;
+  const double limit = idle || all * 0.75 < lo ? lo : all * 0.75 < 64. ? all * 0.75 : 64.;
+  int split = 0;
+  for (int n = fill; n <= 8; n *= 2) {
+    if (n > 2 * fill && (double)(rows * n) * 24. > all * (double)slots) break;
+    const double each = (double)tiles / (n * SK_WARPS);
+    if (each <= limit || (!idle && each <= 32.)) split = n;
+    if (each <= limit) break;
   }
-  return 0;
+  while (split > 1 && tiles < split * 8) split /= 2;  // no CTA with less than two tiles a warp
+  return rows * split <= 0x7fffffff ? split : 0;
 }
 
 // The grid never has more warps than the longest possible list has units.
@@ -925,7 +1003,11 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   const int64_t units = (max_tokens + SK_TILE - 1) / SK_TILE + ROW_COST;  // below 2^28
   const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
   const int64_t slots = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
-  p.split = split_of(rows, max_tokens, D, slots);
+  p.split = split_of(rows, max_tokens, D, slots, p.tile_rows == 8);
+  // Longest first pays where a CTA may have more than a few tiles a warp and several CTAs share an SM or wait for one (64
+  // sequences of 0..8192 tokens in pairs: 91.6 us against 109.9; 128 of 0..4096: 87.0 / 108.4) and costs 0.8 us a CTA (256
+  // sequences of 128: 28.5 us against 25.6).
+  p.ranked = B > 1 && B <= RANKED && rows * p.split > sm_count && units > (int64_t)p.split * SK_WARPS * 8 ? 1 : 0;
   p.ctas = slots;
   if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
   if (p.ctas < 1) p.ctas = 1;
@@ -1068,6 +1150,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   a.ml = (float2*)(ws + p.info_bytes);
   a.part = (float*)(ws + p.info_bytes + p.ml_bytes);
   a.max_ranges = (int)(p.ctas * SK_WARPS);
+  a.ranked = p.ranked;
   a.status = h->status_dev;
   a.limit_ns = h->wait_limit_ns;
   cudaStream_t s = (cudaStream_t)stream;

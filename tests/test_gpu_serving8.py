@@ -443,6 +443,30 @@ def test_sdpa_kv8_many_sequences(ops, room):
     _attend_case(ops, 1, 9, 1, 128, 16, [17] * 700, seed=5, room=room)
 
 
+def _mixed_lengths(B, longest):
+    g = _gen(B)
+    lens = (torch.rand(B, generator=g) ** 2 * (longest + 1)).long().clamp(max=longest).tolist()
+    lens[:6] = [0, longest, 1, longest, 0, 16]
+    return lens
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,Sq", [(150, 4, 2, 128, 1), (256, 2, 1, 64, 1), (257, 2, 1, 128, 1), (150, 8, 2, 64, 3), (150, 8, 2, 128, 3)])
+@pytest.mark.parametrize("kind", ["mixed", "equal", "one"])
+def test_sdpa_kv8_more_rows_than_the_machine_takes_at_once(ops, B, Hq, Hkv, D, Sq, kind):
+    """Up to 256 sequences are taken longest first: every one of them exactly once, whatever their lengths."""
+    longest = 1300
+    lens = {"mixed": _mixed_lengths(B, longest), "equal": [longest] * B, "one": [0] * (B - 1) + [longest]}[kind]
+    got, q, cache, table, lens_t = _attend_case(ops, Sq, Hq, Hkv, D, 64, lens, seed=B + D, check=kind == "mixed" and Sq == 1)
+    # every sequence by itself: other kernels' sums in another order, so a rounding of the output apart
+    for b in {0, 1, B // 2, B - 2, B - 1}:
+        alone = ops.sdpa_kv8(q[b:b + 1], cache, table[b:b + 1], lens_t[b:b + 1])
+        assert torch.isfinite(alone).all()
+        # both lie within 2^-9 of the value (half a step) and twice 2^-11 of the probabilities' mass, which the values' largest bounds
+        vmax = float((cache.v[table[b].long()].float().nan_to_num().abs().amax((1, 2, 3)) * cache.v_scale[table[b].long()].amax(1).nan_to_num()).max())
+        tol = got[b].float().abs() * 2.0 ** -7 + 2.0 ** -9 * vmax
+        assert ((got[b].float() - alone[0].float()).abs() <= tol).all(), b
+
+
 @pytest.mark.parametrize("q_scale,sigma_exp", [(30.0, (-2, 3)), (1.0, (-58, -40)), (1e-25, (60, 110)), (1.0, (-20, 4)), (0.0, (-2, 3))])
 @pytest.mark.parametrize("room", ROOM)
 def test_sdpa_kv8_extreme_scales(ops, q_scale, sigma_exp, room):
