@@ -12,7 +12,8 @@
 // any offset go through the same packs, taken at the aligned places of the whole array with the row's ends masked.
 // Measured at 32768 x 1024 bf16 with a residual (235 MB): two reductions and loads behind stores 55.8 us, loads first 45.1,
 // this form 39.9 (0.90 of the copy bandwidth); 32768 x 1001 (their weights still go element by element): 83.7 us element by
-// element, 49.0 in packs.
+// element, 49.0 in packs; the same in fp32 without a residual: 50.6 us, 45.0 with four CTAs per SM (a few registers spilled)
+// and the odd elements' weights loaded with them.
 #include "emk_common.cuh"
 
 #include <cuda_fp8.h>
@@ -118,7 +119,7 @@ struct Raw<__nv_bfloat16> {
 // pack (fewer than V each) go to one thread each. RES: with a residual (a kernel of its own: without one a row needs half
 // the registers, and twice the rows fit an SM).
 template <typename T, int NV, int TPR, bool RAGGED, bool RES>
-__global__ void __launch_bounds__(256, RAGGED ? (NV == 4 && !RES ? 3 : 2) : NV == 8 ? (RES ? 2 : 3) : NV == 4 ? (RES ? 3 : 4) : 5)
+__global__ void __launch_bounds__(256, RAGGED ? (RES || NV == 8 ? 2 : 4) : NV == 8 ? (RES ? 2 : 3) : NV == 4 ? (RES ? 3 : 4) : 5)
 rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint8_t* __restrict__ q, float* __restrict__ scale,
                     T* hidden, int64_t rows, int cols, float eps) {
   constexpr int V = Raw<T>::V;
@@ -156,7 +157,7 @@ rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint
       }
     }
     // this thread's odd elements: column tid of the head, column tid of the tail
-    float odd[2] = {0.f, 0.f};
+    float odd[2] = {0.f, 0.f}, odd_w[2] = {0.f, 0.f};
     int odd_col[2] = {-1, -1};
     if (RAGGED && row < rows) {
       if (tid < head) odd_col[0] = tid;
@@ -165,6 +166,7 @@ rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint
       for (int j = 0; j < 2; ++j) {
         if (odd_col[j] >= 0) {
           odd[j] = to_f<T>(x[base + odd_col[j]]);
+          odd_w[j] = to_f<T>(__ldg(w + odd_col[j]));
           if (RES) odd[j] = to_f<T>(from_f<T>(odd[j] + to_f<T>(residual[base + odd_col[j]])));
         }
       }
@@ -207,7 +209,7 @@ rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint
         if (odd_col[j] >= 0) {
           if (RES) hidden[base + odd_col[j]] = from_f<T>(odd[j]);
           ss = fmaf(odd[j], odd[j], ss);
-          odd[j] *= to_f<T>(__ldg(w + odd_col[j]));
+          odd[j] *= odd_w[j];
           amax = max_nan(amax, fabsf(odd[j]));
         }
       }
