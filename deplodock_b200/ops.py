@@ -722,8 +722,8 @@ def sdpa_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, seq_len
     (``emk_sdpa_kv8``): the single-token step (``Sq = 1``) and a few draft tokens. ``q``: bf16 ``[B, Sq, Hq, D]``, heads
     contiguous, any token pitch that is a multiple of 8 elements; ``seq_lens``: int32 CUDA tensor ``[B]``, the cached
     tokens of each sequence with the ``Sq`` new ones already appended. Query ``i`` sees the tokens up to position
-    ``seq_lens[b] - Sq + i``; one that sees none (an empty or padding sequence) gets zeros. Returns bf16
-    ``[B, Sq, Hq, D]``."""
+    ``seq_lens[b] - Sq + i``; one that sees none (an empty or padding sequence) gets zeros. Sequences may share pages;
+    ``out`` may be a contiguous ``q`` itself. Returns bf16 ``[B, Sq, Hq, D]``."""
     idx = _cuda_index(q, *cache, page_table, seq_lens, out, workspace)
     _check_contig(*cache, page_table, seq_lens, out, workspace)
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, seq_lens)

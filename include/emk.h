@@ -112,10 +112,11 @@ int emk_softmax_lastdim(emk_handle_t h, const void* x, void* y, int64_t rows, in
 /* RMSNorm with the residual's addition and an e4m3 output with one scale per row, for the 8-bit linear layers:
  *   f = x, or with a residual f = round(x + residual) to `dtype`, stored to hidden (the new residual stream);
  *   y = f * rsqrt(mean(f^2) + eps) * w in fp32;  scale[row] = max(max |y|, 2^-100) / 448;  q = e4m3(y / scale[row]).
- * A row with a NaN or an infinity (or a product f * w past fp32's range) becomes NaN codes with a NaN scale. x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or
- * EMK_BF16), residual and hidden both given or both NULL; hidden may be x or residual itself (in place), q may alias
- * nothing. w: [cols] of `dtype`; q: [rows, cols] e4m3; scale: fp32 [rows]. Any cols; pointers that are 16-byte aligned (q
- * 8-byte) take the vector path. No counterpart in the reference (no 8-bit path). */
+ * A row with a NaN or an infinity (or a product f * w past fp32's range) becomes NaN codes with a NaN scale.
+ * x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or EMK_BF16), residual and hidden both given or both NULL;
+ * hidden may be x or residual itself (in place), q may alias nothing. w: [cols] of `dtype`; q: [rows, cols] e4m3;
+ * scale: fp32 [rows]. Any cols; pointers that are 16-byte aligned (q 8-byte) take the vector path. No counterpart in
+ * the reference (no 8-bit path). */
 int emk_rmsnorm_e4m3(emk_handle_t h, const void* x, const void* residual, const void* w, void* q, float* scale,
                      void* hidden, int64_t rows, int64_t cols, float eps, int dtype, emk_stream_t stream);
 
@@ -289,9 +290,10 @@ int emk_sdpa_causal_gqa_bf16_varlen(emk_handle_t h, const void* q, const void* k
  * emk_sdpa_kv8: o = softmax(scale * q K^T) V over the seq_lens[b] cached tokens of every sequence (int32 [B] on the
  * device, the Sq queries' own tokens included, already appended); query i sits at position seq_lens[b] - Sq + i and
  * sees the tokens up to itself; a query that sees none gets zeros. q: bf16, row (b * Sq + i) of pitch ld_q elements,
- * head h at column h * D; o: bf16 [B * Sq][Hq * D]; Hq a multiple of Hkv. Whatever lies in a page behind a sequence's
- * last token is not used; scales must not be negative, and a zero value scale makes a page's values zero. Lengths are clamped to what max_pages pages hold, page ids to
- * the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
+ * head h at column h * D; o: bf16 [B * Sq][Hq * D], which may be q itself where ld_q is Hq * D; Hq a multiple of Hkv.
+ * Sequences may share pages. Whatever lies in a page behind a sequence's last token is not used; scales must not be
+ * negative, and a zero value scale makes a page's values zero. Lengths are clamped to what max_pages pages hold, page
+ * ids to the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
  * emk_sdpa_kv8_workspace_bytes(h, B, Sq, Hq, Hkv, max_pages * page, D) bytes (0, and NULL, where no sequence can be long),
  * not used between calls; calls that may overlap need one each. The first call for a head dimension and up to / over 8
  * queries x heads a KV head on a device sets the kernels' shared-memory attributes: make it before any stream capture. */
