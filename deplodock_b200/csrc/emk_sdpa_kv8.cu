@@ -24,9 +24,9 @@
 // log2(v_scale) and p * v_scale / max is what is rounded to f16 (2^-12 relative: p in [0, 2^15], so 2^-29 of the largest
 // contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
 //
-// Two kernels share the loop. Where no sequence can be long (split_of), a cluster of CTAs takes a row tile, deals its tiles
-// to its warps and joins their pieces in distributed shared memory: one launch. The CTAs of the longest sequences come first.
-// Otherwise:
+// Three kernels share the loop. Where no sequence can be long (split_of), a cluster of CTAs takes a row tile, deals its tiles
+// to its warps and joins their pieces in distributed shared memory: one launch. The CTAs of the longest sequences come first;
+// where rows are few, CTAs are as large as an SM (wide_split_of). Otherwise:
 // Work split: the tiles of 16 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
 // warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths. Beginning a row costs a
 // warp about as much as a tile (the queries, a pipeline to fill, an output), so a row counts ROW_COST tiles more than it
@@ -157,6 +157,14 @@ struct SkLayout {
   static constexpr int SMEM = RING + 1024;                // the swizzle wants 1024-byte aligned slots
   static constexpr int PIECE_PITCH = D + 4;              // floats; spreads the rows over the banks
   static_assert(ROWS * PIECE_PITCH * 4 <= WARP_RING, "a warp's last piece lies over its ring");
+};
+
+// The wide kernel: one CTA per SM, of as many warps as its registers hold.
+template <int D, int RT>
+struct WideLayout {
+  static constexpr int WARPS = RT == 1 ? 16 : 8;  // (of either head dimension)
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int SMEM = WARPS * SkLayout<D, RT>::WARP_RING + 1024;
 };
 
 // Ring position of a warp: slots that are filled and used next (equal between two parts), phase of the latter's barrier.
@@ -651,6 +659,35 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
   }
 }
 
+// A warp's piece of a row tile: the outputs over its ring, the maxima and sums to m and l.
+template <int D, int RT>
+__device__ __forceinline__ void leave_piece(const Part<D, RT>& part, uint8_t* ring, float* m, float* l) {
+  using L = SkLayout<D, RT>;
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  __syncwarp();  // every lane is done with the ring
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sum = part.l[n][e];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      const int row = n * 8 + 2 * t + e;
+      if (g == 0) {
+        m[row] = part.m[n][e];
+        l[row] = sum;
+      }
+      float* out = reinterpret_cast<float*>(ring) + row * L::PIECE_PITCH + g * (D / 8);
+#pragma unroll
+      for (int j = 0; j < D / 16; j += 2)
+        *reinterpret_cast<float4*>(out + 2 * j) =
+            make_float4(part.o[n][j][e], part.o[n][j][2 + e], part.o[n][j + 1][e], part.o[n][j + 1][2 + e]);
+    }
+  }
+}
+
 __device__ __forceinline__ uint32_t cluster_size_x() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
@@ -727,7 +764,7 @@ __device__ __forceinline__ int sequence_of_rank(const SdpaArgs& a, int rank, int
   return 0;  // not reached: rank < B
 }
 
-// Short sequences: a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose pieces meet in distributed
+// Many rows, or short ones (split_of): a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose pieces meet in distributed
 // shared memory. No list to cut, no workspace, no second kernel: what is left of a call is one launch and one row's latency.
 template <int D, int RT>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM)
@@ -775,29 +812,8 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     uint8_t* ring = smem + warp * L::WARP_RING;
     RingAt at{0, 0, 0};
     Part<D, RT> part;
-    if (row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part)) {
-      __syncwarp();  // every lane is done with the ring, which now takes the piece
-#pragma unroll
-      for (int n = 0; n < RT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float sum = part.l[n][e];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          const int row = n * 8 + 2 * t + e;
-          if (g == 0) {
-            s_m[warp][row] = part.m[n][e];
-            s_l[warp][row] = sum;
-          }
-          float* out = reinterpret_cast<float*>(ring) + row * L::PIECE_PITCH + g * (D / 8);
-#pragma unroll
-          for (int j = 0; j < D / 16; j += 2)
-            *reinterpret_cast<float4*>(out + 2 * j) =
-                make_float4(part.o[n][j][e], part.o[n][j][2 + e], part.o[n][j + 1][e], part.o[n][j + 1][2 + e]);
-        }
-      }
-    }
+    if (row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part))
+      leave_piece<D, RT>(part, ring, s_m[warp], s_l[warp]);
   }
   grid_launch_dependents();
   __syncthreads();
@@ -838,6 +854,126 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
       *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
   }
   if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
+}
+
+// Few rows of a certain length (wide_split_of): the same with one CTA of as many warps as an SM holds, so that a row gets four times (16 rows: twice) the warps
+// out of a cluster. A CTA's pieces meet in its own shared memory before the cluster's do.
+template <int D, int RT>
+__global__ void __launch_bounds__(WideLayout<D, RT>::THREADS, 1)
+sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
+  using L = SkLayout<D, RT>;
+  constexpr int ROWS = L::ROWS, E = D / 32, WARPS = WideLayout<D, RT>::WARPS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t s_full[WARPS][L::STAGES];
+  __shared__ int s_abort;
+  __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
+  __shared__ float s_cm[ROWS], s_cl[ROWS];                 // the CTA's piece
+  __shared__ __align__(16) float s_o[ROWS][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = (int)cluster_size_x(), rank = (int)cluster_ctarank();
+  if (lane == 0) {
+    for (int i = 0; i < L::STAGES; ++i) mbar_init(&s_full[warp][i], 1);
+    if (warp == 0) {
+      s_abort = 0;
+      tma_prefetch_desc(&tma_k);
+      tma_prefetch_desc(&tma_v);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  const int heads = a.Hkv * a.row_tiles;
+  const int row_id = blockIdx.x / split;
+  const int b = row_id / heads, hr = row_id - b * heads;
+  const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
+  const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
+  const int pieces = split * WARPS, piece = rank * WARPS + warp;
+  grid_dependency_wait();
+  const WaitCtx wc{&s_abort, a.status, a.limit_ns};
+  const int len = seq_len(a, b), tiles = seq_tiles(len);
+  const int ta = (int)((int64_t)tiles * piece / pieces), tb = (int)((int64_t)tiles * (piece + 1) / pieces);
+  if (lane < ROWS) {
+    s_m[warp][lane] = -INFINITY;
+    s_l[warp][lane] = 0.f;
+  }
+  __syncwarp();
+  if (tb > ta) {
+    uint8_t* ring = smem + warp * L::WARP_RING;
+    RingAt at{0, 0, 0};
+    Part<D, RT> part;
+    if (row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part))
+      leave_piece<D, RT>(part, ring, s_m[warp], s_l[warp]);
+  }
+  grid_launch_dependents();
+  __syncthreads();
+  if (s_abort) abort_drain();
+  const auto store = [&](int row, const float* acc, float sum) {
+    const int rr = rt * ROWS + row;
+    const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // nothing visible: zeros
+    __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + lane * E;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  };
+  // a warp joins a row: lane i looks after piece i, then the lanes share the channels
+  for (int row = warp; row < rows; row += WARPS) {
+    const float m = lane < WARPS ? s_m[lane][row] : -INFINITY, l = lane < WARPS ? s_l[lane][row] : 0.f;
+    const unsigned holds = __ballot_sync(0xffffffffu, m != -INFINITY || l != 0.f);  // (a NaN sum counts)
+    const float top = warp_max(m);
+    const float f = m == -INFINITY ? 1.f : ex2(m - top);
+    const float sum = warp_sum(l * f);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if ((holds >> i) & 1u) {
+        const float* from = reinterpret_cast<const float*>(smem + i * L::WARP_RING) + row * L::PIECE_PITCH + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(from[e], fi, acc[e]);
+      }
+    }
+    if (split == 1) {
+      store(row, acc, sum);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s_o[row][lane * E + e] = acc[e];
+      if (lane == 0) {
+        s_cm[row] = top;
+        s_cl[row] = sum;
+      }
+    }
+  }
+  if (split == 1) return;  // (uniform over the grid)
+  cluster_sync_all();      // (reached by every thread of every CTA, whatever happened above)
+  for (int row = rank + split * warp; row < rows; row += split * WARPS) {
+    float m = -INFINITY, l = 0.f;
+    if (lane < split) {
+      m = ld_cluster(mapa_u32(smem_u32(&s_cm[row]), (uint32_t)lane));
+      l = ld_cluster(mapa_u32(smem_u32(&s_cl[row]), (uint32_t)lane));
+    }
+    const float top = warp_max(m);
+    const float f = m == -INFINITY ? (l != 0.f ? 1.f : 0.f) : ex2(m - top);
+    const float sum = warp_sum(l * f);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if (i < split) {
+        float v[E];
+        ld_cluster_vec<E>(mapa_u32(smem_u32(&s_o[row][lane * E]), (uint32_t)i), v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], fi, acc[e]);
+      }
+    }
+    store(row, acc, sum);
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
 // Joins the pieces of every row that was cut: block (row of tiles, row of the tile). The places of a row's pieces are
@@ -958,21 +1094,22 @@ bool sizes_ok(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv) {
 
 struct SkPlan {
   int row_tiles, tile_rows, row_cap;
-  int split;  // CTAs per row tile of the rows kernel; 0: the list kernel and its join
-  int ranked;
+  int split;   // CTAs per row tile of the wide or the rows kernel; 0: the list kernel and its join
+  bool wide;
+  int ranked;  // rows kernel: the longest sequences first
   int64_t ctas, info_bytes, ml_bytes, part_bytes;
 };
 
 // CTAs per row tile for the rows kernel, or 0 where the list kernel is to run. The host knows the longest a sequence can be
 // (max_tokens), not the lengths. The rows kernel has no list to cut and nothing to join, and wins wherever its CTAs finish
-// about together (8 heads, one sequence of 1500 tokens: 7.3 us against 9.8; 64 sequences of 128: 6.9 / 12.9; of 1024: 26.2 /
-// 35.4; of 4096: 88.2 / 98.3; 64 of 0..8192 tokens: 91.6 / 102.5; 128 of 0..4096: 87.0 / 108.9); a sequence much longer than
-// the others it drags through a few warps, 0.7 us a tile at least. So: as many CTAs per row as fill the machine, or twice
+// about together (8 heads, 64 sequences of 128 tokens: 6.9 us against 12.9; of 1024: 26.2 / 35.4; of 4096: 88.2 / 98.3; of
+// 0..8192: 91.6 / 102.5; 128 of 0..4096: 87.0 / 108.9); a sequence much longer than the others it drags through a few
+// warps, 0.7 us a tile at least. So: as many CTAs per row as fill the machine, or twice
 // that, such that a row's warps take `limit` tiles each at most of the longest possible sequence:
 //   32 (16 rows to a tile, where a tile takes longer: 24 if twice as many CTAs allow it; 17 x 4 tokens of up to 4097: 23.7 us
 //   against 28.8), or as many as the machine reads in 0.75 us of the time that half of all the tables could hold takes, to 64;
-//   10 where even 8 CTAs per row leave half of the machine idle (one sequence of 4096: 10.4 us against about 11, of 8192: 15.1 /
-//   12.8, of 16384: 24.6 / 15.9).
+//   10 where even 8 CTAs per row leave half of the machine idle (one sequence of 8192: 15.1 us against 12.8, of 16384: 24.6 /
+//   15.9; what is shorter, but not short, goes to the wide kernel).
 // More CTAs than that cost their start (about 6 us of a slot each) and are taken where that is small beside the reading (64 of
 // 0..16384: 163 us in fours, 180 as a list).
 int split_of(int64_t rows, int64_t max_tokens, int64_t D, int64_t slots, bool small_tile) {
@@ -994,6 +1131,20 @@ int split_of(int64_t rows, int64_t max_tokens, int64_t D, int64_t slots, bool sm
   return rows * split <= 0x7fffffff ? split : 0;
 }
 
+// CTAs per row tile for the wide kernel, or 0: as many of 8, 4, 2 and 1 as fit an SM each (clusters of 8 fill no more than
+// about half of the SMs) and have 8 tiles. It wins where a row gets more warps out of it than out of the rows kernel and
+// sequences may be long enough to use them (8 KV heads; one sequence of 1500 tokens: 6.4 us against 7.5, of 4096: 7.6 / 10.5, of
+// 8192: 9.5 / 12.8 in a list; four of 4096: 11.0 / 13.4; 16 of 512: 7.0 / 8.4, of 4096: 25.0 / 27.5; but one of 128: 5.0 / 4.5), up
+// to 16 tiles a warp: beyond that, lengths that differ cost more than the warps gain (16 of 0..8192: 37.6 / 34.7). Where it
+// leaves half of the machine idle, up to 10 (one of 16384: 14.1 / 16.0 in a list, of 32768: 22.6 / 21.1).
+int wide_split_of(int64_t rows, int64_t max_tokens, int64_t sm_count, int64_t warps) {
+  const int64_t tiles = (max_tokens + SK_TILE - 1) / SK_TILE, fit = sm_count - sm_count / 8;
+  if (tiles < 32 || rows > fit) return 0;
+  int split = rows * 16 <= sm_count ? 8 : rows * 4 <= fit ? 4 : rows * 2 <= fit ? 2 : 1;
+  while (split > 1 && tiles < split * 8) split /= 2;
+  return tiles <= (rows * split * 2 > sm_count ? 16 : 10) * split * warps ? split : 0;
+}
+
 // The grid never has more warps than the longest possible list has units.
 SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t max_tokens, int64_t D) {
   SkPlan p;
@@ -1003,11 +1154,13 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   const int64_t units = (max_tokens + SK_TILE - 1) / SK_TILE + ROW_COST;  // below 2^28
   const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
   const int64_t slots = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
-  p.split = split_of(rows, max_tokens, D, slots, p.tile_rows == 8);
+  p.split = wide_split_of(rows, max_tokens, sm_count, p.tile_rows == 8 ? WideLayout<128, 1>::WARPS : WideLayout<128, 2>::WARPS);
+  p.wide = p.split > 0;
+  if (!p.wide) p.split = split_of(rows, max_tokens, D, slots, p.tile_rows == 8);
   // Longest first pays where a CTA may have more than a few tiles a warp and several CTAs share an SM or wait for one (64
   // sequences of 0..8192 tokens in pairs: 91.6 us against 109.9; 128 of 0..4096: 87.0 / 108.4) and costs 0.8 us a CTA (256
   // sequences of 128: 28.5 us against 25.6).
-  p.ranked = B > 1 && B <= RANKED && rows * p.split > sm_count && units > (int64_t)p.split * SK_WARPS * 8 ? 1 : 0;
+  p.ranked = !p.wide && B > 1 && B <= RANKED && rows * p.split > sm_count && units > (int64_t)p.split * SK_WARPS * 8 ? 1 : 0;
   p.ctas = slots;
   if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
   if (p.ctas < 1) p.ctas = 1;
@@ -1033,14 +1186,15 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     if (!once.done[h->device]) {
       EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
       EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_rows_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_wide_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideLayout<D, RT>::SMEM));
       once.done[h->device] = true;
     }
   }
   if (p.split > 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_tiles * p.split), 1, 1);
-    cfg.blockDim = dim3(SK_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = SkLayout<D, RT>::SMEM;
+    cfg.blockDim = dim3(p.wide ? WideLayout<D, RT>::THREADS : SK_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = p.wide ? WideLayout<D, RT>::SMEM : SkLayout<D, RT>::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1051,7 +1205,7 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = h->overlap_launch != 0 ? 2 : 1;
-    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, sdpa_kv8_rows_kernel<D, RT>, tk, tv, a));
+    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, p.wide ? sdpa_kv8_wide_kernel<D, RT> : sdpa_kv8_rows_kernel<D, RT>, tk, tv, a));
     EMK_LAUNCH_CHECK(h);
     return EMK_OK;
   }

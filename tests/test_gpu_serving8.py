@@ -443,6 +443,17 @@ def test_sdpa_kv8_many_sequences(ops, room):
     _attend_case(ops, 1, 9, 1, 128, 16, [17] * 700, seed=5, room=room)
 
 
+@pytest.mark.parametrize("B", [1, 3, 6, 12, 16, 17])
+@pytest.mark.parametrize("G,Sq,D", [(2, 1, 128), (1, 3, 64), (4, 3, 64), (2, 5, 128)])
+def test_sdpa_kv8_few_rows(ops, B, G, Sq, D):
+    """A row's warps lie in 8, 4, 2 or 1 CTAs; sequences shorter than their number of warps, and empty ones."""
+    lens = [1500, 0, 17, 640, 1, 1499, 16, 33, 512, 0, 1024, 250, 3, 1500, 90, 47, 1211][:B]
+    got, *args = _attend_case(ops, Sq, 8 * G, 8, D, 64, lens, seed=B + G + D)
+    for _ in range(3):
+        assert torch.equal(ops.sdpa_kv8(*args), got)
+    ops.device_status()
+
+
 def _mixed_lengths(B, longest):
     g = _gen(B)
     lens = (torch.rand(B, generator=g) ** 2 * (longest + 1)).long().clamp(max=longest).tolist()
