@@ -143,13 +143,14 @@ def rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     idx = _cuda_index(x, weight, residual, out, scale_out, hidden_out)
     _check_contig(x, weight, residual, out, scale_out, hidden_out)
     dtype = _dtype_token(x)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("x needs a last axis of one element at least")
-    cols = x.shape[-1]
+    cols = shape[-1]
     n = x.numel()
-    if weight.dtype != x.dtype or weight.numel() != cols:
+    if weight.dtype is not x.dtype or weight.numel() != cols:
         raise ValueError("weight must be a vector of the row length with the dtype of x")
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+    if residual is not None and (residual.dtype is not x.dtype or residual.shape != shape):
         raise ValueError("residual must have the shape and dtype of x")
     if hidden_out is not None and residual is None:
         raise ValueError("hidden_out is the sum of x and residual: give a residual")
@@ -157,7 +158,9 @@ def rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     _check_buffer("scale_out", scale_out, n // cols, torch.float32)
     _check_buffer("hidden_out", hidden_out, n, x.dtype)
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn) if out is None else out
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if scale_out is None else scale_out
+    scale = scale_out
+    if scale is None:  # (sizes one by one: as a tuple they take a microsecond longer)
+        scale = torch.empty(*(shape[:-1] if len(shape) > 1 else ((),)), dtype=torch.float32, device=x.device)
     hidden = None if residual is None else torch.empty_like(x) if hidden_out is None else hidden_out
     if n > 0:
         _call_on(idx, "emk_rmsnorm_e4m3", x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr(),
@@ -652,18 +655,18 @@ def kv8_cache(num_pages: int, Hkv: int, page: int, D: int = 128, device="cuda") 
 def _kv8_sizes(cache: KV8Cache, page_table: torch.Tensor, lens: torch.Tensor) -> tuple[int, int, int, int, int, int]:
     """Checks a cache, its page table ``[B, max_pages]`` and a length per sequence; (pages, Hkv, page, D, B, max_pages)."""
     k, v, k_scale, v_scale = cache
-    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+    if not (k.dtype is v.dtype is torch.float8_e4m3fn):
         raise TypeError("the cache holds float8_e4m3fn codes")
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+    if not (k_scale.dtype is v_scale.dtype is torch.float32):
         raise TypeError("the cache's scales are float32")
-    if page_table.dtype != torch.int32 or lens.dtype != torch.int32:
+    if not (page_table.dtype is lens.dtype is torch.int32):
         raise TypeError("page_table and the sequence lengths must be int32")
-    if k.dim() != 4 or v.shape != k.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+    shape, scales, table = k.shape, k_scale.shape, page_table.shape
+    if len(shape) != 4 or len(scales) != 2 or v.shape != shape or v_scale.shape != scales or scales[0] != shape[0] or scales[1] != shape[1]:
         raise ValueError("cache shapes must be [pages, Hkv, page, D] for the codes and [pages, Hkv] for the scales")
-    if page_table.dim() != 2 or lens.dim() != 1 or lens.shape[0] != page_table.shape[0]:
+    if len(table) != 2 or lens.dim() != 1 or len(lens) != table[0]:
         raise ValueError("page_table must be [B, max_pages], the lengths [B]")
-    pages, Hkv, page, D = k.shape
-    return pages, Hkv, page, D, page_table.shape[0], page_table.shape[1]
+    return (*shape, *table)
 
 
 def kv8_append_(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, ctx_lens: torch.Tensor,
@@ -676,21 +679,22 @@ def kv8_append_(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: t
     idx = _cuda_index(*cache, k, v, page_table, ctx_lens, cu_seqlens)
     _check_contig(*cache, page_table, ctx_lens, cu_seqlens)
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, ctx_lens)
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    if not (k.dtype is v.dtype is torch.bfloat16):
         raise TypeError("kv8_append_ expects bfloat16 keys and values")
-    if cu_seqlens.dtype != torch.int32:
+    if cu_seqlens.dtype is not torch.int32:
         raise TypeError("cu_seqlens must be int32")
-    if k.dim() != 3 or v.shape != k.shape or k.shape[1] != Hkv or k.shape[2] != D:
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[1] != Hkv or shape[2] != D:
         raise ValueError("keys and values must be [T, Hkv, D] with the cache's Hkv and D")
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != B + 1:
+    if cu_seqlens.dim() != 1 or len(cu_seqlens) != B + 1:
         raise ValueError("cu_seqlens must hold B + 1 entries")
-    T = k.shape[0]
-    for t in (k, v):
-        if T > 0 and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D)):
-            raise ValueError("the heads of a token must be contiguous [Hkv, D]")
+    T = shape[0]
+    k_strides, v_strides = k.stride(), v.stride()
+    if T > 0 and (k_strides[2] != 1 or v_strides[2] != 1 or (Hkv > 1 and (k_strides[1] != D or v_strides[1] != D))):
+        raise ValueError("the heads of a token must be contiguous [Hkv, D]")
     if T > 0 and B > 0:
-        _call_on(idx, "emk_kv8_append", k.data_ptr(), v.data_ptr(), k.stride(0) if T > 1 else Hkv * D,
-                 v.stride(0) if T > 1 else Hkv * D, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+        _call_on(idx, "emk_kv8_append", k.data_ptr(), v.data_ptr(), k_strides[0] if T > 1 else Hkv * D,
+                 v_strides[0] if T > 1 else Hkv * D, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
                  cache.v_scale.data_ptr(), page_table.data_ptr(), ctx_lens.data_ptr(), cu_seqlens.data_ptr(), B, T,
                  max_pages, pages, Hkv, page, D)
     return cache
@@ -727,20 +731,22 @@ def sdpa_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, seq_len
     idx = _cuda_index(q, *cache, page_table, seq_lens, out, workspace)
     _check_contig(*cache, page_table, seq_lens, out, workspace)
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, seq_lens)
-    if q.dtype != torch.bfloat16:
+    if q.dtype is not torch.bfloat16:
         raise TypeError("sdpa_kv8 expects bfloat16 queries")
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] == 0 or Hkv == 0 or q.shape[2] % Hkv != 0:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[2] == 0 or Hkv == 0 or shape[2] % Hkv != 0:
         raise ValueError("q must be [B, Sq, Hq, D] with the cache's D and a multiple of its KV heads")
     if max_pages == 0 or pages == 0:
         raise ValueError("the page table and the cache must hold a page at least")
-    Sq, Hq = q.shape[1], q.shape[2]
-    _check_buffer("out", out, q.numel(), torch.bfloat16)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    if q.numel() == 0:
+    _, Sq, Hq, _ = shape
+    _check_buffer("out", out, B * Sq * Hq * D, torch.bfloat16)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    if B * Sq == 0:
         return o
-    if q.stride(3) != 1 or (Hq > 1 and q.stride(2) != D) or (Sq > 1 and B > 1 and q.stride(0) != Sq * q.stride(1)):
+    by_seq, by_token, by_head, by_element = q.stride()
+    if by_element != 1 or (Hq > 1 and by_head != D) or (Sq > 1 and B > 1 and by_seq != Sq * by_token):
         raise ValueError("the heads of a query must be contiguous [Hq, D] and its tokens evenly spaced")
-    ld = q.stride(1) if Sq > 1 else q.stride(0) if B > 1 else Hq * D
+    ld = by_token if Sq > 1 else by_seq if B > 1 else Hq * D
     need = _sdpa_kv8_workspace_bytes(idx, B, Sq, Hq, Hkv, max_pages * page, D)
     if workspace is None and need > 0:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
