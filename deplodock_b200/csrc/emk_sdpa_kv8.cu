@@ -24,9 +24,9 @@
 // log2(v_scale) and p * v_scale / max is what is rounded to f16 (2^-12 relative: p in [0, 2^15], so 2^-29 of the largest
 // contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
 //
-// Three kernels share the loop. Where no sequence can be long (split_of), a cluster of CTAs takes a row tile, deals its tiles
-// to its warps and joins their pieces in distributed shared memory: one launch. The CTAs of the longest sequences come first;
-// where rows are few, CTAs are as large as an SM (wide_split_of). Otherwise:
+// Four kernels share the loop. Many rows of few tiles (short_rows): a warp each. Where no sequence can be long (split_of): a
+// cluster of CTAs takes a row tile, deals its tiles to its warps and joins their pieces in distributed shared memory, the
+// CTAs of the longest sequences first; with few rows (wide_split_of) CTAs as large as an SM. One launch each. Otherwise:
 // Work split: the tiles of 16 tokens of all (sequence, KV head, row tile) form one list, cut into equal ranges, one per
 // warp: sequences of any mix of lengths load all SMs alike without the host knowing the lengths. Beginning a row costs a
 // warp about as much as a tile (the queries, a pipeline to fill, an output), so a row counts ROW_COST tiles more than it
@@ -67,7 +67,7 @@ struct SdpaArgs {
   float2* ml;    // [ranges][2][row_cap]: maximum, sum
   float* part;   // [ranges][2][row_cap][D]
   int max_ranges;
-  int ranked;    // rows kernel: the longest sequences first
+  int ranked;  // rows kernel: the longest sequences first
   int* status;
   unsigned long long limit_ns;
 };
@@ -451,6 +451,21 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
   return true;
 }
 
+// Row rr of the queries of KV head hkv that a warp has seen to its end: channels [D / 8 * g, ...) of it, by its lanes t = const.
+template <int D, int RT>
+__device__ __forceinline__ void store_row(const SdpaArgs& a, const Part<D, RT>& part, int n, int e, float sum, int b, int hkv,
+                                          int rr, int g) {
+  const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // nothing visible: zeros
+  __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + g * (D / 8);
+#pragma unroll
+  for (int j = 0; j < D / 16; j += 4)
+    *reinterpret_cast<uint4*>(out + 2 * j) =
+        make_uint4(pack_bf16x2(part.o[n][j][e] * inv, part.o[n][j][2 + e] * inv), pack_bf16x2(part.o[n][j + 1][e] * inv, part.o[n][j + 1][2 + e] * inv),
+                   pack_bf16x2(part.o[n][j + 2][e] * inv, part.o[n][j + 2][2 + e] * inv),
+                   pack_bf16x2(part.o[n][j + 3][e] * inv, part.o[n][j + 3][2 + e] * inv));
+}
+
 template <int D, int RT>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa_kv8_kernel(const __grid_constant__ CUtensorMap tma_k,
                                                                                           const __grid_constant__ CUtensorMap tma_v,
@@ -557,16 +572,7 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
         const int row = n * 8 + 2 * t + e;
         if (row >= rows) continue;
         if (whole) {
-          const int rr = rt * ROWS + row;
-          const int qi = rr / a.G, head = hkv * a.G + rr - qi * a.G;
-          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-          __nv_bfloat16* out = a.o + (((int64_t)b * a.Sq + qi) * a.Hq + head) * D + g * CH;
-#pragma unroll
-          for (int j = 0; j < STEPS; j += 4)
-            *reinterpret_cast<uint4*>(out + 2 * j) =
-                make_uint4(pack_bf16x2(part.o[n][j][e] * inv, part.o[n][j][2 + e] * inv), pack_bf16x2(part.o[n][j + 1][e] * inv, part.o[n][j + 1][2 + e] * inv),
-                           pack_bf16x2(part.o[n][j + 2][e] * inv, part.o[n][j + 2][2 + e] * inv),
-                           pack_bf16x2(part.o[n][j + 3][e] * inv, part.o[n][j + 3][2 + e] * inv));
+          store_row<D, RT>(a, part, n, e, sum, b, hkv, rt * ROWS + row, g);
         } else {
           // (the first part of a row ends its range and takes slot 1, any other begins it and takes slot 0)
           const int64_t place = range * 2 * a.row_cap + row;
@@ -856,6 +862,60 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
   if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
+// Many rows of few tiles (short_rows): a warp takes a whole row tile, and nothing is joined.
+template <int D, int RT>
+__global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM)
+sdpa_kv8_short_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
+  using L = SkLayout<D, RT>;
+  constexpr int ROWS = L::ROWS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t s_full[SK_WARPS][L::STAGES];
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+    for (int i = 0; i < L::STAGES; ++i) mbar_init(&s_full[warp][i], 1);
+    if (warp == 0) {
+      s_abort = 0;
+      tma_prefetch_desc(&tma_k);
+      tma_prefetch_desc(&tma_v);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  const WaitCtx wc{&s_abort, a.status, a.limit_ns};
+  const int heads = a.Hkv * a.row_tiles;
+  const int row_id = blockIdx.x * SK_WARPS + warp;
+  if (row_id < a.B * heads) {
+    const int b = row_id / heads, hr = row_id - b * heads;
+    const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
+    const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
+    const int len = seq_len(a, b), tiles = seq_tiles(len);
+    RingAt at{0, 0, 0};
+    Part<D, RT> part;
+    if (row_part<D, RT>(a, tma_k, tma_v, smem + warp * L::WARP_RING, s_full[warp], wc, at, b, hkv, rt, len, 0, tiles, part)) {
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = part.l[n][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int row = n * 8 + 2 * t + e;
+          if (row >= rows) continue;
+          store_row<D, RT>(a, part, n, e, sum, b, hkv, rt * ROWS + row, g);
+        }
+      }
+    }
+  }
+  grid_launch_dependents();
+  __syncthreads();
+  if (s_abort) abort_drain();
+}
+
 // Few rows of a certain length (wide_split_of): the same with one CTA of as many warps as an SM holds, so that a row gets four times (16 rows: twice) the warps
 // out of a cluster. A CTA's pieces meet in its own shared memory before the cluster's do.
 template <int D, int RT>
@@ -1092,17 +1152,19 @@ bool sizes_ok(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv) {
   return Hkv <= limit / row_tiles && B <= limit / (Hkv * row_tiles);
 }
 
+enum class Way { LIST, ROWS, WIDE, SHORT };
+
 struct SkPlan {
   int row_tiles, tile_rows, row_cap;
-  int split;   // CTAs per row tile of the wide or the rows kernel; 0: the list kernel and its join
-  bool wide;
+  Way way;
+  int split;   // CTAs per row tile of the wide or the rows kernel
   int ranked;  // rows kernel: the longest sequences first
   int64_t ctas, info_bytes, ml_bytes, part_bytes;
 };
 
 // CTAs per row tile for the rows kernel, or 0 where the list kernel is to run. The host knows the longest a sequence can be
 // (max_tokens), not the lengths. The rows kernel has no list to cut and nothing to join, and wins wherever its CTAs finish
-// about together (8 heads, 64 sequences of 128 tokens: 6.9 us against 12.9; of 1024: 26.2 / 35.4; of 4096: 88.2 / 98.3; of
+// about together (8 KV heads, 64 sequences of 128 tokens: 6.9 us against 12.9; of 1024: 26.2 / 35.4; of 4096: 88.2 / 98.3; of
 // 0..8192: 91.6 / 102.5; 128 of 0..4096: 87.0 / 108.9); a sequence much longer than the others it drags through a few
 // warps, 0.7 us a tile at least. So: as many CTAs per row as fill the machine, or twice
 // that, such that a row's warps take `limit` tiles each at most of the longest possible sequence:
@@ -1131,6 +1193,15 @@ int split_of(int64_t rows, int64_t max_tokens, int64_t D, int64_t slots, bool sm
   return rows * split <= 0x7fffffff ? split : 0;
 }
 
+// Whether a warp takes a whole row tile: where rows are so many and so short that the CTAs' starts and joins are most of a call,
+// and a warp's serial tiles (0.6 us each) are not (8 KV heads; 64 sequences of 64 tokens: 5.2 us against 5.6, but of 128: 7.7 / 7.0;
+// 128 of 128: 10.0 / 14.1; 256 of 32: 6.4 / 16.3, of 256: 26.2 / 32.6; 1024 of 128: 48.3 / 82.8). Not where the lengths may
+// differ by more tiles than that (128 of 1..512: 25.7 / 19.9).
+bool short_rows(int64_t rows, int64_t max_tokens, int64_t slots) {
+  const int64_t tiles = (max_tokens + SK_TILE - 1) / SK_TILE;
+  return tiles <= 32 && tiles * slots <= rows * 8;
+}
+
 // CTAs per row tile for the wide kernel, or 0: as many of 8, 4, 2 and 1 as fit an SM each (clusters of 8 fill no more than
 // about half of the SMs) and have 8 tiles. It wins where a row gets more warps out of it than out of the rows kernel and
 // sequences may be long enough to use them (8 KV heads; one sequence of 1500 tokens: 6.4 us against 7.5, of 4096: 7.6 / 10.5, of
@@ -1154,20 +1225,26 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   const int64_t units = (max_tokens + SK_TILE - 1) / SK_TILE + ROW_COST;  // below 2^28
   const int64_t rows = B * Hkv * p.row_tiles;                              // below 2^31
   const int64_t slots = (int64_t)sm_count * (p.tile_rows == 8 ? 4 : D == 128 ? SkLayout<128, 2>::CTAS_PER_SM : SkLayout<64, 2>::CTAS_PER_SM);
-  p.split = wide_split_of(rows, max_tokens, sm_count, p.tile_rows == 8 ? WideLayout<128, 1>::WARPS : WideLayout<128, 2>::WARPS);
-  p.wide = p.split > 0;
-  if (!p.wide) p.split = split_of(rows, max_tokens, D, slots, p.tile_rows == 8);
+  p.split = 0;
+  p.way = Way::LIST;
+  if (short_rows(rows, max_tokens, slots)) {
+    p.way = Way::SHORT;
+  } else if ((p.split = wide_split_of(rows, max_tokens, sm_count, p.tile_rows == 8 ? WideLayout<128, 1>::WARPS : WideLayout<128, 2>::WARPS)) > 0) {
+    p.way = Way::WIDE;
+  } else if ((p.split = split_of(rows, max_tokens, D, slots, p.tile_rows == 8)) > 0) {
+    p.way = Way::ROWS;
+  }
   // Longest first pays where a CTA may have more than a few tiles a warp and several CTAs share an SM or wait for one (64
   // sequences of 0..8192 tokens in pairs: 91.6 us against 109.9; 128 of 0..4096: 87.0 / 108.4) and costs 0.8 us a CTA (256
   // sequences of 128: 28.5 us against 25.6).
-  p.ranked = !p.wide && B > 1 && B <= RANKED && rows * p.split > sm_count && units > (int64_t)p.split * SK_WARPS * 8 ? 1 : 0;
+  p.ranked = p.way == Way::ROWS && B > 1 && B <= RANKED && rows * p.split > sm_count && units > (int64_t)p.split * SK_WARPS * 8 ? 1 : 0;
   p.ctas = slots;
   if ((rows * units + SK_WARPS - 1) / SK_WARPS < p.ctas) p.ctas = (rows * units + SK_WARPS - 1) / SK_WARPS;
   if (p.ctas < 1) p.ctas = 1;
   p.info_bytes = align16(rows * (int64_t)sizeof(int2));
   p.ml_bytes = align16(p.ctas * SK_WARPS * 2 * p.row_cap * (int64_t)sizeof(float2));
   p.part_bytes = p.ctas * SK_WARPS * 2 * p.row_cap * D * (int64_t)sizeof(float);
-  if (p.split > 0) p.info_bytes = p.ml_bytes = p.part_bytes = 0;  // no workspace
+  if (p.way != Way::LIST) p.info_bytes = p.ml_bytes = p.part_bytes = 0;  // no workspace
   return p;
 }
 
@@ -1186,15 +1263,24 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     if (!once.done[h->device]) {
       EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
       EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_rows_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_short_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
       EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_wide_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideLayout<D, RT>::SMEM));
       once.done[h->device] = true;
     }
   }
-  if (p.split > 0) {
+  if (p.way == Way::SHORT) {
+    const unsigned ctas = (unsigned)(((int64_t)a.B * a.Hkv * a.row_tiles + SK_WARPS - 1) / SK_WARPS);
+    EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_short_kernel<D, RT>, ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
+                                          h->overlap_launch != 0, tk, tv, a));
+    EMK_LAUNCH_CHECK(h);
+    return EMK_OK;
+  }
+  if (p.way != Way::LIST) {
+    const bool wide = p.way == Way::WIDE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.row_tiles * p.split), 1, 1);
-    cfg.blockDim = dim3(p.wide ? WideLayout<D, RT>::THREADS : SK_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = p.wide ? WideLayout<D, RT>::SMEM : SkLayout<D, RT>::SMEM;
+    cfg.blockDim = dim3(wide ? WideLayout<D, RT>::THREADS : SK_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = wide ? WideLayout<D, RT>::SMEM : SkLayout<D, RT>::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1205,7 +1291,7 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = h->overlap_launch != 0 ? 2 : 1;
-    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, p.wide ? sdpa_kv8_wide_kernel<D, RT> : sdpa_kv8_rows_kernel<D, RT>, tk, tv, a));
+    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, wide ? sdpa_kv8_wide_kernel<D, RT> : sdpa_kv8_rows_kernel<D, RT>, tk, tv, a));
     EMK_LAUNCH_CHECK(h);
     return EMK_OK;
   }
@@ -1271,7 +1357,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
                 (long long)(max_pages * page));
     return EMK_ERR_LIMIT;
   }
-  if (workspace == nullptr && p.split == 0) return EMK_ERR_ARG;
+  if (workspace == nullptr && p.way == Way::LIST) return EMK_ERR_ARG;
   if (workspace_bytes < p.info_bytes + p.ml_bytes + p.part_bytes) {
     EMK_SET_ERR(h, "emk_sdpa_kv8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                 (long long)(p.info_bytes + p.ml_bytes + p.part_bytes));

@@ -443,6 +443,20 @@ def test_sdpa_kv8_many_sequences(ops, room):
     _attend_case(ops, 1, 9, 1, 128, 16, [17] * 700, seed=5, room=room)
 
 
+@pytest.mark.parametrize("B,longest", [(130, 33), (301, 130), (600, 500)])
+@pytest.mark.parametrize("G,Sq,D,Hkv", [(2, 1, 128, 8), (1, 3, 64, 7), (4, 3, 64, 5), (2, 5, 128, 7)])
+def test_sdpa_kv8_many_short_rows(ops, B, longest, G, Sq, D, Hkv):
+    """A warp may take a row to itself; empty rows, and rows that are no multiple of the block's warps."""
+    lens = _mixed_lengths(B, longest)
+    if longest == 500:  # not short rows for every head count: the others' kernels see the same lengths
+        got, q, cache, table, lens_t = _attend_case(ops, Sq, G * Hkv, Hkv, D, 16, lens, seed=B + D, check=False)
+        rows = torch.tensor([0, 1, 5, 300, 598, 599])
+        _attend_check(ops, got[rows.cuda()], q[rows.cuda()].cpu(), _to(cache, "cpu"), table.cpu()[rows], [lens[i] for i in rows], 1 / math.sqrt(D))
+    else:
+        _attend_case(ops, Sq, G * Hkv, Hkv, D, 16, lens, seed=B + D)
+    ops.device_status()
+
+
 @pytest.mark.parametrize("B", [1, 3, 6, 12, 16, 17])
 @pytest.mark.parametrize("G,Sq,D", [(2, 1, 128), (1, 3, 64), (4, 3, 64), (2, 5, 128)])
 def test_sdpa_kv8_few_rows(ops, B, G, Sq, D):
