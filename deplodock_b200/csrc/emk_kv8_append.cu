@@ -186,7 +186,7 @@ __device__ __forceinline__ void rescale_page(uint8_t* codes, int at, float ratio
   }
 }
 
-// Few tokens a sequence: a warp per (page, head, K or V), nothing held between the two readings of a row (the second one
+// Few tokens a sequence (few_tokens): a warp per (page, head, K or V), nothing held between the two readings of a row (the second one
 // hits L1), so that all warps of a step are resident at once.
 template <int D>
 __global__ void __launch_bounds__(128) kv8_append_few_kernel(const AppendArgs a) {
@@ -283,6 +283,19 @@ int launch_append(emk_handle_t h, const AppendArgs& a, cudaStream_t s) {
   return launch_units(h, kv8_append_kernel<D, TPU>, a, THREADS / TPU, THREADS, s);
 }
 
+// Few tokens a sequence: the warps of the few-kernel go through a page's new rows in turn, but the places that stand for nothing
+// (half of them at a token a sequence) cost it a warp instead of a CTA of registers. Up to four tokens a sequence on average in any case;
+// up to 16 where the other kernel's CTAs would fill the machine one and a half times, or more often for pages longer than 64
+// tokens, whose rows a warp takes longer to go through. 64 sequences of 8 tokens: 3.9 us against 6.5, of 16: 5.0 / 7.1; 256 of 8:
+// 6.7 / 17.9; 255 single tokens and a prompt of 2048: 12.2 / 17.9; but 8 of 16: 3.9 / 3.0, and 31 single tokens and a prompt of 256:
+// 7.3 / 4.2. (Where one sequence of 64 has nearly all of the tokens: 7.4 / 6.8, in pages of 256 39 / 20.)
+bool few_tokens(const AppendArgs& a, int64_t sm_count, int64_t D) {
+  if (a.T <= 4 * (int64_t)a.B) return true;
+  const int64_t page = (int64_t)1 << a.page_shift;
+  const double fills = (double)a.items * 2. * a.Hkv * (double)(page * D / (8 * AP_PIECES)) / (1024. * (double)sm_count);
+  return a.T <= 16 * (int64_t)a.B && fills >= 1.5 * (double)(page > 64 ? page : 64) / 64.;
+}
+
 template <int D>
 int launch_append_page(emk_handle_t h, const AppendArgs& a, cudaStream_t s) {
   switch (((1 << a.page_shift) * D) / (8 * AP_PIECES)) {  // threads that hold a page's rows
@@ -336,7 +349,7 @@ extern "C" int emk_kv8_append(emk_handle_t h, const void* k, const void* v, int6
   a.status = h->status_dev;
   a.items = T / page + 2 * B;  // places: first_place(B)
   cudaStream_t s = (cudaStream_t)stream;
-  if (T <= 4 * B)  // (a single long sequence among empty ones is slower this way, and right)
+  if (few_tokens(a, h->sm_count, D))
     return D == 128 ? launch_units(h, kv8_append_few_kernel<128>, a, 4, 128, s) : launch_units(h, kv8_append_few_kernel<64>, a, 4, 128, s);
   return D == 128 ? launch_append_page<128>(h, a, s) : launch_append_page<64>(h, a, s);
 }

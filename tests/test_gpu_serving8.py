@@ -314,6 +314,15 @@ def test_kv8_append_single_tokens(ops, B):
     _check_append(ops, 2, 128, 32, ctx, [1] * B, seed=B, size=(-3, 9))
 
 
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("kind", ["even", "mixed", "prompt"])
+def test_kv8_append_some_tokens_of_many_sequences(ops, page, kind):
+    B = 70
+    ctx = [(53 * b) % 300 for b in range(B)]
+    new = {"even": [9] * B, "mixed": [(11 * b) % 31 for b in range(B)], "prompt": [1] * 30 + [700] + [2] * (B - 31)}[kind]
+    _check_append(ops, 8, 128, page, ctx, new, seed=page, size=(-3, 6))
+
+
 def test_kv8_append_extreme_sizes_and_non_finite(ops):
     _check_append(ops, 2, 64, 16, [3, 20, 0], [20, 5, 9], seed=1, size=(-120, 126))
     _check_append(ops, 2, 128, 16, [3, 20, 0], [20, 5, 9], seed=2, size=(-140, -60))
