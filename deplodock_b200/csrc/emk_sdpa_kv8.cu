@@ -181,8 +181,55 @@ struct Part {
   float m[RT][2], l[RT][2];
 };
 
-// Tiles [ta, tb) of the row tile rt of KV head hkv of sequence b, by one warp. False: a wait ran out (recorded).
+// A tile that not all rows see to its end: a NaN value must not reach the rows whose probability of its token is a masked zero
+// (0 * NaN). NaN codes leave the fragment, and the rows that see their tokens get NaN in those channels here.
 template <int D, int RT>
+__device__ __forceinline__ void spoil_seen(uint32_t (&w)[4][D / 32], int tok0, const int (&limit)[RT][2], Part<D, RT>& part) {
+  const auto nan_bytes = [](uint32_t codes) { return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu); };
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) any |= nan_bytes(w[u][j]);
+  }
+  if (!__any_sync(0xffffffffu, any != 0)) return;
+  const int lane = threadIdx.x & 31;
+  uint32_t seen[RT][2] = {};  // bit c: channel D / 8 * g + c has a NaN among the tokens that the row sees
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint32_t mine = 0;  // of this lane's token u
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint32_t v = nan_bytes(w[u][j]);
+      w[u][j] &= ~v;
+      mine |= (((v & 0x08040201u) * 0x01010101u) >> 24) << (4 * j);  // a bit per byte
+    }
+#pragma unroll
+    for (int src = 0; src < 4; ++src) {  // the four lanes that hold these channels
+      const uint32_t theirs = __shfl_sync(0xffffffffu, mine, (lane & 28) | src);
+      const int tok = tok0 + token_of<D>(2 * src + (u & 1)) + (u >> 1) * 8;
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) seen[n][e] |= tok < limit[n][e] ? theirs : 0u;
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if ((seen[n][x & 1] >> (2 * j + (x >> 1))) & 1u) part.o[n][j][x] = __uint_as_float(0x7fc00000u);
+    }
+  }
+}
+
+// Tiles [ta, tb) of the row tile rt of KV head hkv of sequence b, by one warp. False: a wait ran out (recorded). EVEN: a query
+// token per sequence, so that all rows see the same tokens (a kernel of its own: the limits per row and what follows from them cost
+// 16 warps an SM registers that they do not have, 3 % of 64 sequences of 4096 tokens).
+template <int D, int RT, bool EVEN>
 __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& tma_k, const CUtensorMap& tma_v, uint8_t* ring,
                                          uint64_t* full, const WaitCtx& wc, RingAt& at, int b, int hkv, int rt, int len, int ta,
                                          int tb, Part<D, RT>& part) {
@@ -235,7 +282,7 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
   // of the rows whose logits this lane gets, 2 t and 2 t + 1 of each tile: factor of the logits, tokens that the row sees
   float qs[RT][2];
   int limit[RT][2];
-  int limit_min = len;
+  int limit_min = len;  // (EVEN: of all rows)
 #pragma unroll
   for (int n = 0; n < RT; ++n) {
     const int row = n * 8 + g;
@@ -271,11 +318,11 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
       qf[n][j][1] = pack_f16x2(bf16_lo(hi) * up, bf16_hi(hi) * up);
     }
     const int sees = valid ? max(len - a.Sq + qi + 1, 0) : len;  // rows past the last are computed and dropped
-    limit_min = min(limit_min, __reduce_min_sync(0xffffffffu, sees));
+    if (!EVEN) limit_min = min(limit_min, __reduce_min_sync(0xffffffffu, sees));
 #pragma unroll
     for (int e2 = 0; e2 < 2; ++e2) {
       qs[n][e2] = __shfl_sync(0xffffffffu, factor, (2 * t + e2) * 4);
-      limit[n][e2] = __shfl_sync(0xffffffffu, sees, (2 * t + e2) * 4);
+      limit[n][e2] = EVEN ? len : __shfl_sync(0xffffffffu, sees, (2 * t + e2) * 4);
     }
   }
 
@@ -436,6 +483,7 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
         for (int j = 0; j < L::V_BYTES / 4; ++j) w[u][j] = in ? w[u][j] : 0u;
       }
     }
+    if (!EVEN && edge && limit_min < len) spoil_seen<D, RT>(w, (ta + i) * SK_TILE, limit, part);
 #pragma unroll
     for (int j = 0; j < L::V_BYTES / 4; ++j) {
 #pragma unroll
@@ -466,7 +514,7 @@ __device__ __forceinline__ void store_row(const SdpaArgs& a, const Part<D, RT>& 
                    pack_bf16x2(part.o[n][j + 3][e] * inv, part.o[n][j + 3][2 + e] * inv));
 }
 
-template <int D, int RT>
+template <int D, int RT, bool EVEN>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa_kv8_kernel(const __grid_constant__ CUtensorMap tma_k,
                                                                                           const __grid_constant__ CUtensorMap tma_v,
                                                                                           const SdpaArgs a) {
@@ -555,7 +603,7 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
     const int hkv = hr / a.row_tiles, rt = hr - hkv * a.row_tiles;
     const int rows = min(ROWS, a.G * a.Sq - rt * ROWS);
     Part<D, RT> part;
-    alive = row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part);
+    alive = row_part<D, RT, EVEN>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part);
     if (!alive) break;
     // ---- this range's part of the row: channels [CH g, CH (g + 1)) of rows 2 t and 2 t + 1 of each tile per lane ----
     const bool whole = ta == 0 && tb == tiles;
@@ -772,7 +820,7 @@ __device__ __forceinline__ int sequence_of_rank(const SdpaArgs& a, int rank, int
 
 // Many rows, or short ones (split_of): a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose pieces meet in distributed
 // shared memory. No list to cut, no workspace, no second kernel: what is left of a call is one launch and one row's latency.
-template <int D, int RT>
+template <int D, int RT, bool EVEN>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM)
 sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
   using L = SkLayout<D, RT>;
@@ -818,7 +866,7 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     uint8_t* ring = smem + warp * L::WARP_RING;
     RingAt at{0, 0, 0};
     Part<D, RT> part;
-    if (row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part))
+    if (row_part<D, RT, EVEN>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part))
       leave_piece<D, RT>(part, ring, s_m[warp], s_l[warp]);
   }
   grid_launch_dependents();
@@ -863,7 +911,7 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
 }
 
 // Many rows of few tiles (short_rows): a warp takes a whole row tile, and nothing is joined.
-template <int D, int RT>
+template <int D, int RT, bool EVEN>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM)
 sdpa_kv8_short_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
   using L = SkLayout<D, RT>;
@@ -895,7 +943,7 @@ sdpa_kv8_short_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_co
     const int len = seq_len(a, b), tiles = seq_tiles(len);
     RingAt at{0, 0, 0};
     Part<D, RT> part;
-    if (row_part<D, RT>(a, tma_k, tma_v, smem + warp * L::WARP_RING, s_full[warp], wc, at, b, hkv, rt, len, 0, tiles, part)) {
+    if (row_part<D, RT, EVEN>(a, tma_k, tma_v, smem + warp * L::WARP_RING, s_full[warp], wc, at, b, hkv, rt, len, 0, tiles, part)) {
 #pragma unroll
       for (int n = 0; n < RT; ++n) {
 #pragma unroll
@@ -918,7 +966,7 @@ sdpa_kv8_short_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_co
 
 // Few rows of a certain length (wide_split_of): the same with one CTA of as many warps as an SM holds, so that a row gets four times (16 rows: twice) the warps
 // out of a cluster. A CTA's pieces meet in its own shared memory before the cluster's do.
-template <int D, int RT>
+template <int D, int RT, bool EVEN>
 __global__ void __launch_bounds__(WideLayout<D, RT>::THREADS, 1)
 sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
   using L = SkLayout<D, RT>;
@@ -961,7 +1009,7 @@ sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     uint8_t* ring = smem + warp * L::WARP_RING;
     RingAt at{0, 0, 0};
     Part<D, RT> part;
-    if (row_part<D, RT>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part))
+    if (row_part<D, RT, EVEN>(a, tma_k, tma_v, ring, s_full[warp], wc, at, b, hkv, rt, len, ta, tb, part))
       leave_piece<D, RT>(part, ring, s_m[warp], s_l[warp]);
   }
   grid_launch_dependents();
@@ -1248,7 +1296,7 @@ SkPlan plan_of(int sm_count, int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int
   return p;
 }
 
-template <int D, int RT>
+template <int D, int RT, bool EVEN>
 int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t s) {
   CUtensorMap tk, tv;
   const uint64_t rows = (uint64_t)a.num_pages * a.Hkv << a.page_shift;
@@ -1261,16 +1309,16 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
   {
     std::lock_guard<std::mutex> lk(once.mu);
     if (!once.done[h->device]) {
-      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
-      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_rows_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
-      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_short_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
-      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_wide_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_kernel<D, RT, EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_rows_kernel<D, RT, EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_short_kernel<D, RT, EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SkLayout<D, RT>::SMEM));
+      EMK_CUDA_TRY(h, cudaFuncSetAttribute(sdpa_kv8_wide_kernel<D, RT, EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideLayout<D, RT>::SMEM));
       once.done[h->device] = true;
     }
   }
   if (p.way == Way::SHORT) {
     const unsigned ctas = (unsigned)(((int64_t)a.B * a.Hkv * a.row_tiles + SK_WARPS - 1) / SK_WARPS);
-    EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_short_kernel<D, RT>, ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
+    EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_short_kernel<D, RT, EVEN>, ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
                                           h->overlap_launch != 0, tk, tv, a));
     EMK_LAUNCH_CHECK(h);
     return EMK_OK;
@@ -1291,11 +1339,11 @@ int launch_sdpa(emk_handle_t h, const SdpaArgs& a, const SkPlan& p, cudaStream_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = h->overlap_launch != 0 ? 2 : 1;
-    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, wide ? sdpa_kv8_wide_kernel<D, RT> : sdpa_kv8_rows_kernel<D, RT>, tk, tv, a));
+    EMK_CUDA_TRY(h, cudaLaunchKernelEx(&cfg, wide ? sdpa_kv8_wide_kernel<D, RT, EVEN> : sdpa_kv8_rows_kernel<D, RT, EVEN>, tk, tv, a));
     EMK_LAUNCH_CHECK(h);
     return EMK_OK;
   }
-  EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_kernel<D, RT>, (unsigned)p.ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
+  EMK_CUDA_TRY(h, launch_after_prologue(sdpa_kv8_kernel<D, RT, EVEN>, (unsigned)p.ctas, SK_THREADS, SkLayout<D, RT>::SMEM, s,
                                         h->overlap_launch != 0, tk, tv, a));
   EMK_LAUNCH_CHECK(h);
   // Few rows: a row may be cut into hundreds of pieces, and sixteen warps share them; many rows: a few pieces each.
@@ -1394,6 +1442,7 @@ extern "C" int emk_sdpa_kv8(emk_handle_t h, const void* q, int64_t ld_q, const v
   a.status = h->status_dev;
   a.limit_ns = h->wait_limit_ns;
   cudaStream_t s = (cudaStream_t)stream;
-  if (D == 128) return p.tile_rows == 8 ? launch_sdpa<128, 1>(h, a, p, s) : launch_sdpa<128, 2>(h, a, p, s);
-  return p.tile_rows == 8 ? launch_sdpa<64, 1>(h, a, p, s) : launch_sdpa<64, 2>(h, a, p, s);
+  if (p.tile_rows == 16) return D == 128 ? launch_sdpa<128, 2, false>(h, a, p, s) : launch_sdpa<64, 2, false>(h, a, p, s);
+  if (Sq == 1) return D == 128 ? launch_sdpa<128, 1, true>(h, a, p, s) : launch_sdpa<64, 1, true>(h, a, p, s);
+  return D == 128 ? launch_sdpa<128, 1, false>(h, a, p, s) : launch_sdpa<64, 1, false>(h, a, p, s);
 }

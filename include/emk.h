@@ -291,12 +291,14 @@ int emk_sdpa_causal_gqa_bf16_varlen(emk_handle_t h, const void* q, const void* k
  * device, the Sq queries' own tokens included, already appended); query i sits at position seq_lens[b] - Sq + i and
  * sees the tokens up to itself; a query that sees none gets zeros. q: bf16, row (b * Sq + i) of pitch ld_q elements,
  * head h at column h * D; o: bf16 [B * Sq][Hq * D], which may be q itself where ld_q is Hq * D; Hq a multiple of Hkv.
- * Sequences may share pages. Whatever lies in a page behind a sequence's last token is not used; scales must not be
- * negative, and a zero value scale makes a page's values zero. Lengths are clamped to what max_pages pages hold, page
+ * Sequences may share pages. Whatever lies in a page behind a sequence's last token is not used, and a query's result
+ * does not depend on the tokens behind its position, NaN among them. Scales must be finite and not negative; a zero
+ * value scale makes a page's values zero. Lengths are clamped to what max_pages pages hold, page
  * ids to the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
  * emk_sdpa_kv8_workspace_bytes(h, B, Sq, Hq, Hkv, max_pages * page, D) bytes (0, and NULL, where no sequence can be long),
- * not used between calls; calls that may overlap need one each. The first call for a head dimension and up to / over 8
- * queries x heads a KV head on a device sets the kernels' shared-memory attributes: make it before any stream capture. */
+ * not used between calls; calls that may overlap need one each. The first call for a head dimension, for one or several
+ * query tokens and for up to or over 8 queries x heads a KV head on a device sets the kernels' shared-memory attributes:
+ * make it before any stream capture. */
 int emk_kv8_append(emk_handle_t h, const void* k, const void* v, int64_t ld_k, int64_t ld_v, void* k_codes,
                    void* v_codes, float* k_scale, float* v_scale, const int32_t* page_table, const int32_t* ctx_lens,
                    const int32_t* cu_seqlens, int64_t B, int64_t T, int64_t max_pages, int64_t num_pages, int64_t Hkv,

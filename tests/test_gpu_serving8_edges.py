@@ -84,3 +84,44 @@ def test_two_captured_graphs_in_flight_at_once(ops, room):  # noqa: F811
         for _, out, want, *_ in states:
             assert torch.equal(out, want)
     ops.device_status()
+
+
+@pytest.mark.parametrize("room", ROOM + ["short"])
+@pytest.mark.parametrize("Sq,G,D", [(2, 1, 128), (4, 4, 64), (5, 2, 128), (4, 1, 64), (20, 1, 128)])
+def test_nan_tokens_reach_only_the_queries_that_see_them(ops, room, Sq, G, D):  # noqa: F811
+    """A draft token's NaN values spoil its channel for the queries at or behind it, and leave those before it alone."""
+    page, Hkv = 16, 2
+    lens = [70, 33, 16, Sq, 64, 3] * (200 if room == "short" else 1)
+    B, max_pages = len(lens), 5
+    g = _gen(Sq + D)
+    cache = _random_cache(ops, B * max_pages, Hkv, page, D, 8)
+    rows = torch.randperm(B * max_pages, generator=g).view(B, max_pages).tolist()
+    bad = torch.zeros(B, Hkv, max_pages * page, D, dtype=torch.bool)  # NaN values, by token
+    for b, n in enumerate(lens):
+        for back, head, channels in ((1, 0, [0, 9]), (2, 0, [5, D - 1]), (1, 1, [D // 2]), (Sq, 1, [2, 3])):
+            if back <= n:
+                t = n - back
+                bad[b, head, t, channels] = True
+                cache.v.view(torch.uint8)[rows[b][t // page], head, t % page, channels] = 0x7f if back & 1 else 0xff
+                cache.k.view(torch.uint8)[rows[b][(n - 1) // page], head, (n - 1) % page, 7] = 0x7f  # and the last key
+    q = torch.randn(B, Sq, G * Hkv, D, generator=g).bfloat16()
+    lens_t = torch.tensor(lens, dtype=torch.int32)
+    table = _table(rows, "tight" if room == "short" else room, page).cuda()
+    got = ops.sdpa_kv8(q.cuda(), _to(cache, "cuda"), table, lens_t.cuda())
+    ops.device_status()
+    got = got.cpu()
+    for b, n in enumerate(lens[:6]):
+        for i in range(Sq):
+            m = n - Sq + i + 1
+            want = bad[b, :, :max(m, 0)].any(1)  # [Hkv, D]
+            if m == n:
+                want = torch.ones_like(want)  # the last token's key is NaN
+            assert torch.equal(torch.isnan(got[b, i].float()).view(Hkv, G, D), want[:, None].expand(-1, G, -1)), (b, i)
+    # the finite values are right: the same cache with zeros for the NaN values gives them
+    clean = type(cache)(*(x.clone() for x in cache))
+    for codes in (clean.k.view(torch.uint8), clean.v.view(torch.uint8)):
+        codes[(codes & 0x7f) == 0x7f] = 0
+    ref = ops.sdpa_kv8(q.cuda(), _to(clean, "cuda"), table, lens_t.cuda()).cpu()
+    # (to the tolerance, not to the bit: when one row's maximum moves, the others' roundings move with it)
+    for some in (ref, torch.where(torch.isnan(got), ref, got)):
+        _attend_check(ops, some[:6], q[:6], clean, torch.tensor(rows[:6]), lens[:6], 1 / math.sqrt(D))
