@@ -818,8 +818,9 @@ __device__ __forceinline__ int sequence_of_rank(const SdpaArgs& a, int rank, int
   return 0;  // not reached: rank < B
 }
 
-// Many rows, or short ones (split_of): a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose pieces meet in distributed
-// shared memory. No list to cut, no workspace, no second kernel: what is left of a call is one launch and one row's latency.
+// Many rows, or short ones (split_of): a cluster of 1, 2, 4 or 8 CTAs per row tile deals its tiles to its warps, whose
+// pieces meet in distributed shared memory. No list to cut, no workspace, no second kernel: what is left of a call is one
+// launch and one row's latency.
 template <int D, int RT, bool EVEN>
 __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM)
 sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
@@ -964,8 +965,9 @@ sdpa_kv8_short_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_co
   if (s_abort) abort_drain();
 }
 
-// Few rows of a certain length (wide_split_of): the same with one CTA of as many warps as an SM holds, so that a row gets four times (16 rows: twice) the warps
-// out of a cluster. A CTA's pieces meet in its own shared memory before the cluster's do.
+// Few rows of a certain length (wide_split_of): the same with one CTA of as many warps as an SM holds, so that a row gets
+// four times (16 rows: twice) the warps out of a cluster. A CTA's pieces meet in its own shared memory before the cluster's
+// do.
 template <int D, int RT, bool EVEN>
 __global__ void __launch_bounds__(WideLayout<D, RT>::THREADS, 1)
 sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constant__ CUtensorMap tma_v, const SdpaArgs a) {
