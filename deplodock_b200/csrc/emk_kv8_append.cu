@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(128) kv8_append_few_kernel(const AppendArgs a)
   const int lane = threadIdx.x & 31;
   const int u = (int)(blockIdx.x % a.groups) * 4 + (threadIdx.x >> 5);
   Touched p;
+  grid_dependency_wait();
+  grid_launch_dependents();
   if (u >= 2 * a.Hkv || !find_page(a, blockIdx.x / a.groups, p)) return;  // (a warp at a time)
   const Unit r = unit_of<D>(a, p, u);
   const int tok = lane / LPT, piece = lane % LPT;
@@ -223,6 +225,8 @@ __global__ void __launch_bounds__(TPU < 128 ? 128 : TPU, TPU <= 128 ? 8 : TPU ==
   __shared__ float red[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Touched p;
+  grid_dependency_wait();
+  grid_launch_dependents();
   if (!find_page(a, blockIdx.x / a.groups, p)) return;  // uniform
   const int group = threadIdx.x / TPU, tid = threadIdx.x % TPU;
   const int tok = tid / LPT, piece = tid % LPT;
@@ -273,7 +277,7 @@ int launch_units(emk_handle_t h, K kernel, AppendArgs a, int per, int threads, c
     EMK_SET_ERR(h, "emk_kv8_append: more than 2^31 - 1 blocks");
     return EMK_ERR_LIMIT;
   }
-  kernel<<<(unsigned)(a.items * a.groups), threads, 0, s>>>(a);
+  EMK_CUDA_TRY(h, launch_after_prologue(kernel, (unsigned)(a.items * a.groups), (unsigned)threads, 0, s, h->overlap_launch != 0, a));
   EMK_LAUNCH_CHECK(h);
   return EMK_OK;
 }
