@@ -349,6 +349,11 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
     tma_prefetch_desc(&tma_w);
     tma_prefetch_desc(&tma_x);
   }
+  // W may come to L2 while the kernel before this one still runs: a prefetch reads nothing, so it need not wait (a layer of a
+  // single-token step with 400 MB of weights 29.8 -> 29.0 us).
+  if (warp == 5 && lane == 0) {
+    for (int kb = kb0; kb < kb1 && kb < kb0 + g.stages; ++kb) tma_prefetch_2d(&tma_w, kb * BKB, tn * BM);
+  }
   if (warp == 0) {
     tmem_alloc(&bars->tmem_base, TMEM_COLS);
     tmem_relinquish();
