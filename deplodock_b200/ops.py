@@ -7,6 +7,7 @@ Each function names the reference Torch-IR op it stands for (``emmy/compiler/ir/
 
 from __future__ import annotations
 
+import functools
 import math
 from ctypes import c_void_p
 from typing import NamedTuple
@@ -700,20 +701,15 @@ def kv8_append_(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: t
     return cache
 
 
-_KV8_WORKSPACE_BYTES: dict[tuple, int] = {}
-
-
+@functools.lru_cache(maxsize=1024)  # (of the sizes alone)
 def _sdpa_kv8_workspace_bytes(idx: int, *sizes: int) -> int:
-    n = _KV8_WORKSPACE_BYTES.get((idx, *sizes))
-    if n is None:
-        h = handle(idx)
-        n = _KV8_WORKSPACE_BYTES[(idx, *sizes)] = int(h.lib.emk_sdpa_kv8_workspace_bytes(h.ptr, *sizes))
-    return n
+    h = handle(idx)
+    return int(h.lib.emk_sdpa_kv8_workspace_bytes(h.ptr, *sizes))
 
 
 def sdpa_kv8_workspace(B: int, Sq: int, Hq: int, cache: KV8Cache, max_pages: int) -> torch.Tensor:
-    """Scratch for :func:`sdpa_kv8` over ``cache`` with a page table of ``max_pages`` columns; it holds nothing between
-    calls. Calls that may run at the same time (two streams, two captured graphs) need one each."""
+    """Scratch for :func:`sdpa_kv8` calls of these sizes over ``cache`` with a page table of ``max_pages`` columns (a smaller
+    batch may need more: fewer rows are cut into more pieces); it holds nothing between calls. Calls that may run at the same time (two streams, two captured graphs) need one each."""
     _, Hkv, page, D = cache.k.shape
     n = _sdpa_kv8_workspace_bytes(cache.k.get_device(), int(B), int(Sq), int(Hq), Hkv, int(max_pages) * page, D)
     return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
