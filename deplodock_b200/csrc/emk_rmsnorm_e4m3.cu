@@ -116,12 +116,16 @@ struct Raw<__nv_bfloat16> {
   }
 };
 
+// CTAs per SM: as many as hold the row's packs without spilling (a few registers where there is no alignment to use).
+template <int NV, bool RAGGED, bool RES>
+constexpr int NORM_CTAS = RAGGED ? (RES || NV == 8 ? 2 : 4) : NV == 8 ? (RES ? 2 : 3) : NV == 4 ? (RES ? 3 : 4) : 5;
+
 // TPR threads hold a row (8, 32, 64, 128 or 256), NV packs of V elements each. RAGGED: the rows' length is no multiple of V;
 // packs lie at the multiples of V of the whole array, and the elements of a row before its first and behind its last full
 // pack (fewer than V each) go to one thread each. RES: with a residual (a kernel of its own: without one a row needs half
 // the registers, and twice the rows fit an SM).
 template <typename T, int NV, int TPR, bool RAGGED, bool RES>
-__global__ void __launch_bounds__(256, RAGGED ? (RES || NV == 8 ? 2 : 4) : NV == 8 ? (RES ? 2 : 3) : NV == 4 ? (RES ? 3 : 4) : 5)
+__global__ void __launch_bounds__(256, NORM_CTAS<NV, RAGGED, RES>)
 rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint8_t* __restrict__ q, float* __restrict__ scale,
                     T* hidden, int64_t rows, int cols, float eps) {
   constexpr int V = Raw<T>::V;

@@ -708,8 +708,9 @@ def _sdpa_kv8_workspace_bytes(idx: int, *sizes: int) -> int:
 
 
 def sdpa_kv8_workspace(B: int, Sq: int, Hq: int, cache: KV8Cache, max_pages: int) -> torch.Tensor:
-    """Scratch for :func:`sdpa_kv8` calls of these sizes over ``cache`` with a page table of ``max_pages`` columns (a smaller
-    batch may need more: fewer rows are cut into more pieces); it holds nothing between calls. Calls that may run at the same time (two streams, two captured graphs) need one each."""
+    """Scratch for :func:`sdpa_kv8` calls of these sizes over ``cache`` with a page table of ``max_pages`` columns (a
+    smaller batch may need more: fewer rows are cut into more pieces); it holds nothing between calls. Calls that may run
+    at the same time (two streams, two captured graphs) need one each."""
     _, Hkv, page, D = cache.k.shape
     n = _sdpa_kv8_workspace_bytes(cache.k.get_device(), int(B), int(Sq), int(Hq), Hkv, int(max_pages) * page, D)
     return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)

@@ -65,12 +65,14 @@ REF_ROWS_MAX = 12
 #: by this list. ``tests/test_profile_cli.py`` checks it against the ``__global__`` definitions under ``csrc/``.
 OWN_KERNELS = frozenset({
     "elementwise_kernel", "embed_gather_kernel", "emk_wait_expiry_kernel", "expand_e4m3_bf16_kernel",
-    "fmha_causal_kernel", "gemm2_bf16_kernel", "gemm2_chain_kernel", "gemm_bf16_kernel", "gemm_f32_simt_kernel", "gemm_f32_tiled_kernel",
-    "gemm_simt_kernel", "gemm_w8_kernel", "loop_linear_f32_kernel", "loop_rope_scores_f32_kernel",
+    "fmha_causal_kernel", "gemm2_bf16_kernel", "gemm2_chain_kernel", "gemm2_e4m3_kernel", "gemm_bf16_kernel",
+    "gemm_e4m3_rows_kernel", "gemm_f32_simt_kernel", "gemm_f32_tiled_kernel", "gemm_simt_kernel", "gemm_w8_kernel",
+    "kv8_append_few_kernel", "kv8_append_kernel", "loop_linear_f32_kernel", "loop_rope_scores_f32_kernel",
     "loop_softmax_pv_f32_kernel", "pool_norm_l2_kernel", "qknorm_rope_kernel", "rmsnorm_cta_kernel",
-    "rmsnorm_from_partials_kernel", "rmsnorm_generic_kernel", "rmsnorm_warp_kernel", "sdpa_simt_kernel",
-    "softmax_generic_kernel", "softmax_multiwarp_kernel", "softmax_warp_kernel", "split6_bf16_kernel",
-    "varlen_items_kernel"})
+    "rmsnorm_e4m3_kernel", "rmsnorm_e4m3_long_kernel", "rmsnorm_from_partials_kernel", "rmsnorm_generic_kernel",
+    "rmsnorm_warp_kernel", "sdpa_kv8_join_kernel", "sdpa_kv8_kernel", "sdpa_kv8_rows_kernel",
+    "sdpa_kv8_short_kernel", "sdpa_kv8_wide_kernel", "sdpa_simt_kernel", "softmax_generic_kernel",
+    "softmax_multiwarp_kernel", "softmax_warp_kernel", "split6_bf16_kernel", "varlen_items_kernel"})
 _BASE_NAME_RE = re.compile(r"^(?:void\s+)?(?:[A-Za-z_][A-Za-z_0-9]*::|\(anonymous namespace\)::|<unnamed>::)*"
                            r"([A-Za-z_][A-Za-z_0-9]*)")
 
