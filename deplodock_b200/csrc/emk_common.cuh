@@ -408,6 +408,13 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t smem_addr, uint32_t rank) 
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+
+// The CTAs of a cluster wait for one another and publish nothing: what they have read from each other's shared memory is in
+// registers that later instructions used. (The arrive of cluster_sync_all waits until the thread's global stores are
+// acknowledged.)
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // Arrive on a barrier of a CTA of this cluster WITHOUT release semantics: for hand-offs that guard tensor memory only
 // ("this warp's tcgen05.ld have returned, the accumulator may be overwritten"). tcgen05.wait::ld has already made the
 // loads complete, so nothing in memory has to become visible to the waiter. A releasing arrive at cluster scope made

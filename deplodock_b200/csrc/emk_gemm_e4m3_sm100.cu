@@ -455,7 +455,7 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
     }
   }
   __syncwarp();
-  if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
+  if (split > 1) cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
 }
 
 constexpr int rows_smem(int nt, int stages) {

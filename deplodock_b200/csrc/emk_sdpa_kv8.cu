@@ -908,7 +908,7 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     else
       *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
   }
-  if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
+  if (split > 1) cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
 }
 
 // Many rows of few tiles (short_rows): a warp takes a whole row tile, and nothing is joined.
@@ -1083,7 +1083,7 @@ sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     }
     store(row, acc, sum);
   }
-  cluster_sync_all();  // no CTA leaves while another reads its shared memory
+  cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
 }
 
 // Joins the pieces of every row that was cut: block (row of tiles, row of the tile). The places of a row's pieces are
