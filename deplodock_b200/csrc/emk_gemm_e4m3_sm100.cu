@@ -285,7 +285,7 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (bars->abort_flag) abort_drain();
-  cluster_sync_all();  // the peer's shared and tensor memory stay alive until the leader's MMAs are done
+  cluster_sync_relaxed();  // the peer's shared and tensor memory stay alive until the leader's MMAs are done
   if (warp == 0) tmem_dealloc_pair(tmem_base, 512);
 }
 
