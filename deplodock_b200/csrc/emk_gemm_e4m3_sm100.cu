@@ -563,7 +563,7 @@ int linear_pairs(emk_handle_t h, const void* x, const void* w, const Gemm8Args& 
   // 256-, 192- or 128-column tiles takes 7.3 / 6.0 / 4.8 us at K = 2048 and 3.8 / 3.2 / 2.5 at K = 1024 (operand traffic
   // per multiplication grows as the tile narrows), so narrow tiles pay only where they save rounds; the weights stand a
   // little above those ratios because near a tie the wide tile is the faster. Measured at 1024 x 6144 x 2048:
-  // 17.0 / 15.7 / 17.9 us; 256 x 4096 x 1024: 7.7 / 6.5 / 5.7; 4096 x 6144 x 2048: 42.6 / 44.5 / 53.8.
+  // 16.9 / 15.3 / 17.8 us; 256 x 4096 x 1024: 7.4 / 6.3 / 5.5; 4096 x 6144 x 2048: 42.1 / 43.8 / 53.1.
   const int64_t pairs = h->sm_count / 2, tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
   const auto cost = [&](int64_t bn, int64_t weight) { return (tiles_m * ((g.N + bn - 1) / bn) + pairs - 1) / pairs * weight; };
   const int64_t c256 = cost(256, 100), c192 = cost(192, 88), c128 = cost(128, 69);
@@ -572,9 +572,9 @@ int linear_pairs(emk_handle_t h, const void* x, const void* w, const Gemm8Args& 
 }
 
 // Which kernel: up to 64 rows the pairs would multiply padding; beyond that the rows kernel wins where only its split of K
-// fills the machine: few tiles and a K worth splitting (1024 x 128 x 4096: 7.0 us against 11.4; 512 x 512 x 2048: 6.7
-// against 7.7), or a long K under one row of tiles (128 x 8192 x 8192: 19.7 against 22.4). It loses otherwise
-// (128 x 2048 x 512: 6.8 against 4.9; 128 x 4096 x 1024: 6.4 against 5.8; 256 x 4096 x 1024: 11.0 against 5.8).
+// fills the machine: few tiles and a K worth splitting (1024 x 128 x 4096: 6.9 us against 10.6; 512 x 512 x 2048: 6.4
+// against 7.0), or a long K under one row of tiles (128 x 8192 x 8192: 18.2 against 21.4). It loses otherwise
+// (128 x 2048 x 512: 6.5 against 4.5; 128 x 4096 x 1024: 6.2 against 5.4; 256 x 4096 x 1024: 7.5 against 5.5).
 bool few_rows(int64_t M, int64_t N, int64_t K) {
   if (M <= 64) return true;
   return ((M + BM - 1) / BM * ((N + BM - 1) / BM) <= 16 && K >= 2048) || (M <= BM && K >= 4096);

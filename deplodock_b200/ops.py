@@ -98,10 +98,20 @@ def _call_on(idx: int, name: str, *args) -> None:
         h.check(rc, name)
 
 
-def _check_contig(*tensors: torch.Tensor | None) -> None:
+def _contiguous_index(*tensors: torch.Tensor | None) -> int:
+    """:func:`_cuda_index` of tensors that have to be contiguous, in one pass over them."""
+    idx = None
     for t in tensors:
-        if t is not None and not t.is_contiguous():
+        if t is None:
+            continue
+        d = t.get_device()
+        if d != idx:
+            if d < 0 or idx is not None:
+                _cuda_index(*tensors)  # raises
+            idx = d
+        if not t.is_contiguous():
             raise ValueError("expected contiguous tensors")
+    return idx
 
 
 _DTYPES = {torch.float32: cabi.EMK_F32, torch.bfloat16: cabi.EMK_BF16}
@@ -141,8 +151,7 @@ def rmsnorm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     ``hidden = x + residual``, rounded to x's type, is normalised and returned too; ``hidden_out`` may be ``x`` or
     ``residual`` (in place). float32 or bfloat16, any row length. Returns ``(q, scale)`` or ``(q, scale, hidden)``;
     ``scale`` has the shape of ``x`` without its last axis."""
-    idx = _cuda_index(x, weight, residual, out, scale_out, hidden_out)
-    _check_contig(x, weight, residual, out, scale_out, hidden_out)
+    idx = _contiguous_index(x, weight, residual, out, scale_out, hidden_out)
     dtype = _dtype_token(x)
     shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
@@ -540,8 +549,7 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     """LinearOp on 8-bit operands: e4m3 activations ``[..., K]`` with one fp32 scale per row (what :func:`rmsnorm_e4m3`
     returns) times e4m3 weights ``[N, K]`` with one fp32 scale per output channel (those of :func:`linear_w8`), bf16 out.
     K must be a multiple of 16, N of 8."""
-    idx = _cuda_index(x, x_scale, w, w_scale, out)
-    _check_contig(x, x_scale, w, w_scale, out)
+    idx = _contiguous_index(x, x_scale, w, w_scale, out)
     if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
         raise TypeError("linear_e4m3 expects float8_e4m3fn activations and weights")
     if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
@@ -677,8 +685,9 @@ def kv8_append_(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: t
     ``b`` holds ``ctx_lens[b]`` tokens and gets the rows ``cu_seqlens[b]:cu_seqlens[b+1]`` (int32 CUDA tensors ``[B]``
     and ``[B+1]``, left as they are: the caller advances its lengths). No two sequences may write to one page. Scales are
     powers of two and grow with what a page holds (see ``include/emk.h``)."""
-    idx = _cuda_index(*cache, k, v, page_table, ctx_lens, cu_seqlens)
-    _check_contig(*cache, page_table, ctx_lens, cu_seqlens)
+    idx = _contiguous_index(*cache, page_table, ctx_lens, cu_seqlens)
+    if k.get_device() != idx or v.get_device() != idx:
+        _cuda_index(page_table, k, v)  # raises
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, ctx_lens)
     if not (k.dtype is v.dtype is torch.bfloat16):
         raise TypeError("kv8_append_ expects bfloat16 keys and values")
@@ -725,8 +734,9 @@ def sdpa_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, seq_len
     tokens of each sequence with the ``Sq`` new ones already appended. Query ``i`` sees the tokens up to position
     ``seq_lens[b] - Sq + i``; one that sees none (an empty or padding sequence) gets zeros. Sequences may share pages;
     ``out`` may be a contiguous ``q`` itself. Returns bf16 ``[B, Sq, Hq, D]``."""
-    idx = _cuda_index(q, *cache, page_table, seq_lens, out, workspace)
-    _check_contig(*cache, page_table, seq_lens, out, workspace)
+    idx = _contiguous_index(*cache, page_table, seq_lens, out, workspace)
+    if q.get_device() != idx:
+        _cuda_index(page_table, q)  # raises
     pages, Hkv, page, D, B, max_pages = _kv8_sizes(cache, page_table, seq_lens)
     if q.dtype is not torch.bfloat16:
         raise TypeError("sdpa_kv8 expects bfloat16 queries")

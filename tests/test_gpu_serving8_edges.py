@@ -125,3 +125,22 @@ def test_nan_tokens_reach_only_the_queries_that_see_them(ops, room, Sq, G, D):  
     # (to the tolerance, not to the bit: when one row's maximum moves, the others' roundings move with it)
     for some in (ref, torch.where(torch.isnan(got), ref, got)):
         _attend_check(ops, some[:6], q[:6], clean, torch.tensor(rows[:6]), lens[:6], 1 / math.sqrt(D))
+
+
+def test_a_tensor_left_on_the_cpu_is_refused_wherever_it_stands(ops):  # noqa: F811
+    cache = ops.kv8_cache(3, 2, 16, 64)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, lens, cu = torch.zeros(1, 2, **i32), torch.ones(1, **i32), torch.tensor([0, 1], **i32)
+    k = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(2, 16, device="cuda")
+    x8, w8, s2, s8 = x.to(E4M3), torch.zeros(8, 16, device="cuda").to(E4M3), torch.ones(2, device="cuda"), torch.ones(8, device="cuda")
+    calls = [(ops.sdpa_kv8, [q, cache, table, lens]), (ops.kv8_append_, [cache, k, k, table, lens, cu]),
+             (ops.linear_e4m3, [x8, s2, w8, s8]), (ops.rmsnorm_e4m3, [x, torch.ones(16, device="cuda"), 1e-6, x])]
+    for f, args in calls:
+        f(*args)
+        for i, a in enumerate(args):
+            for there in [a.cpu()] if torch.is_tensor(a) else [a._replace(**{n: getattr(a, n).cpu()}) for n in a._fields] if isinstance(a, tuple) else []:
+                with pytest.raises(ValueError):
+                    f(*args[:i], there, *args[i + 1:])
+    ops.device_status()

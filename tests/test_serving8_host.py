@@ -150,6 +150,24 @@ def test_all_tensors_lie_on_one_device(monkeypatch, devices, want):
         assert ops._cuda_index(*tensors) == want
 
 
+@pytest.mark.parametrize("devices,dense,want", [((0, 0), (1, 1), 0), ((3, None, 3), (1, 1, 1), 3), ((0, 1), (1, 1), ValueError),
+                                                ((-1, 0), (1, 1), ValueError), ((0, 0, -1), (1, 1, 1), ValueError),
+                                                ((0, 0), (1, 0), ValueError), ((2, 2, 2), (0, 1, 1), ValueError)])
+def test_contiguous_tensors_lie_on_one_device(monkeypatch, devices, dense, want):
+    from deplodock_b200 import ops
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    tensors = [None if d is None else _On(d) for d in devices]
+    for t, c in zip(tensors, dense):
+        if t is not None:
+            t.is_contiguous = lambda c=c: bool(c)
+    if want is ValueError:
+        with pytest.raises(ValueError):
+            ops._contiguous_index(*tensors)
+    else:
+        assert ops._contiguous_index(*tensors) == want
+
+
 def test_call_runs_on_the_tensors_device_and_its_stream(monkeypatch):
     """The tensors' device need not be the current one; the stream is that device's."""
     import contextlib
