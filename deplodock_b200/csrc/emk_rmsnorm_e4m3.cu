@@ -75,16 +75,28 @@ __device__ __forceinline__ void load_weight(const T* p, float* f) {
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = to_f<T>(a.e[i]);
 }
-// V codes of y * k
+// The codes' factor r / s, as a product: where the scale is at its floor and r is large (a row of zeros with eps = 1e-12: 1e6 / 1.8e-33)
+// it passes fp32's range, and 0 * inf would be NaN. The values lie below 2^-119 there, so they take 2^64 of it first. One more
+// product for all rows: a second store loop for those rows, or a call, cost the others registers (8 x 1024 1.60 -> 1.72 us).
+struct Factor {
+  float first, k;
+};
+__device__ __forceinline__ Factor codes_factor(float r, float s) {
+  constexpr float UP = 1.8446744073709552e19f;  // 2^64
+  const float k = r / s;
+  if (k > 3.402823466e38f) return {UP, r * (1.f / UP) / s};  // (not where k is NaN: those codes are)
+  return {1.f, k};
+}
+// V codes of y * r / s
 template <int V>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float* y, float k) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* y, Factor c) {
   if constexpr (V == 1) {
-    *p = __nv_cvt_float_to_fp8(y[0] * k, __NV_SATFINITE, __NV_E4M3);
+    *p = __nv_cvt_float_to_fp8(y[0] * c.first * c.k, __NV_SATFINITE, __NV_E4M3);
   } else {
     Pack<uint16_t, V / 2> o;
 #pragma unroll
     for (int i = 0; i < V / 2; ++i)
-      o.e[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * k, y[2 * i + 1] * k), __NV_SATFINITE, __NV_E4M3);
+      o.e[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i] * c.first * c.k, y[2 * i + 1] * c.first * c.k), __NV_SATFINITE, __NV_E4M3);
     *reinterpret_cast<Pack<uint16_t, V / 2>*>(p) = o;
   }
 }
@@ -245,7 +257,7 @@ rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint
     }
     const float r = 1.0f / sqrtf(ss * inv_cols + eps);
     const float s = row_scale(amax * r);
-    const float k = r / s;
+    const Factor k = codes_factor(r, s);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int vi = i * TPR + tid;
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(256) rmsnorm_e4m3_long_kernel(const T* x, cons
     __syncthreads();
     const float r = 1.0f / sqrtf(ss / (float)cols + eps);
     const float s = row_scale(amax * r);
-    const float k = r / s;
+    const Factor k = codes_factor(r, s);
     for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += 256 * V) {
       load_weight<T, V>(src + base + c, f);
       load_weight<T, V>(w + c, wv);

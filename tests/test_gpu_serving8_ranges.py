@@ -1,0 +1,47 @@
+"""Ranges of values that the 8-bit serving operators have to hold over: eps far below and rows far above what fp32's squares
+carry, value scales that lie as far apart as appending can leave them. Tolerances are those of ``test_gpu_serving8``."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_serving8 import _attend_check, _check_norm, _gen, _norm_ref, _random_cache, _to, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+#: rows x columns that reach every form of the norm's kernel: threads per row, packs per thread, odd lengths, long rows
+NORM_SIZES = [(9, 64), (7, 1024), (7, 1023), (5, 4096), (3, 16384), (4, 20000), (4, 20011), (1300, 32), (1301, 250), (1290, 256),
+              (1290, 1024), (1290, 2048)]
+
+
+def _norm_case(ops, rows, cols, dtype, eps, with_residual, kinds, seed):  # noqa: F811
+    """Rows of every kind in turn (neighbours share a warp or a CTA); weights of one, so that f * w is exact."""
+    g = _gen(seed + cols)
+    x = torch.randn(rows, cols, generator=g)
+    for i, kind in enumerate(kinds):
+        x[i::len(kinds)] = kind(x[i::len(kinds)])
+    x = x.to(dtype)
+    r = torch.zeros_like(x)
+    if with_residual:
+        r[::len(kinds)] = torch.randn(r[::len(kinds)].shape, generator=g).to(dtype)
+    w = torch.ones(cols, dtype=dtype)
+    args = (x.cuda(), w.cuda(), eps)
+    got = ops.rmsnorm_e4m3(*args, residual=r.cuda()) if with_residual else ops.rmsnorm_e4m3(*args)
+    ops.device_status()
+    return got, _norm_ref(x, w, eps, r if with_residual else None)
+
+
+@pytest.mark.parametrize("rows,cols", NORM_SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("eps", [1e-12, 1e-30])
+def test_rmsnorm_e4m3_rows_of_zeros_and_small_eps(ops, rows, cols, dtype, with_residual, eps):  # noqa: F811
+    """A row of zeros gives zeros, however large 1 / sqrt(eps) is; so small a row that its scale is at the floor keeps its
+    codes."""
+    kinds = [lambda v: v, lambda v: 0 * v, lambda v: v * 2.0 ** -121, lambda v: v * 2.0 ** -135]
+    got, ref = _norm_case(ops, rows, cols, dtype, eps, with_residual, kinds, 1)
+    assert (got[0][1::4].view(torch.uint8) & 0x7f == 0).all()
+    _check_norm(got, ref, terms=cols)
