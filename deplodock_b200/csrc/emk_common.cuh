@@ -409,9 +409,9 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The CTAs of a cluster wait for one another and publish nothing: what they have read from each other's shared memory is in
-// registers that later instructions used. (The arrive of cluster_sync_all waits until the thread's global stores are
-// acknowledged.)
+// The CTAs of a cluster wait for one another and publish nothing. For READS of each other's shared memory only: the values are in
+// registers that later instructions used. A remote store or arrive is not ordered by it and has to have been waited for before.
+// (The arrive of cluster_sync_all waits until the thread's global stores are acknowledged.)
 __device__ __forceinline__ void cluster_sync_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }

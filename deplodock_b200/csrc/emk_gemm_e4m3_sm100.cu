@@ -173,6 +173,14 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
           }
         }
       }
+      // the leader's last releases of this CTA's stages have arrived before it leaves (a stage that was never filled waits for none)
+      for (int i = 0; i < P8_STAGES && ok; ++i) {
+        ok = mbar_wait(&bars->empty[stage], phase ^ 1u, wc, EMK_DEV_TIMEOUT_PRODUCER);
+        if (++stage == P8_STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
     }
   } else if (warp == P8_MMA_WARP) {
     if (leader && lane == 0) {  // MMA issuer
@@ -255,7 +263,9 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
         if (c + 2 >= NC) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&bars->tmem_empty[acc]), 0));
+          // Only where the accumulator is used again, so that the leader's MMA warp waits for every arrive before it leaves: one that
+          // nobody waits for could reach the leader's shared memory after the leader has gone (the last barrier orders nothing).
+          if (lane == 0 && tile + 2 * npairs < ntiles) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&bars->tmem_empty[acc]), 0));
         }
         __syncwarp();  // the buffer's last contents have been read
 #pragma unroll
@@ -285,7 +295,9 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (bars->abort_flag) abort_drain();
-  cluster_sync_relaxed();  // the peer's shared and tensor memory stay alive until the leader's MMAs are done
+  // The peer's shared and tensor memory stay alive until the leader's MMAs are done. Nothing is on its way to another CTA's shared
+  // memory here: arrives and releases have been waited for above.
+  cluster_sync_relaxed();
   if (warp == 0) tmem_dealloc_pair(tmem_base, 512);
 }
 
