@@ -438,8 +438,8 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   }
 
   __syncthreads();
-  if (warp == 0) tmem_dealloc(tmem_base, TMEM_COLS);
   if (bars->abort_flag) abort_drain();
+  if (warp == 0) tmem_dealloc(tmem_base, TMEM_COLS);
   if (split > 1) cluster_sync_all();  // (reached by every thread of every CTA, whatever happened above)
   // CTA `rank` finishes the tokens rank, rank + split, ...: a warp takes a token's 128 columns, four per lane, and adds
   // the cluster's partial sums in the order of the ranks
