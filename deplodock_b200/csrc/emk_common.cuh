@@ -180,7 +180,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // resident while the kernel before it in the stream is still draining: its CTAs run their set-up (barrier
 // initialisation, tensor-memory allocation, descriptor prefetch) and then stop in grid_dependency_wait() until the
 // earlier kernel has completed and its writes are visible. Every global read and write of such a kernel comes after
-// that wait. Launched the ordinary way, both calls do nothing.
+// that wait, but for hints that bring weights into L2. What an earlier kernel of the library may have written is read with
+// ordinary loads: the non-coherent path (__ldg, const __restrict__ parameters) is for data that is read-only for the whole
+// life of the kernel, which begins before the wait. Launched the ordinary way, both calls do nothing.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -239,7 +239,7 @@ gemm2_e4m3_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
       tile_coords(tile, g.tiles_m, g.tiles_n, P8_GROUP_M, tm, tn);
       const int row = tm * 2 * BM + (int)rank * BM + quarter * 32 + lane;
       const int n0 = tn * BN + part * (BN / 4);
-      const float xs = row < g.M ? __ldg(g.x_scale + row) : 0.f;
+      const float xs = row < g.M ? g.x_scale[row] : 0.f;
       float wl[(BN + 127) / 128];  // the columns' scales, one a lane
 #pragma unroll
       for (int c = 0; c < (BN + 127) / 128; ++c) wl[c] = n0 + c * 32 + lane < g.N ? __ldg(g.w_scale + n0 + c * 32 + lane) : 0.f;
@@ -449,7 +449,7 @@ gemm_e4m3_rows_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
     const uint32_t at = smem_u32(part) + (uint32_t)lane * 16u;
     const int tokens = min(NT, g.M - tm * NT);
     for (int tok = (int)rank + (int)split * warp; tok < tokens; tok += (int)split * (R8_THREADS / 32)) {
-      const float xs = __ldg(g.x_scale + tm * NT + tok);
+      const float xs = g.x_scale[tm * NT + tok];
       float4 v[R8_MAX_SPLIT];
 #pragma unroll
       for (uint32_t s = 0; s < R8_MAX_SPLIT; ++s)

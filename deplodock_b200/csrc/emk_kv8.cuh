@@ -14,7 +14,7 @@ __host__ __device__ __forceinline__ bool kv8_page_ok(int64_t page) {
 
 // A page id from the table, made safe: ids outside the pool are clamped into it (recorded in the bounds-check build).
 __device__ __forceinline__ int kv8_page_id(const int* table_row, int64_t slot, int num_pages, int* status) {
-  const int p = __ldg(table_row + slot);
+  const int p = table_row[slot];
   if (p < 0 || p >= num_pages) emk_record_bounds(status, EMK_DEV_BOUNDS_PAGE);
   return min(max(p, 0), num_pages - 1);
 }

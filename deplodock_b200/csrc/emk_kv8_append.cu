@@ -104,7 +104,7 @@ __device__ __forceinline__ void rescale_codes4(uint32_t& c, float ratio) {
 
 // First place of sequence b (see the top): between 0 and items, not falling in b for lengths that do not fall.
 __device__ __forceinline__ int64_t first_place(const AppendArgs& a, int b) {
-  const int64_t t = min(max((int64_t)__ldg(a.cu + b), (int64_t)0), a.T);
+  const int64_t t = min(max((int64_t)a.cu[b], (int64_t)0), a.T);
   return (t >> a.page_shift) + 2 * (int64_t)b;
 }
 

@@ -74,7 +74,7 @@ struct SdpaArgs {
 
 __device__ __forceinline__ int seq_len(const SdpaArgs& a, int b) {
   const int64_t room = (int64_t)a.max_pages << a.page_shift;
-  const int n = __ldg(a.lens + b);
+  const int n = a.lens[b];
   if (n < 0 || n > room) emk_record_bounds(a.status, EMK_DEV_BOUNDS_CACHE_LEN);
   return (int)min((int64_t)max(n, 0), room);
 }
@@ -254,14 +254,14 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
   };
   int unit_now = unit_of(lane), unit_next = unit_of(32 + lane);
   // and the scales of those 32 tiles, for the tiles that are issued and those that are used
-  float ks_issue = __ldg(a.ks + unit_now), vs_issue = __ldg(a.vs + unit_now), ks_use = 0.f, vs_use = 0.f;
+  float ks_issue = a.ks[unit_now], vs_issue = a.vs[unit_now], ks_use = 0.f, vs_use = 0.f;
   auto issue = [&](int i) {
     if (i < nsub) {
       if ((i & 31) == 0 && i > 0) {
         unit_now = unit_next;
         unit_next = unit_of(i + 32 + lane);
-        ks_issue = __ldg(a.ks + unit_now);
-        vs_issue = __ldg(a.vs + unit_now);
+        ks_issue = a.ks[unit_now];
+        vs_issue = a.vs[unit_now];
       }
       const int unit = __shfl_sync(0xffffffffu, unit_now, i & 31);
       if (lane == 0) {
