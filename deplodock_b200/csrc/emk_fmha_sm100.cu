@@ -140,7 +140,7 @@ __device__ __forceinline__ WorkItem decode_item(const FmhaArgs& a, int w) {
     const int per_entry = a.Hkv * a.pairs;
     const int e = w / per_entry;
     int rem = w - e * per_entry;
-    const int4 ent = __ldg(a.vl_items + e);
+    const int4 ent = a.vl_items[e];
     const int pair = rem % a.pairs;
     it.hkv = rem / a.pairs;
     it.b = 0;

@@ -368,11 +368,11 @@ __device__ __forceinline__ void epilogue_drain(const GemmArgs& g, uint32_t taddr
     if (g.ss_in_segs == 8) {
       uint32_t u[8];
       if (g.coherent) ld_global_cg_v8(pr, u);
-      else ld_global_nc_v8(pr, u);
+      else ld_global_v8(pr, u);
       tot = ((__uint_as_float(u[0]) + __uint_as_float(u[1])) + (__uint_as_float(u[2]) + __uint_as_float(u[3]))) +
             ((__uint_as_float(u[4]) + __uint_as_float(u[5])) + (__uint_as_float(u[6]) + __uint_as_float(u[7])));
     } else {
-      for (int sg = 0; sg < g.ss_in_segs; ++sg) tot += g.coherent ? __ldcg(pr + sg) : __ldg(pr + sg);
+      for (int sg = 0; sg < g.ss_in_segs; ++sg) tot += __ldcg(pr + sg);
     }
     rs = 1.0f / sqrtf(tot * g.ss_inv_dim + g.ss_eps);
   }

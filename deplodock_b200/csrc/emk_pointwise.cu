@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(512, 2) qknorm_rope_kernel(__nv_bfloat16* __re
 // One CTA per sequence: RMSNorm of the last token's hidden row, rounded to bf16 like the module output, then L2
 // normalisation in fp32.
 // `cu_seqlens` null: sequence b is rows b*S .. b*S+S-1; else its last row is cu_seqlens[b+1]-1 (packed sequences).
-__global__ void __launch_bounds__(256) pool_norm_l2_kernel(const __nv_bfloat16* __restrict__ hs,
+__global__ void __launch_bounds__(256) pool_norm_l2_kernel(const __nv_bfloat16* hs,
                                                            const __nv_bfloat16* __restrict__ w,
                                                            float* __restrict__ out, int S, int hidden, float eps,
                                                            const int* __restrict__ cu_seqlens) {

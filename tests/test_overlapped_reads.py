@@ -18,6 +18,12 @@ READ_ONLY = {
     "emk_kv8.cuh": set(),
     "emk_kv8_append.cu": set(),
     "emk_rmsnorm_e4m3.cu": {"w"},
+    # a layer's weights, biases and rotary tables; positions, ids and cu_seqlens come from outside the step
+    "emk_gemm_common.cuh": {"g.f32_bias", "g.scale", "g.residual", "g.qk_pos", "wp", "tp"},
+    "emk_gemm2_sm100.cu": set(),
+    "emk_gemm_chain_sm100.cu": set(),
+    "emk_fmha_sm100.cu": {"cu_seqlens"},
+    "emk_pointwise.cu": {"src", "table", "ids", "w", "cu_seqlens", "head", "cosb", "sinb"},
 }
 
 
