@@ -75,18 +75,10 @@ __device__ __forceinline__ void load_weight(const T* p, float* f) {
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = to_f<T>(a.e[i]);
 }
-// The codes' factor r / s, as a product: where the scale is at its floor and r is large (a row of zeros with eps = 1e-12: 1e6 / 1.8e-33)
-// it passes fp32's range, and 0 * inf would be NaN. The values lie below 2^-119 there, so they take 2^64 of it first. One more
-// product for all rows: a second store loop for those rows, or a call, cost the others registers (8 x 1024 1.60 -> 1.72 us).
+// The codes' factor r / s, as a product (row_codes).
 struct Factor {
   float first, k;
 };
-__device__ __forceinline__ Factor codes_factor(float r, float s) {
-  constexpr float UP = 1.8446744073709552e19f;  // 2^64
-  const float k = r / s;
-  if (k > 3.402823466e38f) return {UP, r * (1.f / UP) / s};  // (not where k is NaN: those codes are)
-  return {1.f, k};
-}
 // V codes of y * r / s
 template <int V>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float* y, Factor c) {
@@ -102,6 +94,49 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* y, Factor c
 }
 
 __device__ __forceinline__ float row_scale(float amax) { return max_nan(amax, AMAX_FLOOR) / E4M3_MAX; }
+
+constexpr float FLT_LARGEST = 3.402823466e38f;
+constexpr float UP = 1.8446744073709552e19f;  // 2^64
+constexpr float MEAN_MIN = 1.262177448e-29f;  // 2^-96: below it the squares of a row's values may have vanished
+
+// Whether fp32 holds the mean square + eps of a row (NaN: no).
+__device__ __forceinline__ bool mean_holds(float mean) { return mean >= MEAN_MIN && mean <= FLT_LARGEST; }
+
+// Scale and codes' factor of a row from r = rsqrt(mean square + eps) and the largest |f * w|. Where the scale is at its floor and r
+// is large (a row of zeros with eps = 1e-12: 1e6 / 1.8e-33) r / s passes fp32's range, and 0 * inf would be NaN. The values lie
+// below 2^-119 there, so they take 2^64 of it first. One more product for all rows: a second store loop for those rows, or a
+// call, cost the others registers (8 x 1024 1.60 -> 1.72 us).
+__device__ __forceinline__ float row_codes(float r, float amax, Factor& c) {
+  const float s = row_scale(amax * r);
+  const float k = r / s;
+  const bool large = k > FLT_LARGEST;  // (not where k is NaN: those codes are)
+  c = {large ? UP : 1.f, large ? r * (1.f / UP) / s : k};
+  return s;
+}
+
+// The same for a row whose squares fp32 does not hold: elements from about 2^64 on, or eps and all elements so small that the squares
+// vanish. The squares are summed again of the row times a power of two (2^-80 or 2^96, `half` twice), by every LANES threads
+// for themselves: `row` is x or the stored sum, `lane` this thread's place among them and `mask` they. (The test for such rows costs
+// 8 x 1024 1.50 -> 1.58 us, 32768 x 1024 with a residual nothing.)
+template <typename T, int LANES>
+__device__ __forceinline__ float row_codes_far(const T* row, int64_t cols, float eps, float mean, float amax, int lane, unsigned mask,
+                                               Factor& c) {
+  const bool small = mean < 1.f;
+  const float half = small ? 281474976710656.f : 9.094947017729282e-13f;  // 2^48, 2^-40
+  __syncwarp(mask);  // what the others have stored of the sum is read here
+  float ss = 0.f;
+#pragma unroll 1
+  for (int64_t i = lane; i < cols; i += LANES) {
+    const float v = to_f<T>(row[i]) * half * half;
+    ss = fmaf(v, v, ss);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+  const float r = 1.0f / sqrtf(ss / (float)cols + eps * half * half * half * half);  // times half^2: the row's
+  const float s = row_scale((amax * half) * (r * half));
+  c = {small ? UP : 1.f, r * half * (small ? 1.f / UP : 1.f) / s * half};
+  return s;
+}
 
 // 16 bytes of a row, kept as they are loaded (a bf16 pack that the compiler takes apart costs a register an element).
 template <typename T>
@@ -255,9 +290,12 @@ rmsnorm_e4m3_kernel(const T* x, const T* residual, const T* __restrict__ w, uint
       }
       turn ^= 1;
     }
-    const float r = 1.0f / sqrtf(ss * inv_cols + eps);
-    const float s = row_scale(amax * r);
-    const Factor k = codes_factor(r, s);
+    const float mean = ss * inv_cols + eps;
+    Factor k;
+    float s = row_codes(1.0f / sqrtf(mean), amax, k);
+    if (!mean_holds(mean) && row < rows)
+      s = row_codes_far<T, LANES>((RES ? hidden : x) + base, cols, eps, mean, amax, lane % LANES,
+                                  (0xffffffffu >> (32 - LANES)) << (lane / LANES * LANES), k);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int vi = i * TPR + tid;
@@ -332,9 +370,10 @@ __global__ void __launch_bounds__(256) rmsnorm_e4m3_long_kernel(const T* x, cons
       amax = max_nan(amax, red_max[i]);
     }
     __syncthreads();
-    const float r = 1.0f / sqrtf(ss / (float)cols + eps);
-    const float s = row_scale(amax * r);
-    const Factor k = codes_factor(r, s);
+    const float mean = ss / (float)cols + eps;
+    Factor k;
+    float s = row_codes(1.0f / sqrtf(mean), amax, k);
+    if (!mean_holds(mean)) s = row_codes_far<T, 32>(src + base, cols, eps, mean, amax, lane, 0xffffffffu, k);
     for (int64_t c = (int64_t)threadIdx.x * V; c < cols; c += 256 * V) {
       load_weight<T, V>(src + base + c, f);
       load_weight<T, V>(w + c, wv);

@@ -45,3 +45,39 @@ def test_rmsnorm_e4m3_rows_of_zeros_and_small_eps(ops, rows, cols, dtype, with_r
     got, ref = _norm_case(ops, rows, cols, dtype, eps, with_residual, kinds, 1)
     assert (got[0][1::4].view(torch.uint8) & 0x7f == 0).all()
     _check_norm(got, ref, terms=cols)
+
+
+@pytest.mark.parametrize("rows,cols", NORM_SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_rmsnorm_e4m3_rows_whose_squares_pass_fp32(ops, rows, cols, dtype, with_residual):  # noqa: F811
+    def one_huge(v):
+        v[:, v.shape[1] // 2] = 3e38
+        return v
+
+    kinds = [lambda v: v, lambda v: v * 1e25, one_huge, lambda v: v * 1e18, lambda v: v * 1e37]
+    got, ref = _norm_case(ops, rows, cols, dtype, 1e-6, with_residual, kinds, 2)
+    _check_norm(got, ref, terms=cols)
+
+
+@pytest.mark.parametrize("rows,cols", NORM_SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-38])
+def test_rmsnorm_e4m3_rows_whose_squares_vanish(ops, rows, cols, dtype, with_residual, eps):  # noqa: F811
+    kinds = [lambda v: v, lambda v: v * 1e-25, lambda v: v * 1e-30, lambda v: v * 1e-20, lambda v: v * 1e-36]
+    got, ref = _norm_case(ops, rows, cols, dtype, eps, with_residual, kinds, 3)
+    _check_norm(got, ref, terms=cols)
+
+
+@pytest.mark.parametrize("cols", [64, 1023, 1024, 20000])
+def test_rmsnorm_e4m3_non_finite_rows_stay_nan(ops, cols):  # noqa: F811
+    x = torch.randn(1300, cols, generator=_gen(4))
+    x[1::4, cols // 3] = float("inf")
+    x[2::4, 0] = float("nan")
+    x[3::4, :2] = torch.tensor([float("-inf"), 3e38])
+    q, scale = ops.rmsnorm_e4m3(x.cuda(), torch.ones(cols).cuda(), 1e-6)
+    bad = torch.isnan(q.float()).all(1).cpu()
+    assert bad[1::4].all() and bad[2::4].all() and bad[3::4].all() and not bad[::4].any()
+    assert torch.equal(torch.isnan(scale).cpu(), bad)
+    assert torch.isfinite(q[::4].float()).all()
