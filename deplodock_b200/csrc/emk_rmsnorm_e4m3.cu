@@ -93,9 +93,12 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* y, Factor c
   }
 }
 
-__device__ __forceinline__ float row_scale(float amax) { return max_nan(amax, AMAX_FLOOR) / E4M3_MAX; }
-
 constexpr float FLT_LARGEST = 3.402823466e38f;
+// (NaN where the largest value passes fp32's range: an infinite scale would leave zero codes)
+__device__ __forceinline__ float row_scale(float amax) {
+  return amax <= FLT_LARGEST ? fmaxf(amax, AMAX_FLOOR) / E4M3_MAX : __uint_as_float(0x7fc00000u);
+}
+
 constexpr float UP = 1.8446744073709552e19f;  // 2^64
 constexpr float MEAN_MIN = 1.262177448e-29f;  // 2^-96: below it the squares of a row's values may have vanished
 

@@ -112,7 +112,8 @@ int emk_softmax_lastdim(emk_handle_t h, const void* x, void* y, int64_t rows, in
 /* RMSNorm with the residual's addition and an e4m3 output with one scale per row, for the 8-bit linear layers:
  *   f = x, or with a residual f = round(x + residual) to `dtype`, stored to hidden (the new residual stream);
  *   y = f * rsqrt(mean(f^2) + eps) * w in fp32;  scale[row] = max(max |y|, 2^-100) / 448;  q = e4m3(y / scale[row]).
- * A row with a NaN or an infinity (or a product f * w past fp32's range) becomes NaN codes with a NaN scale.
+ * A row with a NaN or an infinity, or one in which f * w or a normalised value passes fp32's range, becomes NaN codes with a
+ * NaN scale.
  * Every finite row is normalised, also where its squares lie outside fp32's range; a row of zeros gives zero codes for any
  * eps > 0 and NaN for eps = 0 (0 / 0).
  * x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or EMK_BF16), residual and hidden both given or both NULL;

@@ -81,3 +81,30 @@ def test_rmsnorm_e4m3_non_finite_rows_stay_nan(ops, cols):  # noqa: F811
     assert bad[1::4].all() and bad[2::4].all() and bad[3::4].all() and not bad[::4].any()
     assert torch.equal(torch.isnan(scale).cpu(), bad)
     assert torch.isfinite(q[::4].float()).all()
+
+
+@pytest.mark.parametrize("rows,cols", NORM_SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rmsnorm_e4m3_products_past_fp32_are_nan_rows(ops, rows, cols, dtype):  # noqa: F811
+    """Where f * w, or the normalised value itself, passes fp32's range: NaN codes and a NaN scale, and its neighbours are right."""
+    x = torch.randn(rows, cols, generator=_gen(8)).to(dtype)
+    w = torch.ones(cols, dtype=dtype)
+    w[cols // 2] = 1e30
+    x[:, cols // 2] = 1e-30
+    x[1::3, cols // 2] = 1e12  # f * w
+    x[2::3] *= 1e-20
+    x[2::3, cols // 2] = 1e-3  # 1e30 sqrt(cols) once normalised
+    q, scale = ops.rmsnorm_e4m3(x.cuda(), w.cuda(), 1e-30)
+    far = torch.tensor([i % 3 == 1 for i in range(rows)])
+    assert torch.equal(torch.isnan(scale).cpu(), far) and torch.isnan(q[far.cuda()].float()).all()
+    ok = ~far
+    y, s, _ = _norm_ref(x, w, 1e-30, None)
+    _check_norm((q.cpu()[ok], scale.cpu()[ok]), (y[ok], s[ok], None), terms=cols)
+    # weights so large that a normalised value of more than one passes the range: a lone element's is sqrt(cols)
+    w[:] = 3e38
+    v = torch.zeros(rows, cols, dtype=dtype)
+    v[:, 0] = 1e-3
+    v[::2, 1:] = 1e-3
+    q, scale = ops.rmsnorm_e4m3(v.cuda(), w.cuda(), 1e-12)
+    assert torch.equal(torch.isnan(scale).cpu(), torch.tensor([i % 2 == 1 for i in range(rows)]))
+    assert torch.isnan(q[1::2].float()).all() and not torch.isnan(q[::2].float()).any()
