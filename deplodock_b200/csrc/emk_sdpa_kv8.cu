@@ -49,7 +49,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float P_SHIFT = 8.f;   // p is rounded as 2^8 p relative to the running maximum ...
 constexpr float P_LIMIT = 15.f;  // ... which moves when a logit is more than 7 above it: the rounded p is at most 2^15
 constexpr float BIG = 65536.f;   // from here on fp32 logits are so coarse that their differences need a clamp
-constexpr float V_SCALE_MIN = 7.888609052210118e-31f;  // 2^-100: a zero scale (a page of zeros) has a logarithm
+constexpr float V_SCALE_MIN = 7.888609052210118e-31f;  // 2^-100: a zero scale (a page of zeros) has a logarithm, and smaller ones count as zero
 
 struct SdpaArgs {
   const __nv_bfloat16* q;
@@ -473,12 +473,12 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
         w[u][1] = v.y;
       }
     }
-    // What lies behind the sequence's end counts as zeros, and so does a page whose scale is zero: its tokens count in the sum and
-    // add nothing.
-    if ((ta + i) * SK_TILE + SK_TILE > len || vs_raw == 0.f) {
+    // What lies behind the sequence's end counts as zeros, and so does a page whose scale is zero or below the smallest that the
+    // shift holds: its tokens count in the sum and add nothing.
+    if ((ta + i) * SK_TILE + SK_TILE > len || vs_raw < V_SCALE_MIN) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len && vs_raw != 0.f;
+        const bool in = (ta + i) * SK_TILE + ((u & 1) == 0 ? tv0 : tv1) + (u >> 1) * 8 < len && !(vs_raw < V_SCALE_MIN);
 #pragma unroll
         for (int j = 0; j < L::V_BYTES / 4; ++j) w[u][j] = in ? w[u][j] : 0u;
       }

@@ -297,7 +297,7 @@ int emk_sdpa_causal_gqa_bf16_varlen(emk_handle_t h, const void* q, const void* k
  * Sequences may share pages. Whatever lies in a page behind a sequence's last token is not used, and a query's result
  * does not depend on the tokens behind its position, NaN among them. Probabilities times value scales are rounded to 11
  * bits, and what is below 2^-33 of a row's largest is lost; sums are fp32. Scales must be finite and not negative; a
- * zero value scale makes a page's values zero. Lengths are clamped to what max_pages pages hold, page
+ * value scale below 2^-100, zero among them, makes a page's values zero. Lengths are clamped to what max_pages pages hold, page
  * ids to the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
  * emk_sdpa_kv8_workspace_bytes(h, B, Sq, Hq, Hkv, max_pages * page, D) bytes (0, and NULL, where no sequence can be long),
  * not used between calls; calls that may overlap need one each. The first call for a head dimension, for one or several

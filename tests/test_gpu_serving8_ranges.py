@@ -108,3 +108,40 @@ def test_rmsnorm_e4m3_products_past_fp32_are_nan_rows(ops, rows, cols, dtype):  
     q, scale = ops.rmsnorm_e4m3(v.cuda(), w.cuda(), 1e-12)
     assert torch.equal(torch.isnan(scale).cpu(), torch.tensor([i % 2 == 1 for i in range(rows)]))
     assert torch.isnan(q[1::2].float()).all() and not torch.isnan(q[::2].float()).any()
+
+
+#: batch, longest sequence and room of the page table for the ways to share the work: a warp a row, clusters of small CTAs,
+#: clusters of SM-sized CTAs, the list of tiles
+WAYS = [(300, 80, "tight"), (40, 300, "tight"), (2, 900, "tight"), (3, 900, 1 << 20)]
+
+
+def _spread(ops, B, longest, room, Sq, G, D, exponents, order, seed, Hkv=2, page=16):  # noqa: F811
+    """Sequences whose pages have value scales 2^e, e of ``exponents`` in the given order; queries so small that all pages weigh
+    alike in the sum. Returns the output and what ``_attend_check`` takes, of the first sequences."""
+    g = _gen(seed)
+    max_pages = -(-longest // page)
+    lens = torch.randint(Sq, longest + 1, (B,), generator=g).int()
+    lens[0] = longest
+    table = torch.randperm(B * max_pages, generator=g).view(B, max_pages).int()
+    cache = _random_cache(ops, B * max_pages, Hkv, page, D, seed)
+    e = torch.tensor(exponents)[torch.randint(len(exponents), (B, max_pages, Hkv), generator=g)]
+    if order != "mixed":
+        e = e.sort(1, descending=order == "falling").values
+    cache.v_scale[table.long()] = torch.exp2(e.double()).float()
+    q = (0.05 * torch.randn(B, Sq, G * Hkv, D, generator=g)).bfloat16()
+    wide = table if room == "tight" else torch.cat([table, torch.full((B, room // page - max_pages), -1, dtype=torch.int32)], 1)
+    out = ops.sdpa_kv8(q.cuda(), _to(cache, "cuda"), wide.cuda(), lens.cuda())
+    ops.device_status()
+    n = min(B, 6)
+    return out[:n], q[:n], cache, table[:n], lens[:n].tolist()
+
+
+@pytest.mark.parametrize("B,longest,room", WAYS)
+@pytest.mark.parametrize("Sq,G,D", [(1, 2, 128), (1, 4, 64), (4, 4, 128), (3, 2, 64)])
+def test_value_scales_too_small_to_matter_count_as_zero(ops, B, longest, room, Sq, G, D):  # noqa: F811
+    out, q, cache, table, lens = _spread(ops, B, longest, room, Sq, G, D, [-120], "mixed", 5)
+    assert (out == 0).all()
+    # beside others they weigh in the sum as pages of zeros do
+    out, q, cache, table, lens = _spread(ops, B, longest, room, Sq, G, D, [-120, -3], "mixed", 6)
+    cache.v_scale[cache.v_scale < 2.0 ** -100] = 0.0
+    _attend_check(ops, out, q, cache, table, lens, 1 / math.sqrt(D))
