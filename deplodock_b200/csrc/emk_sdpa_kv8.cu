@@ -18,11 +18,14 @@
 //   V fragment: lane (g, t) holds tokens p(2t), p(2t+1), 8 + both, channels (D/8) g..       (pairs interleaved by prmt)
 // P^T comes out of S^T by movmatrix.
 //
-// e4m3 -> f16 is exact. q is scaled per row by a power of two into f16's range (exact; elements 2^-38 below the row's
-// largest may lose bits, far below the fp32 sum's own rounding). The scales of keys go into the logits; the scale of
-// values cannot multiply the probabilities directly (f16's range), so the running maximum is kept over logit +
-// log2(v_scale) and p * v_scale / max is what is rounded to f16 (2^-12 relative: p in [0, 2^15], so 2^-29 of the largest
-// contribution is still normal), while the sum of the probabilities divides that scale out again in fp32.
+// e4m3 -> f16 is exact. q is scaled per row by a power of two into f16's range: exact for elements down to 2^-31 of the row's
+// largest; smaller ones are off by 2^-39 of that largest at most, far below the fp32 sum's own rounding. The
+// scales of keys go into the logits; the scale of values cannot multiply the probabilities directly (f16's range), so the running
+// maximum is kept over logit + log2(v_scale). A term of the sum is 2^(logit - maximum) in fp32; the term times its page's value
+// scale, 2^8 at the maximum (up to 2^15 before that moves), is rounded to f16: off by 2^-11 relative at most down to 2^-22 of the
+// row's largest, by 2^-33 of that largest below. That rounding is what lets the matrix instruction run in f16;
+// the sum does not see it. The sum keeps a page however far its value scale lies below another's: its terms do not pass through
+// the scaled probability, and where the maximum moves it is multiplied in two steps (decay).
 //
 // Four kernels share the loop. Many rows of few tiles (short_rows): a warp each. Where no sequence can be long (split_of): a
 // cluster of CTAs takes a row tile, deals its tiles to its warps and joins their pieces in distributed shared memory, the
@@ -49,7 +52,12 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float P_SHIFT = 8.f;   // p is rounded as 2^8 p relative to the running maximum ...
 constexpr float P_LIMIT = 15.f;  // ... which moves when a logit is more than 7 above it: the rounded p is at most 2^15
 constexpr float BIG = 65536.f;   // from here on fp32 logits are so coarse that their differences need a clamp
-constexpr float V_SCALE_MIN = 7.888609052210118e-31f;  // 2^-100: a zero scale (a page of zeros) has a logarithm, and smaller ones count as zero
+constexpr float V_SCALE_MIN = 7.888609052210118e-31f;  // 2^-100: smaller value scales, zero among them, count as zero
+// The sum's terms are 2^SUM_SHIFT times larger than the probabilities relative to the maximum, and no page's value scale is taken
+// as less than 2^V_LOG_MIN in that maximum: so neither a term, at most 2^(15 + 20 + 68) and 2^24 of them a lane, nor a probability
+// under the largest scale that appending makes (2^120) leaves fp32's normal range.
+constexpr float SUM_SHIFT = 20.f, SUM_UNIT = 9.5367431640625e-07f;  // 2^-20
+constexpr float V_LOG_MIN = -68.f;
 
 struct SdpaArgs {
   const __nv_bfloat16* q;
@@ -92,10 +100,10 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float rcp(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+// l * 2^d for d <= 0, in two steps: a sum of small value scales next to a maximum of a large one (2^184 apart by appending, so is l)
+__device__ __forceinline__ float decay(float l, float d) {
+  const float half = ex2(0.5f * d);
+  return l * half * half;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -383,18 +391,18 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
         for (int x = 0; x < 4; ++x) s[n][x] = s2[n][0][x] + s2[n][1][x];
       }
     }
-    const float vs = max_nan(vs_raw, V_SCALE_MIN);
-    const float lvs = lg2(vs);
+    const float lvs = fmaxf(lg2(vs_raw), V_LOG_MIN);
+    const float x_limit = P_LIMIT + SUM_SHIFT - lvs;
     const int tok = (ta + i) * SK_TILE + tk;
     const bool edge = (ta + i) * SK_TILE + SK_TILE > limit_min;  // some row does not see all of the tile
-    // p[n][2 u + e]: row n * 8 + 2 t + e, token tok + 8 u. A row that has seen nothing yet has an infinite shift: its
-    // first visible logit makes the maximum move.
+    // p[n][2 u + e]: row n * 8 + 2 t + e, token tok + 8 u: logit - maximum + SUM_SHIFT + P_SHIFT, the sum's term, the
+    // probability. A row that has seen nothing yet has an infinite shift: its first visible logit makes the maximum move.
     float p[RT][4];
     auto exponents = [&]() {
 #pragma unroll
       for (int n = 0; n < RT; ++n) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) p[n][x] = fmaf(s[n][x], qs[n][x & 1] * ks, lvs + shift[n][x & 1]);
+        for (int x = 0; x < 4; ++x) p[n][x] = fmaf(s[n][x], qs[n][x & 1] * ks, shift[n][x & 1]);
         if (edge) {
 #pragma unroll
           for (int x = 0; x < 4; ++x)
@@ -406,7 +414,7 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
     float most = -INFINITY;
 #pragma unroll
     for (int n = 0; n < RT; ++n) most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])));
-    if (__any_sync(0xffffffffu, most > P_LIMIT)) {  // rare after a row's first tiles: no shuffles otherwise
+    if (__any_sync(0xffffffffu, most > x_limit)) {  // rare after a row's first tiles: no shuffles otherwise
       big = false;
 #pragma unroll
       for (int n = 0; n < RT; ++n) {
@@ -422,9 +430,9 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const float to = fmaxf(part.m[n][e], mx);
           f[e] = part.m[n][e] == -INFINITY ? 0.f : ex2(part.m[n][e] - to);
+          part.l[n][e] = part.m[n][e] == -INFINITY ? part.l[n][e] * 0.f : decay(part.l[n][e], part.m[n][e] - to);
           part.m[n][e] = to;
-          shift[n][e] = P_SHIFT - to;
-          part.l[n][e] *= f[e];
+          shift[n][e] = P_SHIFT + SUM_SHIFT - to;
           big = big || (to != -INFINITY && fabsf(to) > BIG);
         }
 #pragma unroll
@@ -442,17 +450,19 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
 #pragma unroll
       for (int n = 0; n < RT; ++n) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) p[n][x] = p[n][x] > P_LIMIT ? P_LIMIT : p[n][x];
+        for (int x = 0; x < 4; ++x) p[n][x] = p[n][x] > x_limit ? x_limit : p[n][x];
       }
     }
-    const float inv_vs = rcp(vs);
+    const float weight = vs_raw * SUM_UNIT;
     uint32_t pb[RT][2];  // P^T: row g, tokens 2 t, 2 t + 1 (+ 8)
 #pragma unroll
     for (int n = 0; n < RT; ++n) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) p[n][x] = ex2(p[n][x]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) part.l[n][e] = fmaf(p[n][e] + p[n][2 + e], inv_vs, part.l[n][e]);
+      for (int e = 0; e < 2; ++e) part.l[n][e] += p[n][e] + p[n][2 + e];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) p[n][x] *= weight;
 #pragma unroll
       for (int u = 0; u < 2; ++u) pb[n][u] = transpose8x8(pack_f16x2(p[n][2 * u], p[n][2 * u + 1]));
     }
@@ -495,6 +505,11 @@ __device__ __forceinline__ bool row_part(const SdpaArgs& a, const CUtensorMap& t
         for (int n = 0; n < RT; ++n) mma_f16(part.o[n][j * 2 + half], a0, a1, a2, a3, pb[n][0], pb[n][1]);
       }
     }
+  }
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) part.l[n][e] *= SUM_UNIT;
   }
   return true;
 }
@@ -676,7 +691,7 @@ __global__ void __launch_bounds__(SK_THREADS, SkLayout<D, RT>::CTAS_PER_SM) sdpa
       for (int w = w0; w < w1; ++w) {
         // a piece without a visible token has -inf here, zeros (or, through a NaN, NaN) in its sums
         const float f = s_m[w][row] == -INFINITY ? 1.f : ex2(s_m[w][row] - top);
-        sum = fmaf(s_l[w][row], f, sum);
+        sum += s_m[w][row] == -INFINITY ? s_l[w][row] : decay(s_l[w][row], s_m[w][row] - top);
         const float* from = reinterpret_cast<const float*>(smem + w * L::WARP_RING) + row * L::PIECE_PITCH + col;
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
@@ -884,7 +899,7 @@ sdpa_kv8_rows_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     const unsigned holds = __ballot_sync(0xffffffffu, m != -INFINITY || l != 0.f);  // (a NaN sum counts)
     const float top = warp_max(m);
     const float f = m == -INFINITY ? 1.f : ex2(m - top);
-    const float sum = warp_sum(l * f);
+    const float sum = warp_sum(m == -INFINITY ? l : decay(l, m - top));
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -1033,7 +1048,7 @@ sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     const unsigned holds = __ballot_sync(0xffffffffu, m != -INFINITY || l != 0.f);  // (a NaN sum counts)
     const float top = warp_max(m);
     const float f = m == -INFINITY ? 1.f : ex2(m - top);
-    const float sum = warp_sum(l * f);
+    const float sum = warp_sum(m == -INFINITY ? l : decay(l, m - top));
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -1067,7 +1082,7 @@ sdpa_kv8_wide_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_con
     }
     const float top = warp_max(m);
     const float f = m == -INFINITY ? (l != 0.f ? 1.f : 0.f) : ex2(m - top);
-    const float sum = warp_sum(l * f);
+    const float sum = warp_sum(m == -INFINITY ? l : decay(l, m - top));
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -1147,9 +1162,9 @@ __global__ void __launch_bounds__(WARPS * 32) sdpa_kv8_join_kernel(const SdpaArg
       s_f[i] = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);
     }
     const float keep = m == -INFINITY ? 1.f : ex2(m - top);
-    m = top;
     // each thread adds its own place's sum; the warps share the outputs out
-    l = fmaf(l, keep, holds ? ml.y * (ml.x == -INFINITY ? 1.f : ex2(ml.x - top)) : 0.f);
+    l = (m == -INFINITY ? l : decay(l, m - top)) + (holds ? (ml.x == -INFINITY ? ml.y : decay(ml.y, ml.x - top)) : 0.f);
+    m = top;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= keep;
     __syncthreads();

@@ -295,10 +295,11 @@ int emk_sdpa_causal_gqa_bf16_varlen(emk_handle_t h, const void* q, const void* k
  * sees the tokens up to itself; a query that sees none gets zeros. q: bf16, row (b * Sq + i) of pitch ld_q elements,
  * head h at column h * D; o: bf16 [B * Sq][Hq * D], which may be q itself where ld_q is Hq * D; Hq a multiple of Hkv.
  * Sequences may share pages. Whatever lies in a page behind a sequence's last token is not used, and a query's result
- * does not depend on the tokens behind its position, NaN among them. Probabilities times value scales are rounded to 11
- * bits, and what is below 2^-33 of a row's largest is lost; sums are fp32. Scales must be finite and not negative; a
- * value scale below 2^-100, zero among them, makes a page's values zero. Lengths are clamped to what max_pages pages hold, page
- * ids to the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
+ * does not depend on the tokens behind its position, NaN among them. Probabilities times value scales are rounded to
+ * fp16 (off by 2^-11 relative at most down to 2^-22 of a row's largest, by 2^-33 of that largest below); logits and sums
+ * are fp32. Scales must be finite and not negative. Value scales of one sequence may lie any way apart; one below 2^-90
+ * costs its page bits, and one below 2^-100, zero among them, makes a page's values zero. Lengths are clamped to what
+ * max_pages pages hold, page ids to the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
  * emk_sdpa_kv8_workspace_bytes(h, B, Sq, Hq, Hkv, max_pages * page, D) bytes (0, and NULL, where no sequence can be long),
  * not used between calls; calls that may overlap need one each. The first call for a head dimension, for one or several
  * query tokens and for up to or over 8 queries x heads a KV head on a device sets the kernels' shared-memory attributes:

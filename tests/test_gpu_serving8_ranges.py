@@ -145,3 +145,12 @@ def test_value_scales_too_small_to_matter_count_as_zero(ops, B, longest, room, S
     out, q, cache, table, lens = _spread(ops, B, longest, room, Sq, G, D, [-120, -3], "mixed", 6)
     cache.v_scale[cache.v_scale < 2.0 ** -100] = 0.0
     _attend_check(ops, out, q, cache, table, lens, 1 / math.sqrt(D))
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+@pytest.mark.parametrize("B,longest,room", WAYS)
+@pytest.mark.parametrize("Sq,G,D", [(1, 2, 128), (1, 4, 64), (4, 4, 128), (3, 2, 64)])
+@pytest.mark.parametrize("exponents", [(-64, 110), (-64, -20, 40, 100), (70, 110)])
+def test_pages_of_any_value_scale_weigh_in_the_sum(ops, order, B, longest, room, Sq, G, D, exponents):  # noqa: F811
+    """A page whose values are too small to be seen beside another's still takes its share of the probability."""
+    _attend_check(ops, *_spread(ops, B, longest, room, Sq, G, D, list(exponents), order, 7), 1 / math.sqrt(D))
