@@ -55,7 +55,7 @@ constexpr float BIG = 65536.f;   // from here on fp32 logits are so coarse that 
 constexpr float V_SCALE_MIN = 7.888609052210118e-31f;  // 2^-100: smaller value scales, zero among them, count as zero
 // The sum's terms are 2^SUM_SHIFT times larger than the probabilities relative to the maximum, and no page's value scale is taken
 // as less than 2^V_LOG_MIN in that maximum: so neither a term, at most 2^(15 + 20 + 68) and 2^24 of them a lane, nor a probability
-// under the largest scale that appending makes (2^120) leaves fp32's normal range.
+// under the largest scale that appending makes (2^120) leaves fp32's normal range. (Appending makes none below 2^-64.)
 constexpr float SUM_SHIFT = 20.f, SUM_UNIT = 9.5367431640625e-07f;  // 2^-20
 constexpr float V_LOG_MIN = -68.f;
 

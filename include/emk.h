@@ -115,7 +115,7 @@ int emk_softmax_lastdim(emk_handle_t h, const void* x, void* y, int64_t rows, in
  * A row with a NaN or an infinity, or one in which f * w or a normalised value passes fp32's range, becomes NaN codes with a
  * NaN scale.
  * Every finite row is normalised, also where its squares lie outside fp32's range; a row of zeros gives zero codes for any
- * eps > 0 and NaN for eps = 0 (0 / 0).
+ * eps > 0 and NaN for eps = 0 (0 / 0). Products f * w below 2^-126 have fp32's subnormal precision.
  * x, residual, hidden: [rows, cols] of `dtype` (EMK_F32 or EMK_BF16), residual and hidden both given or both NULL;
  * hidden may be x or residual itself (in place), q may alias nothing. w: [cols] of `dtype`; q: [rows, cols] e4m3;
  * scale: fp32 [rows]. Any cols; pointers that are 16-byte aligned (q 8-byte) take the vector path. No counterpart in
@@ -297,9 +297,10 @@ int emk_sdpa_causal_gqa_bf16_varlen(emk_handle_t h, const void* q, const void* k
  * Sequences may share pages. Whatever lies in a page behind a sequence's last token is not used, and a query's result
  * does not depend on the tokens behind its position, NaN among them. Probabilities times value scales are rounded to
  * fp16 (off by 2^-11 relative at most down to 2^-22 of a row's largest, by 2^-33 of that largest below); logits and sums
- * are fp32. Scales must be finite and not negative. Value scales of one sequence may lie any way apart; one below 2^-90
- * costs its page bits, and one below 2^-100, zero among them, makes a page's values zero. Lengths are clamped to what
- * max_pages pages hold, page ids to the pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
+ * are fp32. Scales must be finite and not negative. Value scales of one sequence may lie any way apart. Where all
+ * of a row's lie below 2^-68 (emk_kv8_append makes none below 2^-64) the two fp16 borders rise by as many bits, and one below
+ * 2^-100, zero among them, makes a page's values zero. Lengths are clamped to what max_pages pages hold, page ids to the
+ * pool; entries of page_table behind a sequence's pages are not read. `workspace`: device, 16-byte aligned,
  * emk_sdpa_kv8_workspace_bytes(h, B, Sq, Hq, Hkv, max_pages * page, D) bytes (0, and NULL, where no sequence can be long),
  * not used between calls; calls that may overlap need one each. The first call for a head dimension, for one or several
  * query tokens and for up to or over 8 queries x heads a KV head on a device sets the kernels' shared-memory attributes:
