@@ -11,9 +11,9 @@
 // (they may alias), 8 to 256 threads share a row so that none holds more than four 16-byte packs, and rows of any length at
 // any offset go through the same packs, taken at the aligned places of the whole array with the row's ends masked.
 // Measured at 32768 x 1024 bf16 with a residual (235 MB): two reductions and loads behind stores 55.8 us, loads first 45.1,
-// this form 39.9 (0.90 of the copy bandwidth); 32768 x 1001 (their weights still go element by element): 83.7 us element by
-// element, 49.0 in packs; the same in fp32 without a residual: 50.6 us, 45.0 with four CTAs per SM (a few registers spilled)
-// and the odd elements' weights loaded with them.
+// this form 39.4 (0.91 of the copy bandwidth); 32768 x 1001 (their weights still go element by element): 83.7 us element by
+// element, 50.2 in packs; the same in fp32 without a residual: 50.6 us, 40.1 with four CTAs per SM and the odd elements'
+// weights loaded with them.
 // Launched under the tail of the kernel before it, as all kernels of the serving step: a layer of two norms, three linears
 // and one token's append and attention takes 30.4 us so, 35.0 one after the other (512-token prompts gain nothing).
 #include "emk_common.cuh"
@@ -166,7 +166,8 @@ struct Raw<__nv_bfloat16> {
   }
 };
 
-// CTAs per SM: as many as hold the row's packs without spilling (a few registers where there is no alignment to use).
+// CTAs per SM: as many as hold a row's packs in registers, but for a few words: the kernels of four packs in bf16 keep 8 to 32 bytes
+// a thread in local memory (none or 8 where rows are aligned), those of eight packs 56 to 124 (fp32: 8 or none).
 template <int NV, bool RAGGED, bool RES>
 constexpr int NORM_CTAS = RAGGED ? (RES || NV == 8 ? 2 : 4) : NV == 8 ? (RES ? 2 : 3) : NV == 4 ? (RES ? 3 : 4) : 5;
 
@@ -403,7 +404,7 @@ int launch_rows(emk_handle_t h, const T* x, const T* residual, const T* w, uint8
 
 // Threads per row: as few as hold it in four packs each where there are rows for all SMs (short chains of reductions, many
 // rows in flight), a whole CTA of more than 128 packs where there are not (the row's latency counts: 64 x 4096 bf16 with a
-// residual 2.5 us, with half a CTA a row 3.3; 1024 x 4096 7.7 and 9.0).
+// residual 2.2 us, with half a CTA a row 3.3; 1024 x 4096 7.7 and 9.0).
 template <typename T, bool RAGGED>
 int launch_packs(emk_handle_t h, const T* x, const T* residual, const T* w, uint8_t* q, float* scale, T* hidden, int64_t rows,
                  int cols, float eps, cudaStream_t s) {
